@@ -279,6 +279,95 @@ rl_status rl_specdec_verify(rl_sampler* h, const float* logits, int B, int V, in
                             const float* draw_u, int32_t* out_accepted, int32_t* out_tok, void* stream);
 
 /*
+ * Verification of drafted tokens against the target's probabilities
+ * (speculative sampling): the tokens that come out are distributed as the
+ * target's own samples are. The reference's verify_and_accept (rl_specdec_verify
+ * above) compares the target's probability with itself; these take both models'
+ * rows.
+ *
+ * rl_dist_rows -- rows of categorical distributions over V ids. Row r is
+ * softmax(x / T) over its kept ids, x at element r * ld:
+ *   temperature[B]  one per sequence (NULL: 1). T <= 0: all of the row's
+ *                   probability is on its largest kept logit, the lowest id on
+ *                   ties. A non-finite T is an error of the sequence.
+ *   mask            bit-packed allowed ids, a row per logits row (nullable);
+ *                   a row with no bit set allows every id. Masked ids are not
+ *                   looked at: NaN and infinities are allowed there.
+ *   cut             id of the last entry that a top-k / top-p cutoff keeps, in
+ *                   (logit desc, id asc) order: ids behind it have
+ *                   probability 0. One int32 per logits row at
+ *                   cut[r * cut_stride] (NULL, or an id outside [0, V): no
+ *                   cutoff). rl_sample_batch_debug gives it (out_cut + 2 at
+ *                   stride 3) for the rows as they are passed here.
+ *   first_row[B]    the sequence's first row (NULL: sequences follow one
+ *                   another at the widest number of rows); `rows` is the
+ *                   number of rows that may be read.
+ * -inf logits have probability 0. Weights below 2^-126 of the row's largest
+ * count as 0. 1e-30 and 3e38 bound 1 / T.
+ *
+ * rl_specdec_verify_draft -- a chain. Sequence b has n_draft[b] in [0,
+ * max_draft] drafts drafts[b, i], target rows first_row + 0 .. n_draft and
+ * draft rows first_row + 0 .. n_draft - 1 (by default b * (max_draft + 1) and
+ * b * max_draft), row i being the distribution of the token behind i drafts.
+ * Draft i is accepted iff accept_u[b, i] * q(x) < p(x); the walk stops at the
+ * first refusal. One more token follows: behind a refusal from max(p - q, 0),
+ * behind the last draft from p; it is the first id whose running sum is over
+ * draw_u[b] times the whole. drafts and accept_u have row stride max_draft.
+ *
+ * rl_specdec_verify_tree -- a tree of n_node[b] in [1, max_node] nodes. Node 0
+ * is the last token of the sequence, node i > 0 holds tokens[b, i] and hangs
+ * from parent[b, i] < i (entries that are not name no node). Target row i is
+ * the distribution of the token behind node i, draft row i the one that node
+ * i's children were drawn from (draws may repeat). At a node its children are
+ * tried in order of their index: with w = p at first, child x is accepted iff
+ * accept_u[b, child] * q(x) * sum(w) < w(x), and the walk goes on from there;
+ * if not, w := max(w - sum(w) q, 0). Where no child is accepted the token is
+ * drawn from w, as above. tokens, parent and accept_u have row stride
+ * max_node <= RL_VERIFY_MAX_NODES (for the chain max_draft + 1).
+ *
+ * draft == NULL, or a draft temperature <= 0: the drafts were given, not drawn
+ * (prompt lookup, a draft model's best tokens): q is 1 at the draft, so a
+ * refused draft x is taken out of w. With a target temperature <= 0 drafts
+ * equal to the row's largest are accepted, and q is not looked at.
+ * Drafts outside [0, V) have probability 0.
+ *
+ *  out_accepted[B]  drafts accepted
+ *  out_path[B, max_node]  (tree, nullable) the accepted nodes, then -1
+ *  out_tok[B, n]    the accepted tokens, then the drawn one, then -1
+ *  out_prob[B, n]   (nullable) the target's probability of each, 0 behind
+ *                   (n = max_draft + 1, max_node)
+ *  row_status[B]    (nullable) RL_OK; RL_ERR_NONFINITE where the walk met a
+ *                   row with NaN or +inf in a kept place, with no id left, or
+ *                   a non-finite T; RL_ERR_INVALID_ARG for a count or a row
+ *                   outside its range. Such a sequence gets out_accepted -1,
+ *                   tokens and nodes -1 and probabilities 0.
+ * Rows behind the last accepted node are not read. No workspace: calls may
+ * overlap on one handle, and may be captured.
+ */
+typedef struct {
+  const void* logits;
+  rl_dtype dtype;
+  int32_t rows;
+  int64_t ld;
+  const float* temperature;
+  const uint32_t* mask;
+  int64_t mask_stride;
+  const int32_t* cut;
+  int64_t cut_stride;
+  const int32_t* first_row;
+} rl_dist_rows;
+#define RL_VERIFY_MAX_NODES 256
+rl_status rl_specdec_verify_draft(rl_sampler* h, int B, int V, int max_draft, const rl_dist_rows* target,
+                                  const rl_dist_rows* draft, const int32_t* drafts, const int32_t* n_draft,
+                                  const float* accept_u, const float* draw_u, int32_t* out_accepted, int32_t* out_tok,
+                                  float* out_prob, int32_t* row_status, void* stream);
+rl_status rl_specdec_verify_tree(rl_sampler* h, int B, int V, int max_node, const rl_dist_rows* target,
+                                 const rl_dist_rows* draft, const int32_t* tokens, const int32_t* parent,
+                                 const int32_t* n_node, const float* accept_u, const float* draw_u,
+                                 int32_t* out_accepted, int32_t* out_path, int32_t* out_tok, float* out_prob,
+                                 int32_t* row_status, void* stream);
+
+/*
  * Grammar-constrained decoding with a real GBNF grammar: the step after the
  * reference's toy Grammar (src/decoder.rs:378-557), whose get_allowed_tokens
  * (:466-529) matches single tokens against rule variants. A grammar in GBNF

@@ -62,6 +62,17 @@ ROW_PARAMS_DTYPE = np.dtype(
 )
 
 
+class _DistRows(ctypes.Structure):
+    """rl_dist_rows."""
+
+    _fields_ = [("logits", ctypes.c_void_p), ("dtype", ctypes.c_int), ("rows", ctypes.c_int32), ("ld", ctypes.c_int64),
+                ("temperature", ctypes.c_void_p), ("mask", ctypes.c_void_p), ("mask_stride", ctypes.c_int64),
+                ("cut", ctypes.c_void_p), ("cut_stride", ctypes.c_int64), ("first_row", ctypes.c_void_p)]
+
+
+VERIFY_MAX_NODES = 256  # RL_VERIFY_MAX_NODES
+
+
 class RLError(RuntimeError):
     def __init__(self, status, msg):
         super().__init__(f"{STATUS_NAMES.get(status, status)}: {msg}")
@@ -116,6 +127,11 @@ def lib():
         L.rl_specdec_sample.argtypes = [P, P, I, I, I64, P, P, P, P, P]
         L.rl_specdec_verify.restype = I
         L.rl_specdec_verify.argtypes = [P, P, I, I, I64, P, I, P, P, P, P, P, P, P]
+        D = ctypes.POINTER(_DistRows)
+        L.rl_specdec_verify_draft.restype = I
+        L.rl_specdec_verify_draft.argtypes = [P, I, I, I, D, D, P, P, P, P, P, P, P, P, P]
+        L.rl_specdec_verify_tree.restype = I
+        L.rl_specdec_verify_tree.argtypes = [P, I, I, I, D, D, P, P, P, P, P, P, P, P, P, P, P]
         L.rl_greedy_host.restype = I
         L.rl_greedy_host.argtypes = [P, P, I, I, P]
         L.rl_grammar_greedy_host.restype = I
@@ -188,12 +204,68 @@ def _ptr(t):
     return ctypes.c_void_p(t.data_ptr())
 
 
-def _stream(stream):
+def _stream(stream, device=None):
     if stream is None:
         import torch
 
-        stream = torch.cuda.current_stream()
+        stream = torch.cuda.current_stream(device)
     return ctypes.c_void_p(stream.cuda_stream)
+
+
+class DistRows:
+    """Rows of distributions softmax(logits / T) over their kept ids
+    (rl_dist_rows): logits [R, V] f32 or bf16, temperature [B] f32 (None: 1),
+    mask [R, words] int32/uint32 (bit-packed allowed ids), cut [R] int32 (the
+    last id that a top-k / top-p cutoff keeps; a column of sample_debug's cut
+    will do), first_row [B] int32 (None: sequences follow one another)."""
+
+    def __init__(self, logits, temperature=None, mask=None, cut=None, first_row=None):
+        import torch
+
+        if logits.dim() != 2 or logits.stride(1) != 1:
+            raise ValueError("DistRows: logits must be rows [R, V] with unit inner stride")
+        if logits.dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError("DistRows: logits must be f32 or bf16")
+        for name, t, dtypes in (("temperature", temperature, (torch.float32,)), ("first_row", first_row, (torch.int32,)),
+                                ("mask", mask, (torch.int32, torch.uint32)), ("cut", cut, (torch.int32,))):
+            if t is not None and t.dtype not in dtypes:
+                raise ValueError(f"DistRows: {name} must be {dtypes[0]}")
+            if t is not None and t.device != logits.device:
+                raise ValueError(f"DistRows: {name} is on {t.device}, the logits on {logits.device}")
+        for name, t in (("temperature", temperature), ("first_row", first_row)):
+            if t is not None and not t.is_contiguous():
+                raise ValueError(f"DistRows: {name} must be contiguous")
+        if mask is not None and (mask.dim() != 2 or mask.shape[0] < logits.shape[0] or mask.stride(1) != 1):
+            raise ValueError("DistRows: mask must have a row of words for each logits row")
+        if cut is not None and (cut.dim() != 1 or cut.shape[0] < logits.shape[0]):
+            raise ValueError("DistRows: cut must have an id for each logits row")
+        self.logits, self.temperature, self.mask, self.cut, self.first_row = logits, temperature, mask, cut, first_row
+
+    def _c(self, B, who):
+        import torch
+
+        x = self.logits
+        for name, t in (("temperature", self.temperature), ("first_row", self.first_row)):
+            if t is not None and t.numel() != B:
+                raise ValueError(f"{who}: {name} has {t.numel()} entries for {B} sequences")
+        if self.mask is not None and self.mask.shape[1] < (x.shape[1] + 31) // 32:
+            raise ValueError(f"{who}: mask rows have fewer than V bits")
+        p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+        # a single row has no stride to speak of
+        return _DistRows(p(x), RL_BF16 if x.dtype == torch.bfloat16 else RL_F32, x.shape[0],
+                         x.stride(0) if x.shape[0] > 1 else max(x.stride(0), x.shape[1]), p(self.temperature), p(self.mask),
+                         self.mask.stride(0) if self.mask is not None else 0, p(self.cut),
+                         self.cut.stride(0) if self.cut is not None else 0, p(self.first_row))
+
+
+def _operands(who, dev, **named):
+    """The tensors of a call: contiguous, of their type, on its device."""
+    import torch
+
+    for name, (t, dtype, shape) in named.items():
+        if t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous() or t.device != dev:
+            raise ValueError(f"{who}: {name} must be contiguous {dtype} {tuple(shape)} on {dev}, got {t.dtype} "
+                             f"{tuple(t.shape)} on {t.device}")
 
 
 class Sampler:
@@ -459,6 +531,60 @@ class Sampler:
                                       _stream(stream)),
               "rl_specdec_verify")
         return acc, tok
+
+    def specdec_verify_draft(self, target, drafts, n_draft, accept_u, draw_u, draft=None, stream=None):
+        """rl_specdec_verify_draft: drafts [B, K] int32 (n_draft [B] of them
+        valid) against target rows (DistRows, K + 1 a sequence) and the draft
+        rows they were drawn from (DistRows, K a sequence; None: given
+        drafts); accept_u [B, K] and draw_u [B] f32. Returns (accepted [B],
+        tokens [B, K + 1], probs [B, K + 1], row_status [B])."""
+        import torch
+
+        B, K = drafts.shape
+        dev, V = target.logits.device, target.logits.shape[1]
+        who = "specdec_verify_draft"
+        _operands(who, dev, drafts=(drafts, torch.int32, (B, K)), n_draft=(n_draft, torch.int32, (B,)),
+             accept_u=(accept_u, torch.float32, (B, K)), draw_u=(draw_u, torch.float32, (B,)))
+        if draft is not None and (draft.logits.shape[1] != V or draft.logits.device != dev):
+            raise ValueError(f"{who}: the draft rows differ from the target rows in V or device")
+        acc = torch.empty(B, dtype=torch.int32, device=dev)
+        tok = torch.empty(B, K + 1, dtype=torch.int32, device=dev)
+        prob = torch.empty(B, K + 1, dtype=torch.float32, device=dev)
+        st = torch.empty(B, dtype=torch.int32, device=dev)
+        check(lib().rl_specdec_verify_draft(self.h, B, V, K, target._c(B, who),
+                                            draft._c(B, who) if draft is not None else None, _ptr(drafts),
+                                            _ptr(n_draft), _ptr(accept_u), _ptr(draw_u), _ptr(acc), _ptr(tok),
+                                            _ptr(prob), _ptr(st), _stream(stream, dev)),
+              "rl_specdec_verify_draft")
+        return acc, tok, prob, st
+
+    def specdec_verify_tree(self, target, tokens, parent, n_node, accept_u, draw_u, draft=None, stream=None):
+        """rl_specdec_verify_tree: trees of N nodes (tokens, parent [B, N]
+        int32, node 0 the root; n_node [B] of them valid) against target rows
+        (DistRows, N a sequence) and the draft rows the nodes' children were
+        drawn from (DistRows, N a sequence; None: given tokens); accept_u
+        [B, N] and draw_u [B] f32. Returns (accepted [B], path [B, N], tokens
+        [B, N], probs [B, N], row_status [B])."""
+        import torch
+
+        B, N = tokens.shape
+        dev, V = target.logits.device, target.logits.shape[1]
+        who = "specdec_verify_tree"
+        _operands(who, dev, tokens=(tokens, torch.int32, (B, N)), parent=(parent, torch.int32, (B, N)),
+             n_node=(n_node, torch.int32, (B,)), accept_u=(accept_u, torch.float32, (B, N)),
+             draw_u=(draw_u, torch.float32, (B,)))
+        if draft is not None and (draft.logits.shape[1] != V or draft.logits.device != dev):
+            raise ValueError(f"{who}: the draft rows differ from the target rows in V or device")
+        acc = torch.empty(B, dtype=torch.int32, device=dev)
+        path, tok = (torch.empty(B, N, dtype=torch.int32, device=dev) for _ in range(2))
+        prob = torch.empty(B, N, dtype=torch.float32, device=dev)
+        st = torch.empty(B, dtype=torch.int32, device=dev)
+        check(lib().rl_specdec_verify_tree(self.h, B, V, N, target._c(B, who),
+                                           draft._c(B, who) if draft is not None else None, _ptr(tokens), _ptr(parent),
+                                           _ptr(n_node), _ptr(accept_u), _ptr(draw_u), _ptr(acc), _ptr(path),
+                                           _ptr(tok), _ptr(prob), _ptr(st), _stream(stream, dev)),
+              "rl_specdec_verify_tree")
+        return acc, path, tok, prob, st
 
     # -- LM head ------------------------------------------------------------
     @staticmethod
