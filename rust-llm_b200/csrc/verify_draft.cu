@@ -10,24 +10,34 @@
 // the last refusal is the first id whose running sum of w is over u S.
 //
 // One cluster of CTAs walks one sequence, node by node, so rows behind the
-// first refusal are never read (with a draft that is right 70% of the time
-// that is half of the rows of a chain of four). Every CTA holds a contiguous
-// eighth, quarter, ... of the ids, every warp a contiguous part of that, and
-// a lane keeps (max, sum of 2^((x - max) c)) of what it sees: one pass per
-// row. The parts' sums are joined through distributed shared memory and give
-// Z, the accept tests, and later the part in which the drawn token lies: only
-// that part is looked at again. A refusal with a draft row costs a second
-// pass over the two rows (from L2) for the sums of w.
+// first refusal are not needed (with a draft that is right 70% of the time
+// that is half of the rows of a chain of four). Every warp of the cluster
+// holds a contiguous part of the ids, and a lane keeps (max, sum of
+// 2^((x - max) c)) of what it sees: one pass per row. The parts' sums are
+// joined through distributed shared memory and give Z, the accept tests, and
+// later the part in which the drawn token lies: only that part is looked at
+// again. A refusal with a draft row costs a second pass over the two rows
+// (from L2) for the sums of w.
 //
-// Precision: 2^t is ex2.approx (relative error about 2^-22, no bias that
-// p and q or two ids would not share); 1 / T is carried as two floats, so
-// that no error of 1 / T tilts a distribution; sums are doubles. Draws are
-// compared in doubles: a token can differ from the exact one only where the
-// draw lies within about 1e-9 of a border.
+// What bounds it is HBM for many rows and, for few, the dependent steps of the
+// walk. Each lane therefore has a ring of asynchronous copies of its own (it
+// reads what it copied: no barrier), which runs ahead into the rows of the
+// node's first child: they arrive while the cluster joins its sums and
+// decides. Rows that are not 16-byte aligned are loaded without the ring.
+//
+// Precision. A weight is 2^(x c - F): one FMA and ex2.approx, relative error
+// about 2^-22 with no bias that two ids would not share; c = log2(e) / T in
+// single precision tilts a row by at most 2^-25 |t|. A lane's F is the product
+// max c of the first logits it sees, moved only where a later logit lies 64
+// binades above: any F does, as long as the sums are joined with it, and no
+// running maximum has to be kept. Sums are doubles, and draws are compared in
+// doubles: a token can differ from the exact one only where the draw lies
+// within about 1e-8 of a border.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <climits>
 
 #include "common.cuh"
@@ -36,8 +46,17 @@
 namespace rl {
 namespace {
 
-constexpr int kVT = 512;
+constexpr int kVT = 256;
 constexpr int kVW = kVT / 32;
+constexpr int kChunk = 512;       // ids of one ring slot
+constexpr int kSideBytes = 2048;  // of 4-byte logits; bf16 uses half
+constexpr int kSlotBytes = 2 * kSideBytes;  // the target's chunk and the draft's
+constexpr int kSlots = 3;
+constexpr int kRingBytes = kVW * kSlots * kSlotBytes;
+constexpr float kHigh = 18446744073709551616.0f;  // 2^64
+constexpr int kMaxCluster = 16;
+constexpr int kParts = kMaxCluster * kVW;  // parts of a row, at most
+constexpr int kPerLane = kParts / 32;
 
 struct VdSide {
   const void* logits;
@@ -55,7 +74,9 @@ struct VdSide {
 struct VdArgs {
   VdSide p, q;
   int has_q;
+  int ring;                // every row of both sides is 16-byte aligned
   int V, N;                // N: nodes of the widest sequence (outputs' row stride)
+  int part;                // ids of a warp's part (a multiple of 8)
   const int32_t* tokens;   // node i's token and uniform at b * tok_stride + i - tok_off
   const float* accept_u;
   int tok_stride, tok_off;
@@ -70,20 +91,9 @@ struct VdArgs {
   int32_t* row_status;
 };
 
-// 1 / T in base 2, as two floats.
-struct Scale {
-  float hi, lo;
-  double d;
-};
-
-__device__ __forceinline__ Scale scale_of(float T) {
-  Scale c;
-  c.d = fmin(fmax(1.4426950408889634074 / static_cast<double>(T), 1e-30), 3e38);
-  c.hi = static_cast<float>(c.d);
-  // beyond 1e7 two logits that differ at all are far apart, and lo times a
-  // large difference could overflow
-  c.lo = c.hi < 1e7f ? static_cast<float>(c.d - static_cast<double>(c.hi)) : 0.0f;
-  return c;
+// log2(e) / T.
+__device__ __forceinline__ float scale_of(float T) {
+  return static_cast<float>(fmin(fmax(1.4426950408889634074 / static_cast<double>(T), 1e-30), 3e38));
 }
 
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -91,15 +101,46 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float max16(const float (&x)[4][4]) {
+  float t[5];
+#pragma unroll
+  for (int k = 0; k < 5; ++k) t[k] = max_nan(x[(3 * k) >> 2][(3 * k) & 3], x[(3 * k + 1) >> 2][(3 * k + 1) & 3], x[(3 * k + 2) >> 2][(3 * k + 2) & 3]);
+  return max_nan(max_nan(t[0], t[1], t[2]), max_nan(t[3], t[4], x[3][3]));
+}
 __device__ __forceinline__ float ex2(float t) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
   return r;
 }
-// 2^((x - m) c); 0 for x = -inf, NaN for NaN and for x = m = +inf.
-__device__ __forceinline__ float weight(float x, float m, const Scale& c) {
-  const float d = max_nan(x - m, -3.402823466e38f);
-  return ex2(__fmaf_rn(d, c.hi, d * c.lo));
+// Where a row's largest logit m lies in the exponent's domain: F = m c. A
+// product beyond the range of floats (a row of lowest values, say) is marked
+// by an infinite F; there any two logits that differ are infinitely far apart.
+__device__ __forceinline__ float frame(float m, float c) { return m * c; }
+// The weight of x relative to the frame; 0 for x = -inf, NaN for NaN.
+__device__ __forceinline__ float weight(float x, float c, float F) { return ex2(__fmaf_rn(x, c, -F)); }
+__device__ __forceinline__ float weight(float x, float m, float c, float F) {
+  return fabsf(F) < RL_POS_INF ? weight(x, c, F) : (x == m ? 1.0f : x != x ? x : 0.0f);
+}
+// The same with the exponent in double precision.
+__device__ __forceinline__ float weight_d(float x, float m, float c, float F) {
+  if (!(x > RL_NEG_INF)) return 0.0f;
+  if (!(fabsf(F) < RL_POS_INF)) return x == m ? 1.0f : 0.0f;
+  const double t = static_cast<double>(x) * static_cast<double>(c) - static_cast<double>(F);
+  if (!(t >= -126.0)) return 0.0f;
+  const double k = rint(t);  // t is 64 and a little at most
+  return ex2(static_cast<float>(t - k)) * __int_as_float((static_cast<int>(k) + 127) << 23);
+}
+// What a sum relative to frame F (of logit m) is multiplied by to be relative
+// to frame G (of logit M >= m); more than 126 binades apart it drops out.
+__device__ __forceinline__ float rebase(float m, float F, float M, float G) {
+  if (m == M) return 1.0f;
+  const float t = F - G;
+  return t >= -126.0f ? ex2(t) : 0.0f;
 }
 
 // A row of logits with what decides which of its ids are kept.
@@ -107,319 +148,462 @@ template <typename T>
 struct Row {
   const T* x;
   const uint32_t* mask;  // null: no mask, or one that allows every id
-  int V;
   int cut;               // -1: none
   float xcut;
-  Scale c;
 };
 
 __device__ __forceinline__ float to_f(float v) { return v; }
 __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
 
+// A logit x of id j, -inf where a cutoff leaves it out.
 template <typename T>
-__device__ __forceinline__ float kept(const Row<T>& r, float x, int j, uint32_t allowed) {
-  if (!allowed) return RL_NEG_INF;
-  // written so that a NaN stays
-  if (r.cut >= 0 && (x < r.xcut || (x == r.xcut && j > r.cut))) return RL_NEG_INF;
-  return x;
+__device__ __forceinline__ float above_cut(const Row<T>& r, int j, float x) {
+  return r.cut >= 0 && (x < r.xcut || (x == r.xcut && j > r.cut)) ? RL_NEG_INF : x;
 }
 
-template <typename T>
-__device__ __forceinline__ float logit_at(const Row<T>& r, int j) {
-  if (static_cast<unsigned>(j) >= static_cast<unsigned>(r.V)) return RL_NEG_INF;
-  const uint32_t a = r.mask ? (r.mask[j >> 5] >> (j & 31)) & 1u : 1u;
-  return kept(r, to_f(r.x[j]), j, a);
+// Four consecutive logits, from shared or global memory.
+__device__ __forceinline__ void unit(const float* s, float (&x)[4]) {
+  const float4 v = *reinterpret_cast<const float4*>(s);
+  x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
 }
-
-// Eight ids of a row, j0 .. j0 + 7, as 16-byte loads where the row's address
-// allows and all eight lie in the row.
+__device__ __forceinline__ void unit(const __nv_bfloat16* s, float (&x)[4]) {
+  const uint2 v = *reinterpret_cast<const uint2*>(s);
+  x[0] = __uint_as_float(v.x << 16);
+  x[1] = __uint_as_float(v.x & 0xffff0000u);
+  x[2] = __uint_as_float(v.y << 16);
+  x[3] = __uint_as_float(v.y & 0xffff0000u);
+}
+// The same of ids j0 .. j0 + 3 one by one; -inf from id `end` on.
 template <typename T>
-__device__ __forceinline__ void load8(const Row<T>& r, int j0, bool aligned, float (&x)[8]);
-
-template <>
-__device__ __forceinline__ void load8<float>(const Row<float>& r, int j0, bool aligned, float (&x)[8]) {
-  if (aligned && j0 >= 0 && j0 <= r.V - 8) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(r.x + j0));
-    const float4 b = __ldg(reinterpret_cast<const float4*>(r.x + j0 + 4));
-    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-  } else {
+__device__ __forceinline__ void unit_guarded(const T* row, int j0, int end, float (&x)[4]) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      x[k] = static_cast<unsigned>(j0 + k) < static_cast<unsigned>(r.V) ? __ldg(r.x + j0 + k) : RL_NEG_INF;
-  }
+  for (int k = 0; k < 4; ++k) x[k] = j0 + k < end ? to_f(__ldg(row + j0 + k)) : RL_NEG_INF;
 }
 
-template <>
-__device__ __forceinline__ void load8<__nv_bfloat16>(const Row<__nv_bfloat16>& r, int j0, bool aligned, float (&x)[8]) {
-  if (aligned && j0 >= 0 && j0 <= r.V - 8) {
-    const uint4 a = __ldg(reinterpret_cast<const uint4*>(r.x + j0));
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      x[2 * k] = __uint_as_float(w[k] << 16);
-      x[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
-    }
-  } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      x[k] = static_cast<unsigned>(j0 + k) < static_cast<unsigned>(r.V) ? to_f(r.x[j0 + k]) : RL_NEG_INF;
-  }
+// The mask bits of ids j0 .. j0 + 3 (j0 a multiple of 4).
+__device__ __forceinline__ uint32_t bits4(const uint32_t* mask, int j0, int end) {
+  return j0 < end ? __ldg(mask + (j0 >> 5)) >> (j0 & 31) : 0u;
 }
-
-// Puts -inf in the places of the eight that are not kept.
+// Puts -inf in the places of the four that are not kept; a NaN that is not
+// masked stays.
 template <typename T>
-__device__ __forceinline__ void keep8(const Row<T>& r, int j0, float (&x)[8]) {
+__device__ __forceinline__ void keep4(const Row<T>& r, int j0, uint32_t bits, float (&x)[4]) {
   if (r.mask) {
-    uint32_t bits = 0;
-    if (j0 >= 0) {
-      const int w = j0 >> 5, s = j0 & 31;
-      if (j0 < r.V) {
-        const uint32_t lo = r.mask[w];
-        const uint32_t hi = s > 24 && ((w + 1) << 5) < r.V ? r.mask[w + 1] : 0u;
-        bits = __funnelshift_r(lo, hi, s);
-      }
-    } else {
-      bits = r.mask[0] << -j0;  // -8 < j0 < 0
-    }
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
+    for (int k = 0; k < 4; ++k)
       if (!((bits >> k) & 1u)) x[k] = RL_NEG_INF;
   }
   if (r.cut >= 0) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
+    for (int k = 0; k < 4; ++k)
       if (x[k] < r.xcut || (x[k] == r.xcut && j0 + k > r.cut)) x[k] = RL_NEG_INF;
   }
 }
 
-// The ids are cut into groups of eight that start on 16-byte boundaries of
-// the target row: group g holds ids 8 g - off .. 8 g - off + 7.
-template <typename T>
-__device__ __forceinline__ int lead(const T* x) {
-  return static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(T));
-}
-template <typename T>
-__device__ __forceinline__ bool lines_up(const T* x, int off) {
-  return ((reinterpret_cast<uintptr_t>(x) - static_cast<uintptr_t>(off) * sizeof(T)) & 15u) == 0;
-}
+struct __align__(16) Part {
+  double s;  // sum of weights relative to m's frame (T <= 0: NaN marks a NaN)
+  float m;   // a logit of the part, near its largest (T <= 0: the largest)
+  int id;    // T <= 0: lowest id at m
+};
 
-__device__ __forceinline__ double shfl_d(double v, int o) { return __shfl_xor_sync(0xffffffffu, v, o); }
-
-struct Part {
-  double s;  // sum of weights, relative to m
-  float m;
-  int id;    // lowest id at m (rows with T <= 0)
+// What is read of a sequence's nodes at the start.
+struct Node {
+  int tok;
+  float u;
+  float lp, lq;        // the token's logits in its parent's rows; later its weights
+  int cut[2];          // [side] this node's rows' last kept ids
+  float xcut[2];
+  int first;           // first child (INT_MAX: none)
+  int16_t parent;      // -1: none
+  uint8_t bit[2];      // the token's mask bits in its parent's rows
 };
 
 struct Ctl {
-  Part part[2][2][kVW];  // [parity][side][warp]
-  Part cta[2][2];        // [parity][side], read by the other CTAs
-  Part all[2];           // [side] joined: s relative to m
-  double wsum[kVW];      // this CTA's warps' sums of w, in units of the joined frame
+  Part part[2][2][kParts];  // [parity][side]: every CTA's warps write into every CTA
+  double w[2][kParts];      // [parity] the parts' sums of w
   double scan[kVW];
-  double ctaw[2];        // [parity] this CTA's sum of w, read by the other CTAs
-  double before, total;  // sums of w in the CTAs before the draw's, and in all
-  float cx[RL_VERIFY_MAX_NODES], cq[RL_VERIFY_MAX_NODES];  // children's logits
-  float cu[RL_VERIFY_MAX_NODES];
-  int child[RL_VERIFY_MAX_NODES], ctok[RL_VERIFY_MAX_NODES];
-  int removed[RL_VERIFY_MAX_NODES];
-  int nchild, nremoved;
-  int next;      // accepted child, -1: none, -2: sums of w wanted
-  int at;        // first id found by the draw
-  int owner;     // CTA that holds the drawn token, and its warp
-  int ownerw;
-  int status;
-  double rest;   // draw target inside the owner's warp
+  double rest;              // draw target inside the draw's part
+  double Ps, Qs;            // sums of weights of both rows, relative to Pm, Qm
   double C, S, px;
-  int k;         // next child to try
+  float Pm, Qm;
+  int Pid;
+  int status;
+  int k;                    // next child to try
+  int next;                 // accepted child, or kNone, kSums, kRefresh
+  int owner;                // part that holds the drawn token
+  int at;                   // first id found by the draw
+  int nchild, nremoved;
+  int16_t child[RL_VERIFY_MAX_NODES];    // of the present node
+  int16_t removed[RL_VERIFY_MAX_NODES];  // its refused given children
+};
+constexpr int kNone = -1, kSums = -2, kRefresh = -3;
+
+template <int Bytes>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+  if constexpr (Bytes == 16) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  } else {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+  }
+}
+
+// A lane's stream of chunks: its units of the target's ids and (where the node
+// has a draft row) the draft's, through a ring of kSlots slots.
+template <typename TP, typename TQ>
+struct Stream {
+  unsigned char* ring;  // this warp's slots
+  int flight;           // chunks issued and not taken
+  int islot, tslot;
+  int j0, j1;           // the part
+  // what is issued next
+  const TP* p;
+  const TQ* q;          // null: no draft row
+  int node, at;
+  bool live;
+
+  __device__ __forceinline__ void begin(int node_, const TP* p_, const TQ* q_) {
+    node = node_;
+    p = p_;
+    q = q_;
+    at = j0;
+    live = j0 < j1;
+  }
+  // Issues the copies of one chunk: units that lie in the part whole (one that
+  // a row's end cuts is loaded where it is used).
+  __device__ __forceinline__ void issue() {
+    const int lane = threadIdx.x & 31;
+    const uint32_t dst = smem_u32(ring) + islot * kSlotBytes;
+    const int j = at + 4 * lane;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (j + 128 * i + 4 <= j1) {
+        copy_async<4 * sizeof(TP)>(dst + (128 * i + 4 * lane) * sizeof(TP), p + j + 128 * i);
+        if (q) copy_async<4 * sizeof(TQ)>(dst + kSideBytes + (128 * i + 4 * lane) * sizeof(TQ), q + j + 128 * i);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    ++flight;
+    islot = islot + 1 == kSlots ? 0 : islot + 1;
+    at += kChunk;
+    live = at < j1;
+  }
+  // Waits for the next chunk of the stream.
+  __device__ __forceinline__ const unsigned char* take() {
+    static_assert(kSlots == 3, "one wait for each number of younger chunks");
+    --flight;
+    if (flight == 2) asm volatile("cp.async.wait_group 2;" ::: "memory");
+    else if (flight == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    else asm volatile("cp.async.wait_group 0;" ::: "memory");
+    const unsigned char* s = ring + tslot * kSlotBytes;
+    tslot = tslot + 1 == kSlots ? 0 : tslot + 1;
+    return s;
+  }
+  // Lets every copy in flight land.
+  __device__ __forceinline__ void drain() {
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    flight = 0;
+    tslot = islot;
+    live = false;
+  }
 };
 
-// One pass over this warp's groups of a row: (max, sum), or the argmax.
-template <typename T>
-__device__ Part row_part(const Row<T>& r, int off, bool greedy, int g0, int g1) {
-  const int lane = threadIdx.x & 31;
-  const bool al = lines_up(r.x, off);
-  float m = RL_NEG_INF;
-  double s = 0.0;
-  int id = INT_MAX;
-  constexpr int U = sizeof(T) == 4 ? 2 : 4;
-  for (int g = g0 + lane; g < g1; g += 32 * U) {
-    float x[U][8];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (g + 32 * u < g1) {
-        load8<T>(r, 8 * (g + 32 * u) - off, al, x[u]);
-      } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) x[u][k] = RL_NEG_INF;
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int j0 = 8 * (g + 32 * u) - off;
-      if ((r.mask || r.cut >= 0) && g + 32 * u < g1) keep8<T>(r, j0, x[u]);
-      float gm = x[u][0];
-#pragma unroll
-      for (int k = 1; k < 8; ++k) gm = max_nan(gm, x[u][k]);
-      if (greedy) {
-        if (gm > m) {
-          m = gm;
-#pragma unroll
-          for (int k = 7; k >= 0; --k)
-            if (x[u][k] == gm) id = j0 + k;
-        }
-        if (gm != gm) s = __longlong_as_double(0x7ff8000000000000LL);
-        continue;
-      }
-      if (gm > m) {
-        s *= static_cast<double>(weight(m, gm, r.c));
-        m = gm;
-      }
-      if (m == RL_NEG_INF && gm == gm) continue;
-      float e = 0.0f;
-#pragma unroll
-      for (int k = 0; k < 8; k += 2) e += weight(x[u][k], m, r.c) + weight(x[u][k + 1], m, r.c);
-      s += static_cast<double>(e);
-    }
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float m2 = __shfl_xor_sync(0xffffffffu, m, o);
-    const int id2 = __shfl_xor_sync(0xffffffffu, id, o);
-    const double s2 = shfl_d(s, o);
-    const float mm = fmaxf(m, m2);
-    if (greedy) {
-      id = m2 > m ? id2 : (m2 == m ? min(id, id2) : id);
-      s += s2;  // NaN marks a NaN
-    } else {
-      const double a = m == mm ? s : s * exp2((static_cast<double>(m) - mm) * r.c.d);
-      const double b = m2 == mm ? s2 : s2 * exp2((static_cast<double>(m2) - mm) * r.c.d);
-      s = a + b;
-    }
-    m = mm;
-  }
-  Part p;
-  p.s = s;
-  p.m = m;
-  p.id = id;
-  return p;
-}
-
-// Joins the parts held by the lanes of a warp (lanes without one hold
-// m = -inf, s = 0). Weights more than 126 binades below the largest drop out.
-__device__ __forceinline__ Part join_parts(Part p, bool greedy, double c) {
-  float m = p.m;
-  int id = p.id;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float m2 = __shfl_xor_sync(0xffffffffu, m, o);
-    const int id2 = __shfl_xor_sync(0xffffffffu, id, o);
-    id = m2 > m ? id2 : (m2 == m ? min(id, id2) : id);
-    m = fmaxf(m, m2);
-  }
-  double s = p.s;
-  if (!greedy && p.m != m) {
-    const double t = (static_cast<double>(p.m) - static_cast<double>(m)) * c;
-    s = t >= -126.0 ? s * exp2(t) : (s == s ? 0.0 : s);
-  }
-  s = warp_sum_d(s);
-  Part r;
-  r.s = s;
-  r.m = m;
-  r.id = id;
-  return r;
-}
-
 // Whether id j is one of the refused given tokens.
-__device__ __forceinline__ bool is_removed(const Ctl& sh, int n, int j) {
+__device__ __forceinline__ bool is_removed(const Ctl& sh, const Node* nodes, int n, int j) {
   for (int k = 0; k < n; ++k)
-    if (sh.removed[k] == j) return true;
+    if (nodes[sh.removed[k]].tok == j) return true;
   return false;
 }
 
-// The weights w of eight ids: max(p rho - q, 0) with a draft row (in units of
-// q's largest), else p without the refused tokens (in units of p's largest).
-template <typename TP, typename TQ>
-__device__ __forceinline__ void w8(const Row<TP>& rp, const Row<TQ>& rq, float mp, float mq, float rhi, float rlo,
-                                   bool resid, const Ctl& sh, int nrem, int g, int off, bool alp, bool alq,
-                                   float (&w)[8]) {
-  const int j0 = 8 * g - off;
-  float x[8];
-  load8<TP>(rp, j0, alp, x);
-  if (rp.mask || rp.cut >= 0) keep8<TP>(rp, j0, x);
-  if (resid) {
-    float y[8];
-    load8<TQ>(rq, j0, alq, y);
-    if (rq.mask || rq.cut >= 0) keep8<TQ>(rq, j0, y);
+// What a lane has seen of a row: a sum relative to F, the frame of logit m
+// (T <= 0: the largest logit and its lowest id).
+struct Seen {
+  float m, F;
+  double s;
+  int id;
+};
+__device__ __forceinline__ Seen unseen() {
+  return {RL_NEG_INF, __int_as_float(0x7fc00000), 0.0, INT_MAX};  // a frame of NaN: the first chunk sets it
+}
+
+__device__ __forceinline__ void see_max(Seen& z, const float (&x)[4][4], int j0) {
+  const float gm = max16(x);
+  if (gm != gm) z.s = __longlong_as_double(0x7ff8000000000000LL);
+  if (gm > z.m) {
+    z.m = gm;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const float ep = weight(x[k], mp, rp.c), eq = weight(y[k], mq, rq.c);
-      w[k] = fmaxf(__fmaf_rn(ep, rhi, __fmaf_rn(ep, rlo, -eq)), 0.0f);
-    }
-  } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      w[k] = weight(x[k], mp, rp.c);
-      if (nrem > 0 && is_removed(sh, nrem, j0 + k)) w[k] = 0.0f;
-    }
+    for (int k = 15; k >= 0; --k)
+      if (x[k >> 2][k & 3] == gm) z.id = j0 + 128 * (k >> 2) + (k & 3);
   }
 }
 
-// The CTA that holds the draw's target u * total, from the CTAs' sums (one per
-// lane; every CTA finds the same one), the sums before it, and the total. The
-// last CTA with any weight where rounding leaves no sum over the target; -1
-// where there is no weight.
-__device__ __forceinline__ double find_owner(Ctl& sh, double mine, float u) {
+__device__ __forceinline__ void see(Seen& z, const float (&x)[4][4], float c) {
+  float e[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    e[u] = (weight(x[u][0], c, z.F) + weight(x[u][1], c, z.F)) + (weight(x[u][2], c, z.F) + weight(x[u][3], c, z.F));
+  float sum = (e[0] + e[1]) + (e[2] + e[3]);
+  if (!(sum < kHigh)) {
+    // no frame yet, one that is far too low, an infinite one, or a NaN
+    const float gm = max16(x);
+    if (gm != gm) z.s = __longlong_as_double(0x7ff8000000000000LL);
+    if (gm > z.m) {
+      const float F = frame(gm, c);
+      if (z.m > RL_NEG_INF) z.s *= static_cast<double>(rebase(z.m, z.F, gm, F));
+      z.m = gm;
+      z.F = F;
+    }
+    sum = 0.0f;
+    if (z.m > RL_NEG_INF) {
+#pragma unroll
+      for (int k = 0; k < 16; ++k) sum += weight(x[k >> 2][k & 3], z.m, c, z.F);
+    }
+  }
+  z.s += static_cast<double>(sum);
+}
+
+__device__ __forceinline__ float warp_fmax(float v) { return ord_key_inv(__reduce_max_sync(0xffffffffu, ord_key(v))); }
+
+// Both sides' parts of a warp, from its lanes (an unseen side gives an empty part).
+__device__ __forceinline__ void warp_parts(const Seen& a, float ca, const Seen& b, float cb, bool greedy, Part& pa, Part& pb) {
+  pa.m = warp_fmax(a.m);
+  pb.m = warp_fmax(b.m);
+  pa.id = static_cast<int>(__reduce_min_sync(0xffffffffu, static_cast<unsigned>(a.m == pa.m ? a.id : INT_MAX)));
+  pb.id = 0;
+  const float fa = greedy ? 1.0f : a.m > RL_NEG_INF ? rebase(a.m, a.F, pa.m, frame(pa.m, ca)) : 0.0f;
+  const float fb = b.m > RL_NEG_INF ? rebase(b.m, b.F, pb.m, frame(pb.m, cb)) : 0.0f;
+  double sa = a.s == a.s ? a.s * static_cast<double>(fa) : a.s;
+  double sb = b.s == b.s ? b.s * static_cast<double>(fb) : b.s;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const double ta = __shfl_xor_sync(0xffffffffu, sa, o), tb = __shfl_xor_sync(0xffffffffu, sb, o);
+    sa += ta;
+    sb += tb;
+  }
+  pa.s = sa;
+  pb.s = sb;
+}
+
+// Warp 0 joins the parts of both sides: their sums relative to the largest m;
+// the lane's own parts' sums of the target relative to it in w.
+__device__ __forceinline__ void join_parts(const Part* parts, int np, bool greedy, bool with_q, float cp, float cq, Part& P,
+                                           Part& Q, double (&w)[kPerLane]) {
   const int lane = threadIdx.x & 31;
-  double incl = mine;
+  const int per = (np + 31) >> 5;
+  Part a[kPerLane], b[kPerLane];
+  float ma = RL_NEG_INF, mb = RL_NEG_INF;
+#pragma unroll
+  for (int k = 0; k < kPerLane; ++k) {
+    const int i = lane * per + k;
+    a[k].s = b[k].s = 0.0;
+    a[k].m = b[k].m = RL_NEG_INF;
+    a[k].id = INT_MAX;
+    if (k < per && i < np) {
+      a[k] = parts[i];
+      if (with_q) b[k] = parts[kParts + i];
+    }
+    ma = fmaxf(ma, a[k].m);
+    mb = fmaxf(mb, b[k].m);
+  }
+  P.m = warp_fmax(ma);
+  Q.m = warp_fmax(mb);
+  const float Ga = frame(P.m, cp), Gb = frame(Q.m, cq);
+  double sa = 0.0, sb = 0.0;
+  unsigned id = INT_MAX;
+#pragma unroll
+  for (int k = 0; k < kPerLane; ++k) {
+    if (a[k].m == P.m) id = min(id, static_cast<unsigned>(a[k].id));
+    const float fa = greedy ? 1.0f : a[k].m > RL_NEG_INF ? rebase(a[k].m, frame(a[k].m, cp), P.m, Ga) : 0.0f;
+    const float fb = b[k].m > RL_NEG_INF ? rebase(b[k].m, frame(b[k].m, cq), Q.m, Gb) : 0.0f;
+    w[k] = a[k].s == a[k].s ? a[k].s * static_cast<double>(fa) : a[k].s;
+    sa += w[k];
+    sb += b[k].s == b[k].s ? b[k].s * static_cast<double>(fb) : b[k].s;
+  }
+  P.id = static_cast<int>(__reduce_min_sync(0xffffffffu, id));
+  Q.id = 0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const double ta = __shfl_xor_sync(0xffffffffu, sa, o), tb = __shfl_xor_sync(0xffffffffu, sb, o);
+    sa += ta;
+    sb += tb;
+  }
+  P.s = sa;
+  Q.s = sb;
+}
+
+// Loads the chunk of ids [c0, c0 + kChunk) cut at `end` into x: unit i of the
+// lane holds ids c0 + 128 i + 4 lane ... The branches are the warp's: parts
+// end on multiples of eight ids, so that only a row's last chunk can hold a
+// unit that is cut.
+template <typename T>
+__device__ __forceinline__ void chunk_cut(const T* row, int c0, int end, float (&x)[4][4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) unit_guarded(row, c0 + 128 * i + 4 * (static_cast<int>(threadIdx.x) & 31), end, x[i]);
+}
+template <typename T>
+__device__ __forceinline__ void chunk_shared(const T* s, const T* row, int c0, int end, float (&x)[4][4]) {
+  const int lane = threadIdx.x & 31;
+  if (end - c0 >= kChunk) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) unit(s + 128 * i + 4 * lane, x[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int j = c0 + 128 * i + 4 * lane;
+      x[i][0] = x[i][1] = x[i][2] = x[i][3] = RL_NEG_INF;
+      if (j + 4 <= end) unit(s + 128 * i + 4 * lane, x[i]);
+      else if (j < end) unit_guarded(row, j, end, x[i]);
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ void chunk_global(const T* row, int c0, int end, float (&x)[4][4]) {
+  const int lane = threadIdx.x & 31;
+  const T* at = row + c0 + 4 * lane;
+  if (end - c0 < kChunk) {
+    chunk_cut(row, c0, end, x);
+  } else if ((reinterpret_cast<uintptr_t>(row) & (4 * sizeof(T) - 1)) == 0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) unit(at + 128 * i, x[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[i][k] = to_f(__ldg(at + 128 * i + k));
+  }
+}
+template <typename T>
+__device__ __forceinline__ void chunk_keep(const Row<T>& r, int c0, const uint32_t (&bits)[4], float (&x)[4][4]) {
+  if (!r.mask && r.cut < 0) return;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) keep4(r, c0 + 128 * i + 4 * (static_cast<int>(threadIdx.x) & 31), bits[i], x[i]);
+}
+template <typename T>
+__device__ __forceinline__ void chunk_bits(const Row<T>& r, int c0, int end, uint32_t (&bits)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) bits[i] = r.mask ? bits4(r.mask, c0 + 128 * i + 4 * (static_cast<int>(threadIdx.x) & 31), end) : 0u;
+}
+
+// A pass over this warp's part of a node's rows: f(first id of the chunk,
+// target logits, draft logits). The stream goes on into the rows that `ahead`
+// begins once those of this node are issued.
+template <typename TP, typename TQ, typename Ahead, typename F>
+__device__ __forceinline__ void pass(Stream<TP, TQ>& st, bool ring, const Row<TP>& rp, const Row<TQ>& rq, bool with_q,
+                                     Ahead ahead, F f) {
+  for (int c0 = st.j0; c0 < st.j1; c0 += kChunk) {
+    float x[4][4], y[4][4];
+    uint32_t bp[4], bq[4];
+    chunk_bits(rp, c0, st.j1, bp);
+    if (with_q) chunk_bits(rq, c0, st.j1, bq);
+    if (ring) {
+      while (st.flight < kSlots) {
+        if (!st.live) ahead();
+        if (!st.live) break;
+        st.issue();
+      }
+      const unsigned char* slot = st.take();
+      chunk_shared(reinterpret_cast<const TP*>(slot), rp.x, c0, st.j1, x);
+      if (with_q) chunk_shared(reinterpret_cast<const TQ*>(slot + kSideBytes), rq.x, c0, st.j1, y);
+    } else {
+      chunk_global(rp.x, c0, st.j1, x);
+      if (with_q) chunk_global(rq.x, c0, st.j1, y);
+    }
+    chunk_keep(rp, c0, bp, x);
+    if (with_q) chunk_keep(rq, c0, bq, y);
+    f(c0, x, y);
+  }
+}
+
+// Warp 0: the part that holds the draw's target u * total, and the target
+// inside it (every CTA finds the same). The last part with any weight where
+// rounding leaves no sum over the target; -1 where there is no weight.
+__device__ __forceinline__ void find_owner(Ctl& sh, const double (&w)[kPerLane], int np, float u) {
+  const int lane = threadIdx.x & 31;
+  const int per = (np + 31) >> 5;
+  double own = 0.0;
+#pragma unroll
+  for (int k = 0; k < kPerLane; ++k) own += w[k];
+  double incl = own;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const double v = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += v;
   }
   const double total = __shfl_sync(0xffffffffu, incl, 31);
-  const unsigned hit = __ballot_sync(0xffffffffu, mine > 0.0 && incl > static_cast<double>(u) * total);
-  const unsigned some = __ballot_sync(0xffffffffu, mine > 0.0);
-  const int own = hit ? __ffs(hit) - 1 : 31 - __clz(some);
-  const double before = __shfl_sync(0xffffffffu, incl - mine, own & 31);
-  if (lane == 0) {
-    sh.owner = own;
-    sh.before = before;
-    sh.total = total;
+  const double t = static_cast<double>(u) * total;
+  const unsigned hit = __ballot_sync(0xffffffffu, own > 0.0 && incl > t);
+  const unsigned some = __ballot_sync(0xffffffffu, own > 0.0);
+  const int pick = hit ? __ffs(hit) - 1 : 31 - __clz(some);
+  if (lane == (pick < 0 ? 0 : pick)) {
+    // inside the lane's parts, in the same manner
+    double run = incl - own;
+    int at = -1;
+    double before = 0.0;
+#pragma unroll
+    for (int k = 0; k < kPerLane; ++k) {
+      if (w[k] > 0.0 && (at < 0 || !(run > t))) {
+        at = k;
+        before = run;
+      }
+      run += w[k];
+    }
+    sh.owner = pick < 0 ? -1 : lane * per + at;
+    sh.rest = t - before;
+    sh.at = INT_MAX;
   }
-  return total;
 }
 
 template <typename T>
-__device__ __forceinline__ Row<T> make_row(const VdSide& a, int64_t row, int V, float T_) {
+__device__ __forceinline__ Row<T> make_row(const VdSide& a, int64_t row, int cut, float xcut) {
   Row<T> r;
   r.x = static_cast<const T*>(a.logits) + row * a.ld;
-  r.V = V;
   r.mask = a.mask ? a.mask + row * a.mask_stride : nullptr;
-  r.cut = a.cut ? a.cut[row * a.cut_stride] : -1;
-  if (static_cast<unsigned>(r.cut) >= static_cast<unsigned>(V)) r.cut = -1;
-  r.xcut = r.cut >= 0 ? to_f(r.x[r.cut]) : 0.0f;
-  r.c = scale_of(T_);
+  r.cut = cut;
+  r.xcut = xcut;
   return r;
 }
 
-// A mask row without a bit allows every id (block-wide).
+// One side's share of a node's entry: the token's logit (-inf outside the row)
+// and mask bit in the parent's row, the node's own row's cutoff.
 template <typename T>
-__device__ __forceinline__ void drop_empty_mask(Row<T>& r) {
-  if (!r.mask) return;
-  const int words = (r.V + 31) >> 5;
+__device__ __forceinline__ void read_node(const VdSide& a, int64_t row0, int V, int node, int parent, int tok, bool own_row,
+                                          float& logit, uint8_t& bit, int& cut, float& xcut) {
+  logit = RL_NEG_INF;
+  bit = 1;
+  cut = -1;
+  xcut = 0.0f;
+  const T* x = static_cast<const T*>(a.logits);
+  if (parent >= 0 && static_cast<unsigned>(tok) < static_cast<unsigned>(V)) {
+    const int64_t row = row0 + parent;
+    logit = to_f(x[row * a.ld + tok]);
+    if (a.mask) bit = (a.mask[row * a.mask_stride + (tok >> 5)] >> (tok & 31)) & 1u;
+  }
+  if (a.cut && own_row) {
+    const int64_t row = row0 + node;
+    const int c = a.cut[row * a.cut_stride];
+    if (static_cast<unsigned>(c) < static_cast<unsigned>(V)) {
+      cut = c;
+      xcut = to_f(x[row * a.ld + c]);
+    }
+  }
+}
+
+// Whether a mask row has a bit (one without allows every id); block-wide.
+__device__ __forceinline__ bool any_bit(const uint32_t* mask, int V) {
+  const int words = (V + 31) >> 5;
   uint32_t any = 0;
   for (int w = threadIdx.x; w < words; w += kVT) {
-    uint32_t m = r.mask[w];
-    if (w == words - 1 && (r.V & 31)) m &= (1u << (r.V & 31)) - 1u;
+    uint32_t m = mask[w];
+    if (w == words - 1 && (V & 31)) m &= (1u << (V & 31)) - 1u;
     any |= m;
   }
-  if (!__syncthreads_or(any != 0u)) r.mask = nullptr;
+  return __syncthreads_or(any != 0u) != 0;
 }
 
 template <typename TP, typename TQ>
 __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ VdArgs a) {
+  extern __shared__ __align__(128) unsigned char ring_base[];
   __shared__ Ctl sh;
+  Node* const nodes = reinterpret_cast<Node*>(ring_base + kRingBytes);
   namespace cgx = cooperative_groups;
   const cgx::cluster_group cl = cgx::this_cluster();
   const int C = static_cast<int>(cl.num_blocks());
@@ -427,17 +611,18 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
   const int b = blockIdx.x / C;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int V = a.V, N = a.N;
+  const bool tree = a.parent != nullptr;
+  const bool ring = a.ring != 0;
+  const int np = C * kVW, mypart = rank * kVW + warp;
   int32_t* out_tok = a.out_tok + static_cast<int64_t>(b) * N;
   int32_t* out_path = a.out_path ? a.out_path + static_cast<int64_t>(b) * N : nullptr;
   float* out_prob = a.out_prob ? a.out_prob + static_cast<int64_t>(b) * N : nullptr;
-  const int32_t* tokens = a.tokens + static_cast<int64_t>(b) * a.tok_stride - a.tok_off;
-  const float* accept_u = a.accept_u + static_cast<int64_t>(b) * a.tok_stride - a.tok_off;
-  const int32_t* parent = a.parent ? a.parent + static_cast<int64_t>(b) * a.tok_stride : nullptr;
 
   // ---- the sequence's numbers, checked ----
   const int n = a.count[b] + a.count_add;
   const float Tp = a.p.T ? a.p.T[b] : 1.0f;
   const float Tq = a.has_q && a.q.T ? a.q.T[b] : 1.0f;
+  const float du = a.draw_u[b];
   const bool greedy = Tp <= 0.0f;
   const bool drawn = a.has_q && !(Tq <= 0.0f) && !greedy;  // q comes from draft rows
   const int64_t p0 = a.p.first_row ? a.p.first_row[b] : static_cast<int64_t>(b) * a.p.per_seq;
@@ -445,176 +630,241 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
   int status = RL_OK;
   if (n < 1 || n > N || p0 < 0 || p0 + n > a.p.rows) status = RL_ERR_INVALID_ARG;
   // the last node of a chain has no children, and no draft row
-  else if (drawn && n > 1 && (q0 < 0 || q0 + n - (parent ? 0 : 1) > a.q.rows)) status = RL_ERR_INVALID_ARG;
+  else if (drawn && n > 1 && (q0 < 0 || q0 + n - (tree ? 0 : 1) > a.q.rows)) status = RL_ERR_INVALID_ARG;
   else if (!(fabsf(Tp) < RL_POS_INF) || !(fabsf(Tq) < RL_POS_INF)) status = RL_ERR_NONFINITE;
+  const float cp = scale_of(greedy ? 1.0f : Tp), cq = scale_of(drawn ? Tq : 1.0f);
+
+  if (C > 1) cgx::this_cluster().barrier_arrive();
+  for (int i = tid; i < N; i += kVT) {
+    const int64_t at = static_cast<int64_t>(b) * a.tok_stride + i - a.tok_off;
+    const bool is = i >= a.tok_off;  // a chain's node 0 has no entry
+    Node& nd = nodes[i];
+    nd.tok = is ? a.tokens[at] : -1;
+    nd.u = is ? a.accept_u[at] : 0.0f;
+    int f = tree ? a.parent[at] : i - 1;
+    if (f < 0 || f >= i) f = -1;
+    nd.parent = static_cast<int16_t>(f);
+    nd.first = !tree && i + 1 < n ? i + 1 : INT_MAX;
+    if (status == RL_OK && i < n) {
+      read_node<TP>(a.p, p0, V, i, f, nd.tok, true, nd.lp, nd.bit[0], nd.cut[0], nd.xcut[0]);
+      if (drawn) read_node<TQ>(a.q, q0, V, i, f, nd.tok, tree || i + 1 < n, nd.lq, nd.bit[1], nd.cut[1], nd.xcut[1]);
+    }
+  }
+  __syncthreads();
+  if (tree && status == RL_OK) {
+    for (int i = tid; i < n; i += kVT)
+      if (nodes[i].parent >= 0) atomicMin(&nodes[nodes[i].parent].first, i);
+    __syncthreads();
+  }
+
+  // ---- this warp's part of the ids, its stream of chunks ----
+  Stream<TP, TQ> st;
+  st.ring = ring_base + warp * (kSlots * kSlotBytes);
+  st.flight = st.islot = st.tslot = 0;
+  st.j0 = static_cast<int>(min(static_cast<int64_t>(mypart) * a.part, static_cast<int64_t>(V)));
+  st.j1 = static_cast<int>(min(static_cast<int64_t>(st.j0) + a.part, static_cast<int64_t>(V)));
+  st.live = false;
+  st.node = 0;
+  const TP* const px0 = static_cast<const TP*>(a.p.logits) + p0 * a.p.ld;
+  const TQ* const qx0 = drawn ? static_cast<const TQ*>(a.q.logits) + q0 * a.q.ld : nullptr;
+  const auto begin_node = [&](int i) {
+    const bool wq = drawn && nodes[i].first != INT_MAX;
+    st.begin(i, px0 + i * a.p.ld, wq ? qx0 + i * a.q.ld : nullptr);
+  };
+  const auto ahead = [&] {
+    const int c = nodes[st.node].first;
+    if (c != INT_MAX) begin_node(c);
+  };
+  const auto nothing = [] {};
 
   int node = 0, acc = 0, par = 0;
-  int token = -1;     // drawn token, in the CTA that finds it (thread 0)
-  double tprob = 0.0;
-  bool found = false;
+  int token = -1;  // drawn token, in the CTA that finds it (thread 0)
+  float tprob = 0.0f;
+  bool found = false, started = false;
+  if (status == RL_OK && ring) begin_node(0);
   while (status == RL_OK) {
-    // ---- the node's children (thread-uniform), their logits ----
-    Row<TP> rp = make_row<TP>(a.p, p0 + node, V, greedy ? 1.0f : Tp);
-    const int off = lead(rp.x);
-    drop_empty_mask(rp);
+    // ---- the node's rows and its children ----
+    const Node& nd = nodes[node];
+    Row<TP> rp = make_row<TP>(a.p, p0 + node, nd.cut[0], nd.xcut[0]);
+    const int firstc = nd.first;
+    const bool with_q = drawn && firstc != INT_MAX;
+    Row<TQ> rq = {};
+    if (with_q) rq = make_row<TQ>(a.q, q0 + node, nd.cut[1], nd.xcut[1]);
+    if (rp.mask && !any_bit(rp.mask, V)) rp.mask = nullptr;
+    if (rq.mask && !any_bit(rq.mask, V)) rq.mask = nullptr;
+    // ---- this warp's sums of both rows, into every CTA of the cluster ----
+    Seen zp = unseen(), zq = unseen();
+    pass(st, ring, rp, rq, with_q, ahead, [&](int c0, const float (&x)[4][4], const float (&y)[4][4]) {
+      if (greedy) see_max(zp, x, c0 + 4 * lane);
+      else see(zp, x, cp);
+      if (with_q) see(zq, y, cq);
+    });
+    {
+      Part pp, pq;
+      warp_parts(zp, cp, zq, cq, greedy, pp, pq);
+      // every CTA of the cluster has started: its shared memory may be written
+      if (C > 1 && !started) cgx::this_cluster().barrier_wait();
+      started = true;
+      if (lane < C) {
+        Part* to = C > 1 ? cl.map_shared_rank(&sh.part[par][0][0], lane) : &sh.part[par][0][0];
+        to[mypart] = pp;
+        if (with_q) to[kParts + mypart] = pq;
+      }
+    }
+    if (C > 1) cl.sync();
+    else __syncthreads();
+    // ---- joined by warp 0 of every CTA ----
+    double wp[kPerLane];
     if (warp == 0) {
-      int c = 0;
-      if (parent) {
-        for (int i0 = node + 1; i0 < n; i0 += 32) {
-          const bool is = i0 + lane < n && parent[i0 + lane] == node;
-          const unsigned k = __ballot_sync(0xffffffffu, is);
-          if (is) sh.child[c + __popc(k & ((1u << lane) - 1u))] = i0 + lane;
-          c += __popc(k);
+      Part P, Q;
+      join_parts(sh.part[par][0], np, greedy, with_q, cp, cq, P, Q, wp);
+      if (!with_q) Q.s = 1.0, Q.m = 0.0f;
+      const float Fp = frame(P.m, cp), Fq = frame(Q.m, cq);
+      // the children: their weights
+      int nchild = 0;
+      for (int i0 = firstc; i0 < n; i0 += 32) {
+        const int i = i0 + lane;
+        const bool is = i < n && (tree ? nodes[i].parent == node : i == firstc);
+        const unsigned k = __ballot_sync(0xffffffffu, is);
+        if (is) {
+          Node& c = nodes[i];
+          sh.child[nchild + __popc(k & ((1u << lane) - 1u))] = static_cast<int16_t>(i);
+          const float x = rp.mask && !c.bit[0] ? RL_NEG_INF : above_cut(rp, c.tok, c.lp);
+          c.lp = weight_d(x, P.m, cp, Fp);
+          if (with_q) {
+            const float y = rq.mask && !c.bit[1] ? RL_NEG_INF : above_cut(rq, c.tok, c.lq);
+            c.lq = weight_d(y, Q.m, cq, Fq);
+          }
         }
-      } else if (node + 1 < n) {
-        if (lane == 0) sh.child[0] = node + 1;
-        c = 1;
+        nchild += __popc(k);
+        if (!tree) break;
       }
       if (lane == 0) {
-        sh.nchild = c;
+        sh.status = (P.s != P.s || !(fabsf(P.m) < RL_POS_INF) || Q.s != Q.s || !(fabsf(Q.m) < RL_POS_INF))
+                        ? RL_ERR_NONFINITE
+                        : RL_OK;
+        sh.Ps = P.s;
+        sh.Qs = Q.s;
+        sh.Pm = P.m;
+        sh.Qm = Q.m;
+        sh.Pid = P.id;
+        sh.C = 0.0;
+        sh.S = 1.0;
+        sh.k = 0;
+        sh.nchild = nchild;
         sh.nremoved = 0;
       }
-    }
-    __syncthreads();
-    const int nchild = sh.nchild;
-    const bool with_q = drawn && nchild > 0;
-    Row<TQ> rq = {};
-    if (with_q) {
-      rq = make_row<TQ>(a.q, q0 + node, V, Tq);
-      drop_empty_mask(rq);
-    }
-    for (int k = tid; k < nchild; k += kVT) {
-      const int t = tokens[sh.child[k]];
-      sh.ctok[k] = t;
-      sh.cu[k] = accept_u[sh.child[k]];
-      sh.cx[k] = logit_at(rp, t);
-      sh.cq[k] = with_q ? logit_at(rq, t) : RL_NEG_INF;
-    }
-    // ---- this warp's part of the ids ----
-    const int groups = (off + V + 7) >> 3;
-    const int per_cta = (groups + C - 1) / C;
-    const int per_warp = (per_cta + kVW - 1) / kVW;
-    const int c1 = min((rank + 1) * per_cta, groups);
-    const int g0 = min(rank * per_cta + warp * per_warp, c1), g1 = min(g0 + per_warp, c1);
-    // ---- sums of both rows, joined over the CTA and the cluster ----
-    {
-      const Part pp = row_part<TP>(rp, off, greedy, g0, g1);
-      if (lane == 0) sh.part[par][0][warp] = pp;
-      if (with_q) {
-        const Part pq = row_part<TQ>(rq, off, false, g0, g1);
-        if (lane == 0) sh.part[par][1][warp] = pq;
-      }
-    }
-    __syncthreads();
-    if (warp < (with_q ? 2 : 1)) {
-      const double c = warp ? rq.c.d : rp.c.d;
-      Part e = {0.0, RL_NEG_INF, INT_MAX};
-      if (lane < kVW) e = sh.part[par][warp][lane];
-      e = join_parts(e, greedy, c);
-      if (lane == 0) sh.cta[par][warp] = e;
-    }
-    cl.sync();
-    if (warp < (with_q ? 2 : 1)) {
-      const double c = warp ? rq.c.d : rp.c.d;
-      Part e = {0.0, RL_NEG_INF, INT_MAX};
-      if (lane < C) e = *cl.map_shared_rank(&sh.cta[par][warp], lane);
-      e = join_parts(e, greedy, c);
-      if (lane == 0) sh.all[warp] = e;
+      __syncwarp();
     }
     par ^= 1;
-    __syncthreads();
-    const Part P = sh.all[0];
-    const Part Q = with_q ? sh.all[1] : Part{1.0, 0.0f, 0};
-    if (P.s != P.s || !(fabsf(P.m) < RL_POS_INF) || Q.s != Q.s || !(fabsf(Q.m) < RL_POS_INF)) {
-      status = RL_ERR_NONFINITE;
-      break;
-    }
-    const bool alp = lines_up(rp.x, off), alq = with_q && lines_up(rq.x, off);
-    // ---- accept tests: thread 0 of every CTA, all alike ----
-    bool sums = false;  // sh.wsum / sh.total hold the sums of w
-    if (tid == 0) {
-      sh.C = 0.0;
-      sh.S = 1.0;
-      sh.k = 0;
-    }
-    int next = -1;
+    bool sums = false;  // sh.w holds the parts' sums of w = max(p - C q, 0)
     float rhi = 0.0f, rlo = 0.0f;
+    int next = kNone;
     while (true) {
-      if (tid == 0) {
-        int k = sh.k, nx = -1;
-        for (; k < nchild; ++k) {
+      // ---- accept tests: thread 0 of every CTA, all alike; both sides of a
+      // test are multiplied by the rows' sums ----
+      if (tid == 0 && sh.status == RL_OK) {
+        int k = sh.k, nx = kNone;
+        double S = sh.S;
+        for (; k < sh.nchild; ++k) {
+          const int c = sh.child[k];
           if (greedy) {
-            if (sh.ctok[k] == P.id) {
-              nx = sh.child[k];
-              sh.px = 1.0;
+            if (nodes[c].tok == sh.Pid) {
+              nx = c;
+              sh.px = sh.Ps = 1.0;
               break;
             }
             continue;
           }
-          const float x = sh.cx[k];
-          const double px = x > RL_NEG_INF ? exp2((static_cast<double>(x) - P.m) * rp.c.d) / P.s : 0.0;
+          const double ep = nodes[c].lp;
           if (with_q) {
-            const float y = sh.cq[k];
-            const double qx = y > RL_NEG_INF ? exp2((static_cast<double>(y) - Q.m) * rq.c.d) / Q.s : 0.0;
-            if (static_cast<double>(sh.cu[k]) * qx * sh.S < px - sh.C * qx) {
-              nx = sh.child[k];
-              sh.px = px;
+            const double eq = nodes[c].lq * sh.Ps;
+            if (static_cast<double>(nodes[c].u) * S * eq < ep * sh.Qs - sh.C * eq) {
+              nx = c;
+              sh.px = ep;
               break;
             }
-            sh.C += sh.S;  // refused: the sums of the new w are wanted
-            nx = -2;
+            sh.C += S;  // refused: the sums of the new w are wanted
+            nx = kSums;
             ++k;
             break;
           }
-          const bool gone = is_removed(sh, sh.nremoved, sh.ctok[k]);
-          if (!gone && static_cast<double>(sh.cu[k]) * sh.S < px) {
-            nx = sh.child[k];
-            sh.px = px;
+          const bool gone = is_removed(sh, nodes, sh.nremoved, nodes[c].tok);
+          if (!gone && static_cast<double>(nodes[c].u) * S * sh.Ps < ep) {
+            nx = c;
+            sh.px = ep;
             break;
           }
-          if (!gone && px > 0.0) {
-            sh.removed[sh.nremoved++] = sh.ctok[k];
-            sh.S = fmax(sh.S - px, 0.0);
+          if (!gone && ep > 0.0) {
+            sh.removed[sh.nremoved++] = static_cast<int16_t>(c);
+            S = fmax(S - ep / sh.Ps, 0.0);
           }
         }
+        if (nx == kNone && sh.nremoved > 0) nx = kRefresh;
+        sh.S = S;
         sh.k = k;
         sh.next = nx;
       }
       __syncthreads();
+      status = sh.status;
       next = sh.next;
-      if (next != -2) break;
+      if (status != RL_OK || next != kSums) break;
       // ---- sums of w = max(p - C q, 0) over the parts ----
-      const double rho = Q.s / (sh.C * P.s);
+      if (ring) {
+        st.drain();
+        st.begin(node, rp.x, rq.x);
+      }
+      const double rho = sh.Qs / (sh.C * sh.Ps);
       rhi = static_cast<float>(rho);
       rlo = static_cast<float>(rho - static_cast<double>(rhi));
+      const float Pm = sh.Pm, Qm = sh.Qm, Fp = frame(Pm, cp), Fq = frame(Qm, cq);
       double s = 0.0;
-      for (int g = g0 + lane; g < g1; g += 32) {
-        float w[8];
-        w8<TP, TQ>(rp, rq, P.m, Q.m, rhi, rlo, true, sh, 0, g, off, alp, alq, w);
-        s += static_cast<double>(((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])));
-      }
+      pass(st, ring, rp, rq, true, nothing, [&](int, const float (&x)[4][4], const float (&y)[4][4]) {
+        float w = 0.0f;
+        if (fabsf(Fp) < RL_POS_INF && fabsf(Fq) < RL_POS_INF) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float ep = weight(x[i][k], cp, Fp), eq = weight(y[i][k], cq, Fq);
+              v[k] = fmaxf(__fmaf_rn(ep, rhi, __fmaf_rn(ep, rlo, -eq)), 0.0f);
+            }
+            w += (v[0] + v[1]) + (v[2] + v[3]);
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            const float ep = weight(x[k >> 2][k & 3], Pm, cp, Fp), eq = weight(y[k >> 2][k & 3], Qm, cq, Fq);
+            w += fmaxf(__fmaf_rn(ep, rhi, __fmaf_rn(ep, rlo, -eq)), 0.0f);
+          }
+        }
+        s += static_cast<double>(w);
+      });
       s = warp_sum_d(s);
-      if (lane == 0) sh.wsum[warp] = s;
-      __syncthreads();
+      if (lane < C) (C > 1 ? cl.map_shared_rank(&sh.w[par][0], lane) : &sh.w[par][0])[mypart] = s;
+      if (C > 1) cl.sync();
+      else __syncthreads();
       if (warp == 0) {
-        const double t = warp_sum_d(lane < kVW ? sh.wsum[lane] : 0.0);
-        if (lane == 0) sh.ctaw[par] = t;
-      }
-      cl.sync();
-      if (warp == 0) {
-        const double mine = lane < C ? *cl.map_shared_rank(&sh.ctaw[par], lane) : 0.0;
-        const double all = find_owner(sh, mine, a.draw_u[b]);
-        if (lane == 0) sh.S = all * sh.C / Q.s;  // as a probability
+        double t = 0.0;
+        for (int i = lane; i < np; i += 32) t += sh.w[par][i];
+        t = warp_sum_d(t);
+        if (lane == 0) sh.S = t * sh.C / sh.Qs;  // as a probability
+        __syncwarp();
       }
       par ^= 1;
       sums = true;
-      __syncthreads();
     }
+    if (status != RL_OK) break;
     if (next >= 0) {
       if (rank == 0 && tid == 0) {
-        out_tok[acc] = tokens[next];
+        out_tok[acc] = nodes[next].tok;
         if (out_path) out_path[acc] = next;
-        if (out_prob) out_prob[acc] = static_cast<float>(sh.px);
+        if (out_prob) out_prob[acc] = static_cast<float>(sh.px / sh.Ps);
+      }
+      if (ring && (sums || next != firstc)) {
+        st.drain();
+        begin_node(next);
       }
       node = next;
       ++acc;
@@ -624,87 +874,90 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
     // ---- no child is accepted: the last token ----
     if (greedy) {
       if (rank == 0 && tid == 0) {
-        token = P.id;
-        tprob = 1.0;
+        token = sh.Pid;
+        tprob = 1.0f;
         found = true;
       }
       break;
     }
-    const bool resid = sums && sh.total > 0.0;  // all of w rounded away: from p
+    const bool resid = sums && sh.S > 0.0;  // else all of w rounded away: from p
     const int nrem = sh.nremoved;
-    if (!resid) {
-      // w = p, without refused given tokens: their warps sum again
-      double f = 0.0;
-      if (lane == 0) {
-        const Part e = sh.part[par ^ 1][0][warp];
-        const double t = (static_cast<double>(e.m) - static_cast<double>(P.m)) * rp.c.d;
-        f = t >= -126.0 ? e.s * exp2(t) : 0.0;
+    const float Pm = sh.Pm, Qm = sh.Qm, Fp = frame(Pm, cp), Fq = frame(Qm, cq);
+    // The weights w of ids j .. j + 3: max(p rho - q, 0) in units of q's
+    // largest, or p without the refused given tokens in units of p's largest.
+    const auto w4 = [&](int j, int end, float (&w)[4]) {
+      float x[4];
+      unit_guarded(rp.x, j, end, x);
+      keep4(rp, j, rp.mask ? bits4(rp.mask, j, end) : 0u, x);
+      if (resid) {
+        float y[4];
+        unit_guarded(rq.x, j, end, y);
+        keep4(rq, j, rq.mask ? bits4(rq.mask, j, end) : 0u, y);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float ep = weight(x[k], Pm, cp, Fp), eq = weight(y[k], Qm, cq, Fq);
+          w[k] = fmaxf(__fmaf_rn(ep, rhi, __fmaf_rn(ep, rlo, -eq)), 0.0f);
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          w[k] = weight(x[k], Pm, cp, Fp);
+          if (nrem > 0 && is_removed(sh, nodes, nrem, j + k)) w[k] = 0.0f;
+        }
       }
-      if (sums) f = 0.0;
-      bool again = sums;  // the parts' buffer may hold a later exchange
+    };
+    if (!resid && nrem > 0) {
+      // the parts that hold refused given tokens sum again (taking a weight
+      // off a sum would leave its rounding)
+      const Part me = sh.part[par ^ 1][0][mypart];
+      double f = me.m > RL_NEG_INF ? me.s * static_cast<double>(rebase(me.m, frame(me.m, cp), Pm, Fp)) : 0.0;
+      bool again = false;
       for (int k = 0; k < nrem; ++k) {
-        const int g = (sh.removed[k] + off) >> 3;
-        again |= g >= g0 && g < g1;
+        const int t = nodes[sh.removed[k]].tok;
+        again |= t >= st.j0 && t < st.j1;
       }
       if (again) {
         double s = 0.0;
-        for (int g = g0 + lane; g < g1; g += 32) {
-          float w[8];
-          w8<TP, TQ>(rp, rq, P.m, Q.m, 0.0f, 0.0f, false, sh, nrem, g, off, alp, false, w);
-          s += static_cast<double>(((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])));
+        for (int j = st.j0 + 4 * lane; j < st.j1; j += 128) {
+          float w[4];
+          w4(j, st.j1, w);
+          s += static_cast<double>((w[0] + w[1]) + (w[2] + w[3]));
         }
         f = warp_sum_d(s);
       }
-      if (lane == 0) sh.wsum[warp] = f;
-      __syncthreads();
-      if (warp == 0) {
-        const double t = warp_sum_d(lane < kVW ? sh.wsum[lane] : 0.0);
-        if (lane == 0) sh.ctaw[par] = t;
-      }
-      cl.sync();
-      if (warp == 0) {
-        const double mine = lane < C ? *cl.map_shared_rank(&sh.ctaw[par], lane) : 0.0;
-        find_owner(sh, mine, a.draw_u[b]);
-      }
+      if (lane < C) (C > 1 ? cl.map_shared_rank(&sh.w[par][0], lane) : &sh.w[par][0])[mypart] = f;
+      if (C > 1) cl.sync();
+      else __syncthreads();
       par ^= 1;
-      __syncthreads();
     }
-    // ---- which warp of which CTA holds the drawn token ----
+    // ---- which part holds the drawn token ----
     if (warp == 0) {
-      const double t = static_cast<double>(a.draw_u[b]) * sh.total;
-      const double w = lane < kVW ? sh.wsum[lane] : 0.0;
-      double incl = w;
+      if (resid || nrem > 0) {
+        const int per = (np + 31) >> 5;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double v = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += v;
+        for (int k = 0; k < kPerLane; ++k)
+          wp[k] = k < per && lane * per + k < np ? sh.w[par ^ 1][lane * per + k] : 0.0;
       }
-      // where rounding leaves no sum over t: the last part with any weight
-      const unsigned hit = __ballot_sync(0xffffffffu, w > 0.0 && sh.before + incl > t);
-      const unsigned some = __ballot_sync(0xffffffffu, w > 0.0);
-      const int pick = hit ? __ffs(hit) - 1 : 31 - __clz(some);
-      const double from = __shfl_sync(0xffffffffu, sh.before + incl - w, pick & 31);
-      if (lane == 0) {
-        sh.ownerw = pick;
-        sh.rest = t - from;
-        sh.at = INT_MAX;
-      }
+      find_owner(sh, wp, np, du);
     }
     __syncthreads();
-    if (sh.owner == rank) {
-      // ---- the drawn token inside that warp's part, by the whole CTA ----
-      const int w0 = min(rank * per_cta + sh.ownerw * per_warp, c1), w1 = min(w0 + per_warp, c1);
-      const int per = (w1 - w0 + kVT - 1) / kVT;
-      const int a0 = min(w0 + tid * per, w1), a1 = min(a0 + per, w1);
+    const int owner = sh.owner;
+    if (owner >= 0 && owner / kVW == rank) {
+      // ---- the drawn token inside that part, by the whole CTA ----
+      const int w0 = static_cast<int>(min(static_cast<int64_t>(owner) * a.part, static_cast<int64_t>(V)));
+      const int w1 = static_cast<int>(min(static_cast<int64_t>(w0) + a.part, static_cast<int64_t>(V)));
+      const int per = ((w1 - w0 + kVT - 1) / kVT + 3) & ~3;
+      const int a0 = static_cast<int>(min(static_cast<int64_t>(w0) + static_cast<int64_t>(tid) * per, static_cast<int64_t>(w1)));
+      const int a1 = min(a0 + per, w1);
       double s = 0.0;
       int last = -1;
-      for (int g = a0; g < a1; ++g) {
-        float w[8];
-        w8<TP, TQ>(rp, rq, P.m, Q.m, rhi, rlo, resid, sh, nrem, g, off, alp, alq, w);
+      for (int j = a0; j < a1; j += 4) {
+        float w[4];
+        w4(j, a1, w);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
+        for (int k = 0; k < 4; ++k) {
           s += static_cast<double>(w[k]);
-          if (w[k] > 0.0f) last = 8 * g - off + k;
+          if (w[k] > 0.0f) last = j + k;
         }
       }
       double incl = s;
@@ -715,20 +968,20 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
       }
       if (lane == 31) sh.scan[warp] = incl;
       __syncthreads();
-      double base = 0.0;
-      for (int w = 0; w < warp; ++w) base += sh.scan[w];
-      double run = base + incl - s;
-      if (run + s > sh.rest && s > 0.0) {
-        for (int g = a0; g < a1; ++g) {
-          float w[8];
-          w8<TP, TQ>(rp, rq, P.m, Q.m, rhi, rlo, resid, sh, nrem, g, off, alp, alq, w);
+      double run = incl - s;
+      for (int w = 0; w < warp; ++w) run += sh.scan[w];
+      const double rest = sh.rest;
+      if (run + s > rest && s > 0.0) {
+        bool hit = false;
+        for (int j = a0; j < a1 && !hit; j += 4) {
+          float w[4];
+          w4(j, a1, w);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
+          for (int k = 0; k < 4; ++k) {
             run += static_cast<double>(w[k]);
-            if (w[k] > 0.0f && run > sh.rest) {
-              atomicMin(&sh.at, 8 * g - off + k);
-              g = a1;
-              break;
+            if (!hit && w[k] > 0.0f && run > rest) {
+              atomicMin(&sh.at, j + k);
+              hit = true;
             }
           }
         }
@@ -744,21 +997,20 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
       }
       if (tid == 0) {
         token = sh.at;
-        if (token >= 0) {
-          const float x = logit_at(rp, token);
-          tprob = exp2((static_cast<double>(x) - P.m) * rp.c.d) / P.s;
-        }
+        if (token >= 0) tprob = static_cast<float>(weight_d(to_f(rp.x[token]), Pm, cp, Fp) / sh.Ps);
         found = true;
       }
-    } else if (sh.owner < 0 && rank == 0 && tid == 0) {
+    } else if (owner < 0 && rank == 0 && tid == 0) {
       found = true;  // every id with weight was refused (uniforms of 1): no token
     }
     break;
   }
+  if (C > 1 && !started) cgx::this_cluster().barrier_wait();
+  if (ring) st.drain();
   // ---- outputs ----
   if (found) {
     out_tok[acc] = token;
-    if (out_prob) out_prob[acc] = static_cast<float>(tprob);
+    if (out_prob) out_prob[acc] = tprob;
   }
   if (rank == 0) {
     const int from = status == RL_OK ? acc + 1 : 0;
@@ -773,7 +1025,6 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
       if (a.row_status) a.row_status[b] = status;
     }
   }
-  cl.sync();  // no CTA leaves while another may read its shared memory
 }
 
 struct VdGuard {
@@ -791,7 +1042,20 @@ struct VdGuard {
 
 template <typename TP, typename TQ>
 cudaError_t launch(const VdArgs& a, int B, int C, cudaStream_t stream) {
+  static std::atomic<int> configured[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64 || !configured[dev].load(std::memory_order_acquire)) {
+    e = cudaFuncSetAttribute(verify_kernel<TP, TQ>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             kRingBytes + RL_VERIFY_MAX_NODES * static_cast<int>(sizeof(Node)));
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(verify_kernel<TP, TQ>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64) configured[dev].store(1, std::memory_order_release);
+  }
   cudaLaunchConfig_t cfg = {};
+  cfg.dynamicSmemBytes = kRingBytes + static_cast<size_t>(a.N) * sizeof(Node);
   cfg.gridDim = dim3(static_cast<unsigned>(B) * C);
   cfg.blockDim = dim3(kVT);
   cfg.stream = stream;
@@ -827,6 +1091,24 @@ rl_status side_of(const rl_dist_rows* d, int V, int per_seq, VdSide* s) {
   return RL_OK;
 }
 
+// CTAs of a sequence's cluster: as many as fill the GPU once (two CTAs an SM),
+// since a walk's steps follow one another and only its rows can be split, but
+// four where there are sequences enough, and at least 2048 ids a CTA, below
+// which the join costs more than it saves. us a call at 2 / 4 / 8 / 16 CTAs:
+// 64 x 4 x 128256 f32 120 / 81 / 95 / 143, 16 trees of 29 nodes x 128256 110 /
+// 65 / 45 / 41, one chain of 3 x 32000 20.5 / 15.7 / 13.9 / 14.7.
+int cluster_size(int B, int V) {
+  int C = 1;
+  while (C < kMaxCluster && (C < 4 || static_cast<int64_t>(B) * C * 2 <= 256) && V / (2 * C) >= 2048) C *= 2;
+  return C;
+}
+
+// Whether every row starts on a 16-byte boundary.
+bool rows_aligned(const rl_dist_rows* d) {
+  const int64_t size = d->dtype == RL_F32 ? 4 : 2;
+  return reinterpret_cast<uintptr_t>(d->logits) % 16 == 0 && (d->rows <= 1 || d->ld * size % 16 == 0);
+}
+
 rl_status verify(rl_sampler* h, int B, int V, VdArgs& a, const rl_dist_rows* target, const rl_dist_rows* draft,
                  int q_per_seq, cudaStream_t stream) {
   rl_status st = side_of(target, V, a.N, &a.p);
@@ -842,10 +1124,13 @@ rl_status verify(rl_sampler* h, int B, int V, VdArgs& a, const rl_dist_rows* tar
     qb = draft->dtype == RL_BF16;
   }
   a.has_q = draft != nullptr;
+  a.ring = rows_aligned(target) && (!draft || rows_aligned(draft));
   a.V = V;
   VdGuard g(h->device);
   if (!g.ok) return set_error(RL_ERR_CUDA, "rl_specdec_verify: cudaSetDevice failed");
-  const int C = 1;
+  const int C = cluster_size(B, V);
+  // parts in whole groups of eight ids: they start on 16-byte boundaries
+  a.part = static_cast<int>(((static_cast<int64_t>(V) + C * kVW - 1) / (C * kVW) + 7) & ~int64_t(7));
   using bf = __nv_bfloat16;
   const cudaError_t e = pb ? (qb ? launch<bf, bf>(a, B, C, stream) : launch<bf, float>(a, B, C, stream))
                            : (qb ? launch<float, bf>(a, B, C, stream) : launch<float, float>(a, B, C, stream));
