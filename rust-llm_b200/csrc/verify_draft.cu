@@ -20,10 +20,9 @@
 // (from L2) for the sums of w.
 //
 // What bounds it is HBM for many rows and, for few, the dependent steps of the
-// walk. Each lane therefore has a ring of asynchronous copies of its own (it
-// reads what it copied: no barrier), which runs ahead into the rows of the
-// node's first child: they arrive while the cluster joins its sums and
-// decides. Rows that are not 16-byte aligned are loaded without the ring.
+// walk. While the cluster joins its sums and decides, the rows of the node's
+// first child are fetched into L2; a pass then runs on L2, a warp's next chunk
+// loaded as soon as the registers of the last are free, 24 warps an SM.
 //
 // Precision. A weight is 2^(x c - F): one FMA and ex2.approx, relative error
 // about 2^-22 with no bias that two ids would not share; c = log2(e) / T in
@@ -37,7 +36,6 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
-#include <atomic>
 #include <climits>
 
 #include "common.cuh"
@@ -48,13 +46,9 @@ namespace {
 
 constexpr int kVT = 256;
 constexpr int kVW = kVT / 32;
-constexpr int kChunk = 512;       // ids of one ring slot
-constexpr int kSideBytes = 2048;  // of 4-byte logits; bf16 uses half
-constexpr int kSlotBytes = 2 * kSideBytes;  // the target's chunk and the draft's
-constexpr int kSlots = 3;
-constexpr int kRingBytes = kVW * kSlots * kSlotBytes;
+constexpr int kChunk = 512;  // ids a warp loads at once
 constexpr float kHigh = 18446744073709551616.0f;  // 2^64
-constexpr int kMaxCluster = 16;
+constexpr int kMaxCluster = 8;
 constexpr int kParts = kMaxCluster * kVW;  // parts of a row, at most
 constexpr int kPerLane = kParts / 32;
 
@@ -74,7 +68,6 @@ struct VdSide {
 struct VdArgs {
   VdSide p, q;
   int has_q;
-  int ring;                // every row of both sides is 16-byte aligned
   int V, N;                // N: nodes of the widest sequence (outputs' row stride)
   int part;                // ids of a warp's part (a multiple of 8)
   const int32_t* tokens;   // node i's token and uniform at b * tok_stride + i - tok_off
@@ -124,16 +117,18 @@ __device__ __forceinline__ float frame(float m, float c) { return m * c; }
 // The weight of x relative to the frame; 0 for x = -inf, NaN for NaN.
 __device__ __forceinline__ float weight(float x, float c, float F) { return ex2(__fmaf_rn(x, c, -F)); }
 __device__ __forceinline__ float weight(float x, float m, float c, float F) {
-  return fabsf(F) < RL_POS_INF ? weight(x, c, F) : (x == m ? 1.0f : x != x ? x : 0.0f);
+  const float e = weight(x, c, F);
+  const float f = x == m ? 1.0f : (x != x ? x : 0.0f);
+  return fabsf(F) < RL_POS_INF ? e : f;
 }
-// The same with the exponent in double precision.
-__device__ __forceinline__ float weight_d(float x, float m, float c, float F) {
+// The same with the exponent in two floats.
+__device__ __forceinline__ float weight_2(float x, float m, float c, float F) {
   if (!(x > RL_NEG_INF)) return 0.0f;
   if (!(fabsf(F) < RL_POS_INF)) return x == m ? 1.0f : 0.0f;
-  const double t = static_cast<double>(x) * static_cast<double>(c) - static_cast<double>(F);
-  if (!(t >= -126.0)) return 0.0f;
-  const double k = rint(t);  // t is 64 and a little at most
-  return ex2(static_cast<float>(t - k)) * __int_as_float((static_cast<int>(k) + 127) << 23);
+  const float p = __fmul_rn(x, c), e = __fmaf_rn(x, c, -p);
+  const float t = __fadd_rn(p, -F), v = __fadd_rn(t, -p);
+  const float f = __fadd_rn(__fadd_rn(p, -__fadd_rn(t, -v)), __fadd_rn(-F, -v));  // p - F = t + f
+  return ex2(t) * ex2(__fadd_rn(e, f));
 }
 // What a sum relative to frame F (of logit m) is multiplied by to be relative
 // to frame G (of logit M >= m); more than 126 binades apart it drops out.
@@ -161,13 +156,13 @@ __device__ __forceinline__ float above_cut(const Row<T>& r, int j, float x) {
   return r.cut >= 0 && (x < r.xcut || (x == r.xcut && j > r.cut)) ? RL_NEG_INF : x;
 }
 
-// Four consecutive logits, from shared or global memory.
+// Four consecutive logits.
 __device__ __forceinline__ void unit(const float* s, float (&x)[4]) {
-  const float4 v = *reinterpret_cast<const float4*>(s);
+  const float4 v = __ldg(reinterpret_cast<const float4*>(s));
   x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
 }
 __device__ __forceinline__ void unit(const __nv_bfloat16* s, float (&x)[4]) {
-  const uint2 v = *reinterpret_cast<const uint2*>(s);
+  const uint2 v = __ldg(reinterpret_cast<const uint2*>(s));
   x[0] = __uint_as_float(v.x << 16);
   x[1] = __uint_as_float(v.x & 0xffff0000u);
   x[2] = __uint_as_float(v.y << 16);
@@ -238,75 +233,6 @@ struct Ctl {
 };
 constexpr int kNone = -1, kSums = -2, kRefresh = -3;
 
-template <int Bytes>
-__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
-  if constexpr (Bytes == 16) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-  } else {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
-  }
-}
-
-// A lane's stream of chunks: its units of the target's ids and (where the node
-// has a draft row) the draft's, through a ring of kSlots slots.
-template <typename TP, typename TQ>
-struct Stream {
-  unsigned char* ring;  // this warp's slots
-  int flight;           // chunks issued and not taken
-  int islot, tslot;
-  int j0, j1;           // the part
-  // what is issued next
-  const TP* p;
-  const TQ* q;          // null: no draft row
-  int node, at;
-  bool live;
-
-  __device__ __forceinline__ void begin(int node_, const TP* p_, const TQ* q_) {
-    node = node_;
-    p = p_;
-    q = q_;
-    at = j0;
-    live = j0 < j1;
-  }
-  // Issues the copies of one chunk: units that lie in the part whole (one that
-  // a row's end cuts is loaded where it is used).
-  __device__ __forceinline__ void issue() {
-    const int lane = threadIdx.x & 31;
-    const uint32_t dst = smem_u32(ring) + islot * kSlotBytes;
-    const int j = at + 4 * lane;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (j + 128 * i + 4 <= j1) {
-        copy_async<4 * sizeof(TP)>(dst + (128 * i + 4 * lane) * sizeof(TP), p + j + 128 * i);
-        if (q) copy_async<4 * sizeof(TQ)>(dst + kSideBytes + (128 * i + 4 * lane) * sizeof(TQ), q + j + 128 * i);
-      }
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-    ++flight;
-    islot = islot + 1 == kSlots ? 0 : islot + 1;
-    at += kChunk;
-    live = at < j1;
-  }
-  // Waits for the next chunk of the stream.
-  __device__ __forceinline__ const unsigned char* take() {
-    static_assert(kSlots == 3, "one wait for each number of younger chunks");
-    --flight;
-    if (flight == 2) asm volatile("cp.async.wait_group 2;" ::: "memory");
-    else if (flight == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
-    else asm volatile("cp.async.wait_group 0;" ::: "memory");
-    const unsigned char* s = ring + tslot * kSlotBytes;
-    tslot = tslot + 1 == kSlots ? 0 : tslot + 1;
-    return s;
-  }
-  // Lets every copy in flight land.
-  __device__ __forceinline__ void drain() {
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-    flight = 0;
-    tslot = islot;
-    live = false;
-  }
-};
-
 // Whether id j is one of the refused given tokens.
 __device__ __forceinline__ bool is_removed(const Ctl& sh, const Node* nodes, int n, int j) {
   for (int k = 0; k < n; ++k)
@@ -354,8 +280,14 @@ __device__ __forceinline__ void see(Seen& z, const float (&x)[4][4], float c) {
     }
     sum = 0.0f;
     if (z.m > RL_NEG_INF) {
+      if (fabsf(z.F) < RL_POS_INF) {
 #pragma unroll
-      for (int k = 0; k < 16; ++k) sum += weight(x[k >> 2][k & 3], z.m, c, z.F);
+        for (int u = 0; u < 4; ++u)
+          sum += (weight(x[u][0], c, z.F) + weight(x[u][1], c, z.F)) + (weight(x[u][2], c, z.F) + weight(x[u][3], c, z.F));
+      } else {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) sum += x[k >> 2][k & 3] == z.m ? 1.0f : 0.0f;
+      }
     }
   }
   z.s += static_cast<double>(sum);
@@ -393,11 +325,13 @@ __device__ __forceinline__ void join_parts(const Part* parts, int np, bool greed
   float ma = RL_NEG_INF, mb = RL_NEG_INF;
 #pragma unroll
   for (int k = 0; k < kPerLane; ++k) {
+    w[k] = 0.0;
+    if (k >= per) continue;
     const int i = lane * per + k;
     a[k].s = b[k].s = 0.0;
     a[k].m = b[k].m = RL_NEG_INF;
     a[k].id = INT_MAX;
-    if (k < per && i < np) {
+    if (i < np) {
       a[k] = parts[i];
       if (with_q) b[k] = parts[kParts + i];
     }
@@ -411,6 +345,7 @@ __device__ __forceinline__ void join_parts(const Part* parts, int np, bool greed
   unsigned id = INT_MAX;
 #pragma unroll
   for (int k = 0; k < kPerLane; ++k) {
+    if (k >= per) continue;
     if (a[k].m == P.m) id = min(id, static_cast<unsigned>(a[k].id));
     const float fa = greedy ? 1.0f : a[k].m > RL_NEG_INF ? rebase(a[k].m, frame(a[k].m, cp), P.m, Ga) : 0.0f;
     const float fb = b[k].m > RL_NEG_INF ? rebase(b[k].m, frame(b[k].m, cq), Q.m, Gb) : 0.0f;
@@ -431,86 +366,98 @@ __device__ __forceinline__ void join_parts(const Part* parts, int np, bool greed
 }
 
 // Loads the chunk of ids [c0, c0 + kChunk) cut at `end` into x: unit i of the
-// lane holds ids c0 + 128 i + 4 lane ... The branches are the warp's: parts
-// end on multiples of eight ids, so that only a row's last chunk can hold a
-// unit that is cut.
-template <typename T>
-__device__ __forceinline__ void chunk_cut(const T* row, int c0, int end, float (&x)[4][4]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) unit_guarded(row, c0 + 128 * i + 4 * (static_cast<int>(threadIdx.x) & 31), end, x[i]);
-}
-template <typename T>
-__device__ __forceinline__ void chunk_shared(const T* s, const T* row, int c0, int end, float (&x)[4][4]) {
+// lane holds ids c0 + 128 i + 4 lane ... A row that does not start on a unit's
+// boundary is loaded id by id.
+template <bool Plain, typename T>
+__device__ __forceinline__ void chunk_load(const Row<T>& r, int c0, int end, float (&x)[4][4]) {
   const int lane = threadIdx.x & 31;
-  if (end - c0 >= kChunk) {
+  const bool whole = end - c0 >= kChunk;
+  const T* at = r.x + c0 + 4 * lane;
+  if (Plain || (reinterpret_cast<uintptr_t>(r.x) & (4 * sizeof(T) - 1)) == 0) {
+    if (whole) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) unit(s + 128 * i + 4 * lane, x[i]);
+      for (int i = 0; i < 4; ++i) unit(at + 128 * i, x[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int j = c0 + 128 * i + 4 * lane;
+        x[i][0] = x[i][1] = x[i][2] = x[i][3] = RL_NEG_INF;
+        if (j + 4 <= end) unit(at + 128 * i, x[i]);
+        else if (j < end) unit_guarded(r.x, j, end, x[i]);
+      }
+    }
   } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) unit_guarded(r.x, c0 + 128 * i + 4 * lane, end, x[i]);
+  }
+}
+template <bool Plain, typename T>
+__device__ __forceinline__ void chunk_keep(const Row<T>& r, int c0, int end, float (&x)[4][4]) {
+  if constexpr (!Plain) {
+    if (!r.mask && r.cut < 0) return;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int j = c0 + 128 * i + 4 * lane;
-      x[i][0] = x[i][1] = x[i][2] = x[i][3] = RL_NEG_INF;
-      if (j + 4 <= end) unit(s + 128 * i + 4 * lane, x[i]);
-      else if (j < end) unit_guarded(row, j, end, x[i]);
+      const int j = c0 + 128 * i + 4 * (static_cast<int>(threadIdx.x) & 31);
+      keep4(r, j, r.mask ? bits4(r.mask, j, end) : 0u, x[i]);
     }
   }
-}
-template <typename T>
-__device__ __forceinline__ void chunk_global(const T* row, int c0, int end, float (&x)[4][4]) {
-  const int lane = threadIdx.x & 31;
-  const T* at = row + c0 + 4 * lane;
-  if (end - c0 < kChunk) {
-    chunk_cut(row, c0, end, x);
-  } else if ((reinterpret_cast<uintptr_t>(row) & (4 * sizeof(T) - 1)) == 0) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) unit(at + 128 * i, x[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) x[i][k] = to_f(__ldg(at + 128 * i + k));
-  }
-}
-template <typename T>
-__device__ __forceinline__ void chunk_keep(const Row<T>& r, int c0, const uint32_t (&bits)[4], float (&x)[4][4]) {
-  if (!r.mask && r.cut < 0) return;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) keep4(r, c0 + 128 * i + 4 * (static_cast<int>(threadIdx.x) & 31), bits[i], x[i]);
-}
-template <typename T>
-__device__ __forceinline__ void chunk_bits(const Row<T>& r, int c0, int end, uint32_t (&bits)[4]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) bits[i] = r.mask ? bits4(r.mask, c0 + 128 * i + 4 * (static_cast<int>(threadIdx.x) & 31), end) : 0u;
 }
 
-// A pass over this warp's part of a node's rows: f(first id of the chunk,
-// target logits, draft logits). The stream goes on into the rows that `ahead`
-// begins once those of this node are issued.
-template <typename TP, typename TQ, typename Ahead, typename F>
-__device__ __forceinline__ void pass(Stream<TP, TQ>& st, bool ring, const Row<TP>& rp, const Row<TQ>& rq, bool with_q,
-                                     Ahead ahead, F f) {
-  for (int c0 = st.j0; c0 < st.j1; c0 += kChunk) {
-    float x[4][4], y[4][4];
-    uint32_t bp[4], bq[4];
-    chunk_bits(rp, c0, st.j1, bp);
-    if (with_q) chunk_bits(rq, c0, st.j1, bq);
-    if (ring) {
-      while (st.flight < kSlots) {
-        if (!st.live) ahead();
-        if (!st.live) break;
-        st.issue();
-      }
-      const unsigned char* slot = st.take();
-      chunk_shared(reinterpret_cast<const TP*>(slot), rp.x, c0, st.j1, x);
-      if (with_q) chunk_shared(reinterpret_cast<const TQ*>(slot + kSideBytes), rq.x, c0, st.j1, y);
-    } else {
-      chunk_global(rp.x, c0, st.j1, x);
-      if (with_q) chunk_global(rq.x, c0, st.j1, y);
-    }
-    chunk_keep(rp, c0, bp, x);
-    if (with_q) chunk_keep(rq, c0, bq, y);
-    f(c0, x, y);
+// Passes over this warp's part [j0, j1) of one row or of two: f(first id of the
+// chunk, logits). The next chunk is loaded as soon as f is done with the last.
+template <bool Plain, typename T, typename F>
+__device__ __forceinline__ void pass(const Row<T>& r, int j0, int j1, F f) {
+  float x[4][4];
+  if (j0 < j1) chunk_load<Plain>(r, j0, j1, x);
+  for (int c0 = j0; c0 < j1; c0 += kChunk) {
+    chunk_keep<Plain>(r, c0, j1, x);
+    f(c0, x);
+    if (c0 + kChunk < j1) chunk_load<Plain>(r, c0 + kChunk, j1, x);
   }
+}
+// f on the target's chunk, g on the draft's.
+template <bool Plain, typename TP, typename TQ, typename F, typename G>
+__device__ __forceinline__ void pass_two(const Row<TP>& rp, const Row<TQ>& rq, int j0, int j1, F f, G g) {
+  float x[4][4], y[4][4];
+  if (j0 < j1) {
+    chunk_load<Plain>(rp, j0, j1, x);
+    chunk_load<Plain>(rq, j0, j1, y);
+  }
+  for (int c0 = j0; c0 < j1; c0 += kChunk) {
+    chunk_keep<Plain>(rp, c0, j1, x);
+    f(c0, x);
+    if (c0 + kChunk < j1) chunk_load<Plain>(rp, c0 + kChunk, j1, x);
+    chunk_keep<Plain>(rq, c0, j1, y);
+    g(c0, y);
+    if (c0 + kChunk < j1) chunk_load<Plain>(rq, c0 + kChunk, j1, y);
+  }
+}
+// f on both.
+template <bool Plain, typename TP, typename TQ, typename F>
+__device__ __forceinline__ void pass_both(const Row<TP>& rp, const Row<TQ>& rq, int j0, int j1, F f) {
+  float x[4][4], y[4][4];
+  if (j0 < j1) {
+    chunk_load<Plain>(rp, j0, j1, x);
+    chunk_load<Plain>(rq, j0, j1, y);
+  }
+  for (int c0 = j0; c0 < j1; c0 += kChunk) {
+    chunk_keep<Plain>(rp, c0, j1, x);
+    chunk_keep<Plain>(rq, c0, j1, y);
+    f(x, y);
+    if (c0 + kChunk < j1) {
+      chunk_load<Plain>(rp, c0 + kChunk, j1, x);
+      chunk_load<Plain>(rq, c0 + kChunk, j1, y);
+    }
+  }
+}
+
+// Fetches ids [j0, j1) of a row into L2, a line a lane.
+template <typename T>
+__device__ __forceinline__ void fetch(const T* row, int j0, int j1) {
+  if (j0 >= j1) return;
+  const char* a = reinterpret_cast<const char*>(row + j0);
+  const char* e = reinterpret_cast<const char*>(row + j1);
+  for (a += 128 * (threadIdx.x & 31); a < e; a += 128 * 32) asm volatile("prefetch.global.L2 [%0];" ::"l"(a));
 }
 
 // Warp 0: the part that holds the draw's target u * total, and the target
@@ -599,11 +546,11 @@ __device__ __forceinline__ bool any_bit(const uint32_t* mask, int V) {
   return __syncthreads_or(any != 0u) != 0;
 }
 
-template <typename TP, typename TQ>
+// Plain: rows on 16-byte boundaries, without masks and cutoffs.
+template <typename TP, typename TQ, bool Plain>
 __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ VdArgs a) {
-  extern __shared__ __align__(128) unsigned char ring_base[];
+  extern __shared__ Node nodes[];  // a.N of them
   __shared__ Ctl sh;
-  Node* const nodes = reinterpret_cast<Node*>(ring_base + kRingBytes);
   namespace cgx = cooperative_groups;
   const cgx::cluster_group cl = cgx::this_cluster();
   const int C = static_cast<int>(cl.num_blocks());
@@ -612,7 +559,6 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int V = a.V, N = a.N;
   const bool tree = a.parent != nullptr;
-  const bool ring = a.ring != 0;
   const int np = C * kVW, mypart = rank * kVW + warp;
   int32_t* out_tok = a.out_tok + static_cast<int64_t>(b) * N;
   int32_t* out_path = a.out_path ? a.out_path + static_cast<int64_t>(b) * N : nullptr;
@@ -634,6 +580,15 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
   else if (!(fabsf(Tp) < RL_POS_INF) || !(fabsf(Tq) < RL_POS_INF)) status = RL_ERR_NONFINITE;
   const float cp = scale_of(greedy ? 1.0f : Tp), cq = scale_of(drawn ? Tq : 1.0f);
 
+  // ---- this warp's part of the ids ----
+  const int j0 = static_cast<int>(min(static_cast<int64_t>(mypart) * a.part, static_cast<int64_t>(V)));
+  const int j1 = static_cast<int>(min(static_cast<int64_t>(j0) + a.part, static_cast<int64_t>(V)));
+  const TP* const px0 = static_cast<const TP*>(a.p.logits) + p0 * a.p.ld;
+  const TQ* const qx0 = drawn ? static_cast<const TQ*>(a.q.logits) + q0 * a.q.ld : nullptr;
+  if (status == RL_OK) {  // the root's rows are on their way while the nodes are read
+    fetch(px0, j0, j1);
+    if (drawn && n > 1) fetch(qx0, j0, j1);
+  }
   if (C > 1) cgx::this_cluster().barrier_arrive();
   for (int i = tid; i < N; i += kVT) {
     const int64_t at = static_cast<int64_t>(b) * a.tok_stride + i - a.tok_off;
@@ -657,31 +612,11 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
     __syncthreads();
   }
 
-  // ---- this warp's part of the ids, its stream of chunks ----
-  Stream<TP, TQ> st;
-  st.ring = ring_base + warp * (kSlots * kSlotBytes);
-  st.flight = st.islot = st.tslot = 0;
-  st.j0 = static_cast<int>(min(static_cast<int64_t>(mypart) * a.part, static_cast<int64_t>(V)));
-  st.j1 = static_cast<int>(min(static_cast<int64_t>(st.j0) + a.part, static_cast<int64_t>(V)));
-  st.live = false;
-  st.node = 0;
-  const TP* const px0 = static_cast<const TP*>(a.p.logits) + p0 * a.p.ld;
-  const TQ* const qx0 = drawn ? static_cast<const TQ*>(a.q.logits) + q0 * a.q.ld : nullptr;
-  const auto begin_node = [&](int i) {
-    const bool wq = drawn && nodes[i].first != INT_MAX;
-    st.begin(i, px0 + i * a.p.ld, wq ? qx0 + i * a.q.ld : nullptr);
-  };
-  const auto ahead = [&] {
-    const int c = nodes[st.node].first;
-    if (c != INT_MAX) begin_node(c);
-  };
-  const auto nothing = [] {};
-
   int node = 0, acc = 0, par = 0;
+  int no_mask = 0;  // the node's rows whose mask has no bit: 1 the target's, 2 the draft's
   int token = -1;  // drawn token, in the CTA that finds it (thread 0)
   float tprob = 0.0f;
   bool found = false, started = false;
-  if (status == RL_OK && ring) begin_node(0);
   while (status == RL_OK) {
     // ---- the node's rows and its children ----
     const Node& nd = nodes[node];
@@ -690,15 +625,21 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
     const bool with_q = drawn && firstc != INT_MAX;
     Row<TQ> rq = {};
     if (with_q) rq = make_row<TQ>(a.q, q0 + node, nd.cut[1], nd.xcut[1]);
-    if (rp.mask && !any_bit(rp.mask, V)) rp.mask = nullptr;
-    if (rq.mask && !any_bit(rq.mask, V)) rq.mask = nullptr;
+    if (Plain || (no_mask & 1)) rp.mask = nullptr;
+    if (Plain || (no_mask & 2)) rq.mask = nullptr;
+    if (Plain) rp.cut = rq.cut = -1;
     // ---- this warp's sums of both rows, into every CTA of the cluster ----
     Seen zp = unseen(), zq = unseen();
-    pass(st, ring, rp, rq, with_q, ahead, [&](int c0, const float (&x)[4][4], const float (&y)[4][4]) {
+    const auto see_p = [&](int c0, const float (&x)[4][4]) {
       if (greedy) see_max(zp, x, c0 + 4 * lane);
       else see(zp, x, cp);
-      if (with_q) see(zq, y, cq);
-    });
+    };
+    if (with_q) pass_two<Plain>(rp, rq, j0, j1, see_p, [&](int, const float (&y)[4][4]) { see(zq, y, cq); });
+    else pass<Plain>(rp, j0, j1, see_p);
+    if (firstc != INT_MAX && (drawn || greedy)) {  // likely to be accepted
+      fetch(px0 + firstc * a.p.ld, j0, j1);
+      if (drawn && nodes[firstc].first != INT_MAX) fetch(qx0 + firstc * a.q.ld, j0, j1);
+    }
     {
       Part pp, pq;
       warp_parts(zp, cp, zq, cq, greedy, pp, pq);
@@ -720,9 +661,10 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
       join_parts(sh.part[par][0], np, greedy, with_q, cp, cq, P, Q, wp);
       if (!with_q) Q.s = 1.0, Q.m = 0.0f;
       const float Fp = frame(P.m, cp), Fq = frame(Q.m, cq);
+      const bool good = P.s == P.s && fabsf(P.m) < RL_POS_INF && Q.s == Q.s && fabsf(Q.m) < RL_POS_INF;
       // the children: their weights
       int nchild = 0;
-      for (int i0 = firstc; i0 < n; i0 += 32) {
+      for (int i0 = good ? firstc : INT_MAX; i0 < n; i0 += 32) {
         const int i = i0 + lane;
         const bool is = i < n && (tree ? nodes[i].parent == node : i == firstc);
         const unsigned k = __ballot_sync(0xffffffffu, is);
@@ -730,19 +672,17 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
           Node& c = nodes[i];
           sh.child[nchild + __popc(k & ((1u << lane) - 1u))] = static_cast<int16_t>(i);
           const float x = rp.mask && !c.bit[0] ? RL_NEG_INF : above_cut(rp, c.tok, c.lp);
-          c.lp = weight_d(x, P.m, cp, Fp);
+          c.lp = weight_2(x, P.m, cp, Fp);
           if (with_q) {
             const float y = rq.mask && !c.bit[1] ? RL_NEG_INF : above_cut(rq, c.tok, c.lq);
-            c.lq = weight_d(y, Q.m, cq, Fq);
+            c.lq = weight_2(y, Q.m, cq, Fq);
           }
         }
         nchild += __popc(k);
         if (!tree) break;
       }
       if (lane == 0) {
-        sh.status = (P.s != P.s || !(fabsf(P.m) < RL_POS_INF) || Q.s != Q.s || !(fabsf(Q.m) < RL_POS_INF))
-                        ? RL_ERR_NONFINITE
-                        : RL_OK;
+        sh.status = good ? RL_OK : RL_ERR_NONFINITE;
         sh.Ps = P.s;
         sh.Qs = Q.s;
         sh.Pm = P.m;
@@ -810,16 +750,12 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
       next = sh.next;
       if (status != RL_OK || next != kSums) break;
       // ---- sums of w = max(p - C q, 0) over the parts ----
-      if (ring) {
-        st.drain();
-        st.begin(node, rp.x, rq.x);
-      }
       const double rho = sh.Qs / (sh.C * sh.Ps);
       rhi = static_cast<float>(rho);
       rlo = static_cast<float>(rho - static_cast<double>(rhi));
       const float Pm = sh.Pm, Qm = sh.Qm, Fp = frame(Pm, cp), Fq = frame(Qm, cq);
       double s = 0.0;
-      pass(st, ring, rp, rq, true, nothing, [&](int, const float (&x)[4][4], const float (&y)[4][4]) {
+      pass_both<Plain>(rp, rq, j0, j1, [&](const float (&x)[4][4], const float (&y)[4][4]) {
         float w = 0.0f;
         if (fabsf(Fp) < RL_POS_INF && fabsf(Fq) < RL_POS_INF) {
 #pragma unroll
@@ -855,19 +791,25 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
       par ^= 1;
       sums = true;
     }
-    if (status != RL_OK) break;
+    if (status != RL_OK) {
+      // an empty row: once more without its mask, if that has no bit
+      const bool ep = rp.mask && sh.Pm == RL_NEG_INF && !any_bit(rp.mask, V);
+      const bool eq = with_q && rq.mask && sh.Qm == RL_NEG_INF && !any_bit(rq.mask, V);
+      no_mask |= (ep ? 1 : 0) | (eq ? 2 : 0);
+      if (!ep && !eq) break;
+      status = RL_OK;
+      __syncthreads();
+      continue;
+    }
     if (next >= 0) {
       if (rank == 0 && tid == 0) {
         out_tok[acc] = nodes[next].tok;
         if (out_path) out_path[acc] = next;
         if (out_prob) out_prob[acc] = static_cast<float>(sh.px / sh.Ps);
       }
-      if (ring && (sums || next != firstc)) {
-        st.drain();
-        begin_node(next);
-      }
       node = next;
       ++acc;
+      no_mask = 0;
       __syncthreads();  // sh.child ... are rewritten for the next node
       continue;
     }
@@ -914,15 +856,24 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
       bool again = false;
       for (int k = 0; k < nrem; ++k) {
         const int t = nodes[sh.removed[k]].tok;
-        again |= t >= st.j0 && t < st.j1;
+        again |= t >= j0 && t < j1;
       }
       if (again) {
         double s = 0.0;
-        for (int j = st.j0 + 4 * lane; j < st.j1; j += 128) {
-          float w[4];
-          w4(j, st.j1, w);
-          s += static_cast<double>((w[0] + w[1]) + (w[2] + w[3]));
-        }
+        pass<Plain>(rp, j0, j1, [&](int c0, float (&x)[4][4]) {
+          for (int k = 0; k < nrem; ++k) {
+            const int t = nodes[sh.removed[k]].tok - c0;  // its lane takes it out
+            if (t >= 0 && t < kChunk && ((t >> 2) & 31) == lane) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                if (i == ((t >> 7) << 2 | (t & 3))) x[i >> 2][i & 3] = RL_NEG_INF;
+            }
+          }
+          float w = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) w += weight(x[i >> 2][i & 3], Pm, cp, Fp);
+          s += static_cast<double>(w);
+        });
         f = warp_sum_d(s);
       }
       if (lane < C) (C > 1 ? cl.map_shared_rank(&sh.w[par][0], lane) : &sh.w[par][0])[mypart] = f;
@@ -997,7 +948,7 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
       }
       if (tid == 0) {
         token = sh.at;
-        if (token >= 0) tprob = static_cast<float>(weight_d(to_f(rp.x[token]), Pm, cp, Fp) / sh.Ps);
+        if (token >= 0) tprob = static_cast<float>(weight_2(to_f(rp.x[token]), Pm, cp, Fp) / sh.Ps);
         found = true;
       }
     } else if (owner < 0 && rank == 0 && tid == 0) {
@@ -1006,7 +957,6 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
     break;
   }
   if (C > 1 && !started) cgx::this_cluster().barrier_wait();
-  if (ring) st.drain();
   // ---- outputs ----
   if (found) {
     out_tok[acc] = token;
@@ -1040,22 +990,10 @@ struct VdGuard {
   }
 };
 
-template <typename TP, typename TQ>
+template <typename TP, typename TQ, bool Plain>
 cudaError_t launch(const VdArgs& a, int B, int C, cudaStream_t stream) {
-  static std::atomic<int> configured[64];
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  if (dev < 0 || dev >= 64 || !configured[dev].load(std::memory_order_acquire)) {
-    e = cudaFuncSetAttribute(verify_kernel<TP, TQ>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             kRingBytes + RL_VERIFY_MAX_NODES * static_cast<int>(sizeof(Node)));
-    if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(verify_kernel<TP, TQ>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return e;
-    if (dev >= 0 && dev < 64) configured[dev].store(1, std::memory_order_release);
-  }
   cudaLaunchConfig_t cfg = {};
-  cfg.dynamicSmemBytes = kRingBytes + static_cast<size_t>(a.N) * sizeof(Node);
+  cfg.dynamicSmemBytes = static_cast<size_t>(a.N) * sizeof(Node);
   cfg.gridDim = dim3(static_cast<unsigned>(B) * C);
   cfg.blockDim = dim3(kVT);
   cfg.stream = stream;
@@ -1066,7 +1004,18 @@ cudaError_t launch(const VdArgs& a, int B, int C, cudaStream_t stream) {
   at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, verify_kernel<TP, TQ>, a);
+  return cudaLaunchKernelEx(&cfg, verify_kernel<TP, TQ, Plain>, a);
+}
+
+template <typename TP, typename TQ>
+cudaError_t launch(const VdArgs& a, int B, int C, bool plain, cudaStream_t stream) {
+  return plain ? launch<TP, TQ, true>(a, B, C, stream) : launch<TP, TQ, false>(a, B, C, stream);
+}
+
+// Whether every row starts on a 16-byte boundary and keeps all of its ids.
+bool is_plain(const rl_dist_rows* d) {
+  return reinterpret_cast<uintptr_t>(d->logits) % 16 == 0 && (d->rows <= 1 || d->ld * (d->dtype == RL_F32 ? 4 : 2) % 16 == 0) &&
+         !d->mask && !d->cut;
 }
 
 rl_status side_of(const rl_dist_rows* d, int V, int per_seq, VdSide* s) {
@@ -1091,22 +1040,16 @@ rl_status side_of(const rl_dist_rows* d, int V, int per_seq, VdSide* s) {
   return RL_OK;
 }
 
-// CTAs of a sequence's cluster: as many as fill the GPU once (two CTAs an SM),
-// since a walk's steps follow one another and only its rows can be split, but
-// four where there are sequences enough, and at least 2048 ids a CTA, below
-// which the join costs more than it saves. us a call at 2 / 4 / 8 / 16 CTAs:
-// 64 x 4 x 128256 f32 120 / 81 / 95 / 143, 16 trees of 29 nodes x 128256 110 /
-// 65 / 45 / 41, one chain of 3 x 32000 20.5 / 15.7 / 13.9 / 14.7.
+// CTAs of a sequence's cluster. A walk's steps follow one another and only its
+// rows can be split: eight where they find room on the GPU at once (two CTAs an
+// SM), four where there are sequences enough, and at least 2048 ids a CTA,
+// below which the join costs more than it saves. us a call at 2 / 4 / 8 / 16
+// CTAs: 64 x 4 x 128256 f32 115 / 81 / 94 / 142, 16 trees of 29 nodes x 128256
+// 86 / 53 / 39 / 41, one chain of 3 x 32000 18.0 / 14.2 / 13.0 / 14.1.
 int cluster_size(int B, int V) {
   int C = 1;
   while (C < kMaxCluster && (C < 4 || static_cast<int64_t>(B) * C * 2 <= 256) && V / (2 * C) >= 2048) C *= 2;
   return C;
-}
-
-// Whether every row starts on a 16-byte boundary.
-bool rows_aligned(const rl_dist_rows* d) {
-  const int64_t size = d->dtype == RL_F32 ? 4 : 2;
-  return reinterpret_cast<uintptr_t>(d->logits) % 16 == 0 && (d->rows <= 1 || d->ld * size % 16 == 0);
 }
 
 rl_status verify(rl_sampler* h, int B, int V, VdArgs& a, const rl_dist_rows* target, const rl_dist_rows* draft,
@@ -1124,16 +1067,16 @@ rl_status verify(rl_sampler* h, int B, int V, VdArgs& a, const rl_dist_rows* tar
     qb = draft->dtype == RL_BF16;
   }
   a.has_q = draft != nullptr;
-  a.ring = rows_aligned(target) && (!draft || rows_aligned(draft));
   a.V = V;
   VdGuard g(h->device);
   if (!g.ok) return set_error(RL_ERR_CUDA, "rl_specdec_verify: cudaSetDevice failed");
   const int C = cluster_size(B, V);
   // parts in whole groups of eight ids: they start on 16-byte boundaries
   a.part = static_cast<int>(((static_cast<int64_t>(V) + C * kVW - 1) / (C * kVW) + 7) & ~int64_t(7));
+  const bool plain = is_plain(target) && (!draft || is_plain(draft));
   using bf = __nv_bfloat16;
-  const cudaError_t e = pb ? (qb ? launch<bf, bf>(a, B, C, stream) : launch<bf, float>(a, B, C, stream))
-                           : (qb ? launch<float, bf>(a, B, C, stream) : launch<float, float>(a, B, C, stream));
+  const cudaError_t e = pb ? (qb ? launch<bf, bf>(a, B, C, plain, stream) : launch<bf, float>(a, B, C, plain, stream))
+                           : (qb ? launch<float, bf>(a, B, C, plain, stream) : launch<float, float>(a, B, C, plain, stream));
   if (e != cudaSuccess) return set_error(RL_ERR_CUDA, cudaGetErrorString(e));
   return RL_OK;
 }

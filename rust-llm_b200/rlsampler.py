@@ -204,12 +204,21 @@ def _ptr(t):
     return ctypes.c_void_p(t.data_ptr())
 
 
-def _stream(stream, device=None):
+def _stream(stream):
+    if stream is None:
+        import torch
+
+        stream = torch.cuda.current_stream()
+    return ctypes.c_void_p(stream.cuda_stream)
+
+
+def _raw_stream(stream, device):
+    """The stream's handle: the device's current stream where none is given."""
     if stream is None:
         import torch
 
         stream = torch.cuda.current_stream(device)
-    return ctypes.c_void_p(stream.cuda_stream)
+    return stream.cuda_stream
 
 
 class DistRows:
@@ -219,53 +228,54 @@ class DistRows:
     last id that a top-k / top-p cutoff keeps; a column of sample_debug's cut
     will do), first_row [B] int32 (None: sequences follow one another)."""
 
+    __slots__ = ("logits", "temperature", "mask", "cut", "first_row", "V", "device", "c")
+
     def __init__(self, logits, temperature=None, mask=None, cut=None, first_row=None):
         import torch
 
-        if logits.dim() != 2 or logits.stride(1) != 1:
+        shape, stride, dev, dtype = logits.shape, logits.stride(), logits.device, logits.dtype
+        if len(shape) != 2 or (stride[1] != 1 and shape[1] > 1):
             raise ValueError("DistRows: logits must be rows [R, V] with unit inner stride")
-        if logits.dtype not in (torch.float32, torch.bfloat16):
+        if dtype is not torch.float32 and dtype is not torch.bfloat16:
             raise ValueError("DistRows: logits must be f32 or bf16")
-        for name, t, dtypes in (("temperature", temperature, (torch.float32,)), ("first_row", first_row, (torch.int32,)),
-                                ("mask", mask, (torch.int32, torch.uint32)), ("cut", cut, (torch.int32,))):
-            if t is not None and t.dtype not in dtypes:
-                raise ValueError(f"DistRows: {name} must be {dtypes[0]}")
-            if t is not None and t.device != logits.device:
-                raise ValueError(f"DistRows: {name} is on {t.device}, the logits on {logits.device}")
-        for name, t in (("temperature", temperature), ("first_row", first_row)):
-            if t is not None and not t.is_contiguous():
-                raise ValueError(f"DistRows: {name} must be contiguous")
-        if mask is not None and (mask.dim() != 2 or mask.shape[0] < logits.shape[0] or mask.stride(1) != 1):
-            raise ValueError("DistRows: mask must have a row of words for each logits row")
-        if cut is not None and (cut.dim() != 1 or cut.shape[0] < logits.shape[0]):
-            raise ValueError("DistRows: cut must have an id for each logits row")
+        R, V = shape
+        tp = mp = cp = fp = None
+        ms = cs = 0
+        if temperature is not None:
+            if temperature.dtype is not torch.float32 or temperature.device != dev or not temperature.is_contiguous():
+                raise ValueError("DistRows: temperature must be contiguous f32 on the logits' device")
+            tp = temperature.data_ptr()
+        if first_row is not None:
+            if first_row.dtype is not torch.int32 or first_row.device != dev or not first_row.is_contiguous():
+                raise ValueError("DistRows: first_row must be contiguous int32 on the logits' device")
+            fp = first_row.data_ptr()
+        if mask is not None:
+            if mask.dtype not in (torch.int32, torch.uint32) or mask.device != dev:
+                raise ValueError("DistRows: mask must be int32 or uint32 words on the logits' device")
+            if mask.dim() != 2 or mask.shape[0] < R or mask.shape[1] * 32 < V or (mask.shape[1] > 1 and mask.stride(1) != 1):
+                raise ValueError("DistRows: mask must have a row of words for each logits row")
+            mp, ms = mask.data_ptr(), mask.stride(0) if R > 1 else max(mask.stride(0), mask.shape[1])
+        if cut is not None:
+            if cut.dtype is not torch.int32 or cut.device != dev or cut.dim() != 1 or cut.shape[0] < R:
+                raise ValueError("DistRows: cut must have an int32 id for each logits row, on its device")
+            cp, cs = cut.data_ptr(), cut.stride(0)
         self.logits, self.temperature, self.mask, self.cut, self.first_row = logits, temperature, mask, cut, first_row
-
-    def _c(self, B, who):
-        import torch
-
-        x = self.logits
-        for name, t in (("temperature", self.temperature), ("first_row", self.first_row)):
-            if t is not None and t.numel() != B:
-                raise ValueError(f"{who}: {name} has {t.numel()} entries for {B} sequences")
-        if self.mask is not None and self.mask.shape[1] < (x.shape[1] + 31) // 32:
-            raise ValueError(f"{who}: mask rows have fewer than V bits")
-        p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+        self.V, self.device = V, dev
         # a single row has no stride to speak of
-        return _DistRows(p(x), RL_BF16 if x.dtype == torch.bfloat16 else RL_F32, x.shape[0],
-                         x.stride(0) if x.shape[0] > 1 else max(x.stride(0), x.shape[1]), p(self.temperature), p(self.mask),
-                         self.mask.stride(0) if self.mask is not None else 0, p(self.cut),
-                         self.cut.stride(0) if self.cut is not None else 0, p(self.first_row))
+        self.c = _DistRows(logits.data_ptr(), RL_BF16 if dtype is torch.bfloat16 else RL_F32, R,
+                           stride[0] if R > 1 else max(stride[0], V), tp, mp, ms, cp, cs, fp)
+
+    def _of(self, B, who):
+        """The C struct, for B sequences."""
+        for t in (self.temperature, self.first_row):
+            if t is not None and t.numel() != B:
+                raise ValueError(f"{who}: temperature and first_row must have an entry for each of {B} sequences")
+        return self.c
 
 
-def _operands(who, dev, **named):
-    """The tensors of a call: contiguous, of their type, on its device."""
-    import torch
-
-    for name, (t, dtype, shape) in named.items():
-        if t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous() or t.device != dev:
-            raise ValueError(f"{who}: {name} must be contiguous {dtype} {tuple(shape)} on {dev}, got {t.dtype} "
-                             f"{tuple(t.shape)} on {t.device}")
+def _wrong(who, name, t, dtype, shape, dev):
+    return ValueError(f"{who}: {name} must be contiguous {dtype} {tuple(shape)} on {dev}, got {t.dtype} {tuple(t.shape)} "
+                      f"on {t.device}")
 
 
 class Sampler:
@@ -540,21 +550,27 @@ class Sampler:
         tokens [B, K + 1], probs [B, K + 1], row_status [B])."""
         import torch
 
-        B, K = drafts.shape
-        dev, V = target.logits.device, target.logits.shape[1]
-        who = "specdec_verify_draft"
-        _operands(who, dev, drafts=(drafts, torch.int32, (B, K)), n_draft=(n_draft, torch.int32, (B,)),
-             accept_u=(accept_u, torch.float32, (B, K)), draw_u=(draw_u, torch.float32, (B,)))
-        if draft is not None and (draft.logits.shape[1] != V or draft.logits.device != dev):
+        who, dev, V = "specdec_verify_draft", target.device, target.V
+        i32, f32 = torch.int32, torch.float32
+        B, K = shape = drafts.shape
+        one = (B,)
+        if drafts.dtype is not i32 or drafts.device != dev or not drafts.is_contiguous():
+            raise _wrong(who, "drafts", drafts, i32, shape, dev)
+        if n_draft.dtype is not i32 or n_draft.shape != one or n_draft.device != dev or not n_draft.is_contiguous():
+            raise _wrong(who, "n_draft", n_draft, i32, one, dev)
+        if accept_u.dtype is not f32 or accept_u.shape != shape or accept_u.device != dev or not accept_u.is_contiguous():
+            raise _wrong(who, "accept_u", accept_u, f32, shape, dev)
+        if draw_u.dtype is not f32 or draw_u.shape != one or draw_u.device != dev or not draw_u.is_contiguous():
+            raise _wrong(who, "draw_u", draw_u, f32, one, dev)
+        if draft is not None and (draft.V != V or draft.device != dev):
             raise ValueError(f"{who}: the draft rows differ from the target rows in V or device")
-        acc = torch.empty(B, dtype=torch.int32, device=dev)
-        tok = torch.empty(B, K + 1, dtype=torch.int32, device=dev)
-        prob = torch.empty(B, K + 1, dtype=torch.float32, device=dev)
-        st = torch.empty(B, dtype=torch.int32, device=dev)
-        check(lib().rl_specdec_verify_draft(self.h, B, V, K, target._c(B, who),
-                                            draft._c(B, who) if draft is not None else None, _ptr(drafts),
-                                            _ptr(n_draft), _ptr(accept_u), _ptr(draw_u), _ptr(acc), _ptr(tok),
-                                            _ptr(prob), _ptr(st), _stream(stream, dev)),
+        t, d = target._of(B, who), draft._of(B, who) if draft is not None else None
+        acc, st = torch.empty_like(n_draft), torch.empty_like(n_draft)
+        tok = torch.empty((B, K + 1), dtype=i32, device=dev)
+        prob = torch.empty((B, K + 1), dtype=f32, device=dev)
+        check(lib().rl_specdec_verify_draft(self.h, B, V, K, t, d, drafts.data_ptr(), n_draft.data_ptr(),
+                                            accept_u.data_ptr(), draw_u.data_ptr(), acc.data_ptr(), tok.data_ptr(),
+                                            prob.data_ptr(), st.data_ptr(), _raw_stream(stream, dev)),
               "rl_specdec_verify_draft")
         return acc, tok, prob, st
 
@@ -567,22 +583,28 @@ class Sampler:
         [B, N], probs [B, N], row_status [B])."""
         import torch
 
-        B, N = tokens.shape
-        dev, V = target.logits.device, target.logits.shape[1]
-        who = "specdec_verify_tree"
-        _operands(who, dev, tokens=(tokens, torch.int32, (B, N)), parent=(parent, torch.int32, (B, N)),
-             n_node=(n_node, torch.int32, (B,)), accept_u=(accept_u, torch.float32, (B, N)),
-             draw_u=(draw_u, torch.float32, (B,)))
-        if draft is not None and (draft.logits.shape[1] != V or draft.logits.device != dev):
+        who, dev, V = "specdec_verify_tree", target.device, target.V
+        i32, f32 = torch.int32, torch.float32
+        B, N = shape = tokens.shape
+        one = (B,)
+        if tokens.dtype is not i32 or tokens.device != dev or not tokens.is_contiguous():
+            raise _wrong(who, "tokens", tokens, i32, shape, dev)
+        if parent.dtype is not i32 or parent.shape != shape or parent.device != dev or not parent.is_contiguous():
+            raise _wrong(who, "parent", parent, i32, shape, dev)
+        if n_node.dtype is not i32 or n_node.shape != one or n_node.device != dev or not n_node.is_contiguous():
+            raise _wrong(who, "n_node", n_node, i32, one, dev)
+        if accept_u.dtype is not f32 or accept_u.shape != shape or accept_u.device != dev or not accept_u.is_contiguous():
+            raise _wrong(who, "accept_u", accept_u, f32, shape, dev)
+        if draw_u.dtype is not f32 or draw_u.shape != one or draw_u.device != dev or not draw_u.is_contiguous():
+            raise _wrong(who, "draw_u", draw_u, f32, one, dev)
+        if draft is not None and (draft.V != V or draft.device != dev):
             raise ValueError(f"{who}: the draft rows differ from the target rows in V or device")
-        acc = torch.empty(B, dtype=torch.int32, device=dev)
-        path, tok = (torch.empty(B, N, dtype=torch.int32, device=dev) for _ in range(2))
-        prob = torch.empty(B, N, dtype=torch.float32, device=dev)
-        st = torch.empty(B, dtype=torch.int32, device=dev)
-        check(lib().rl_specdec_verify_tree(self.h, B, V, N, target._c(B, who),
-                                           draft._c(B, who) if draft is not None else None, _ptr(tokens), _ptr(parent),
-                                           _ptr(n_node), _ptr(accept_u), _ptr(draw_u), _ptr(acc), _ptr(path),
-                                           _ptr(tok), _ptr(prob), _ptr(st), _stream(stream, dev)),
+        t, d = target._of(B, who), draft._of(B, who) if draft is not None else None
+        acc, st = torch.empty_like(n_node), torch.empty_like(n_node)
+        path, tok, prob = torch.empty_like(tokens), torch.empty_like(tokens), torch.empty_like(accept_u)
+        check(lib().rl_specdec_verify_tree(self.h, B, V, N, t, d, tokens.data_ptr(), parent.data_ptr(), n_node.data_ptr(),
+                                           accept_u.data_ptr(), draw_u.data_ptr(), acc.data_ptr(), path.data_ptr(),
+                                           tok.data_ptr(), prob.data_ptr(), st.data_ptr(), _raw_stream(stream, dev)),
               "rl_specdec_verify_tree")
         return acc, path, tok, prob, st
 
