@@ -449,6 +449,49 @@ rl_status rl_lmhead_sample(rl_sampler* h, const uint16_t* hidden, int64_t ldh, c
                            int32_t* row_status, void* stream);
 
 /*
+ * The LM head with 4-bit weights and group scales: a quarter of the bytes that
+ * a decode step reads for its logits (the reference's loader has 4-bit blocks
+ * with one scale, src/quantize.rs, and expands them to f32).
+ *
+ * rl_q4_weight -- weight[v, k] = scale[v, k / group] * (code[v, k] - 8).
+ *   q      rows of H / 2 bytes at row stride ldq bytes (16-byte aligned, ldq a
+ *          multiple of 16). Elements 8 i .. 8 i + 7 of a row are the i-th
+ *          little-endian 32-bit word: element 8 i + 2 j in its bits 4 j .. 4 j
+ *          + 3, element 8 i + 2 j + 1 in bits 16 + 4 j .. 16 + 4 j + 3 (even
+ *          elements in the low half, odd ones in the high half).
+ *   scale  bf16 [V, lds], lds >= H / group
+ *   group  32, 64 or 128; H a multiple of group and of 64
+ * Products are exact in f32 and sums are f32; a group's sum is multiplied by
+ * its scale in f32.
+ *
+ * rl_lmhead_q4_quantize: such a weight from the bf16 one that rl_lmhead_*
+ *   takes (read once, laid out once): per group scale = -m / 8 for the element
+ *   m of the largest magnitude (the first of equals; exact in bf16), code =
+ *   round-half-even(w / scale) + 8 clamped to 0 .. 15; an all-zero group has
+ *   scale 0 and codes 8. A group that holds NaN or an infinity gets a NaN scale.
+ * rl_lmhead_q4_logits / _greedy / _sample: rl_lmhead_logits / _greedy /
+ *   _sample on it (same outputs, same limits on hidden and B).
+ */
+typedef struct {
+  const uint8_t* q;
+  int64_t ldq;
+  const uint16_t* scale;
+  int64_t lds;
+  int32_t group;
+} rl_q4_weight;
+rl_status rl_lmhead_q4_quantize(rl_sampler* h, const uint16_t* weight, int64_t ldw, int H, int V, int group, uint8_t* q,
+                                int64_t ldq, uint16_t* scale, int64_t lds, void* stream);
+rl_status rl_lmhead_q4_logits(rl_sampler* h, const uint16_t* hidden, int64_t ldh, const rl_q4_weight* weight, int B,
+                              int H, int V, void* out_logits, rl_dtype out_dtype, int64_t ldo, void* stream);
+rl_status rl_lmhead_q4_greedy(rl_sampler* h, const uint16_t* hidden, int64_t ldh, const rl_q4_weight* weight, int B,
+                              int H, int V, int32_t* out_tok, int32_t* row_status, float* out_logits, int64_t ldo,
+                              void* stream);
+rl_status rl_lmhead_q4_sample(rl_sampler* h, const uint16_t* hidden, int64_t ldh, const rl_q4_weight* weight, int B,
+                              int H, int V, const int32_t* hist, const int32_t* hist_len, int hist_stride,
+                              const rl_row_params* params, const float* uniforms, int32_t* out_tok, float* out_prob,
+                              int32_t* row_status, void* stream);
+
+/*
  * Vocabulary-sharded sampling (a row's logits split by vocabulary across
  * devices). No single reference function: it splits the spec pipeline above
  * so that each device streams only its columns and the devices exchange 4 KB

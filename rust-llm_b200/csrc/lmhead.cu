@@ -36,6 +36,7 @@
 
 #include "common.cuh"
 #include "internal.h"
+#include "lmhead.cuh"
 
 namespace rl {
 
@@ -58,129 +59,6 @@ struct LmArgs {
   uint64_t* part;        // [B, gridDim.x] packed (value, id) maxima, or null
   int* err;              // set to 1 when a wait runs out
 };
-
-namespace {
-
-__device__ __forceinline__ uint64_t lm_policy_first() {
-  uint64_t p;
-  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
-  return p;
-}
-__device__ __forceinline__ uint64_t lm_policy_last() {
-  uint64_t p;
-  asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(p));
-  return p;
-}
-
-// 2-D tiled TMA load into this CTA's shared memory (no multicast); x is the
-// K coordinate, always a multiple of 64 elements (128 bytes).
-__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar,
-                                            uint64_t policy) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
-      " [%0], [%1, {%3, %4}], [%2], %5;" ::"r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "l"(policy)
-      : "memory");
-}
-
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-// Shared-memory matrix descriptor: K-major operand with the 128-byte swizzle
-// (8-row groups of 1024 bytes: stride byte offset 1024; the leading byte
-// offset is unused for this layout and set to 16 bytes), descriptor version 1.
-__device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr) {
-  return static_cast<uint64_t>((saddr >> 4) & 0x3fffu) | (static_cast<uint64_t>(1u) << 16) |
-         (static_cast<uint64_t>(1024u >> 4) << 32) | (static_cast<uint64_t>(1u) << 46) |
-         (static_cast<uint64_t>(2u) << 61);
-}
-
-// Instruction descriptor of kind::f16: bf16 A and B (both K-major), f32
-// accumulator, M = 128, N = n.
-__device__ __forceinline__ uint32_t lm_idesc(int n) {
-  return (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(128 >> 4) << 24);
-}
-
-__device__ __forceinline__ void umma_bf16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, int acc) {
-  const uint32_t z = 0u;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d_tmem),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc), "r"(z), "r"(z), "r"(z), "r"(z)
-      : "memory");
-}
-
-// Arrives on `bar` once every tcgen05 operation this thread issued before it
-// has completed.
-__device__ __forceinline__ void umma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
-}
-
-__device__ __forceinline__ void mbar_arrive1(uint64_t* bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-
-// 32 TMEM lanes (this warp's quadrant) x 16 columns: register j of lane l is
-// column col + j of lane (quadrant base + l).
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
-      "[%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
-
-// (value, id) packed so that the larger u64 is the later maximum: the
-// greedy_sample order (last maximum; -0.0 and +0.0 tie).
-__device__ __forceinline__ uint64_t lm_key(float v, int id) {
-  return (static_cast<uint64_t>(ord_key(__fadd_rn(v, 0.0f))) << 32) | static_cast<uint32_t>(id);
-}
-__device__ __forceinline__ uint64_t umax64(uint64_t a, uint64_t b) { return a > b ? a : b; }
-__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int o) {
-  const uint32_t lo = __shfl_xor_sync(0xffffffffu, static_cast<uint32_t>(v), o);
-  const uint32_t hi = __shfl_xor_sync(0xffffffffu, static_cast<uint32_t>(v >> 32), o);
-  return (static_cast<uint64_t>(hi) << 32) | lo;
-}
-
-// Per-column maximum over the warp's 32 lanes for 16 columns, by a
-// transposing butterfly (31 exchanges instead of 16 x 5): afterwards lane l
-// holds column (l & 15).
-__device__ __forceinline__ uint64_t warp_colmax16(uint64_t (&k)[16]) {
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int j = 0; j < 16; ++j) k[j] = umax64(k[j], shfl_xor64(k[j], 16));
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const bool up = (lane & 8) != 0;
-    const uint64_t send = up ? k[j] : k[j + 8];
-    const uint64_t keep = up ? k[j + 8] : k[j];
-    k[j] = umax64(keep, shfl_xor64(send, 8));
-  }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const bool up = (lane & 4) != 0;
-    const uint64_t send = up ? k[j] : k[j + 4];
-    const uint64_t keep = up ? k[j + 4] : k[j];
-    k[j] = umax64(keep, shfl_xor64(send, 4));
-  }
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const bool up = (lane & 2) != 0;
-    const uint64_t send = up ? k[j] : k[j + 2];
-    const uint64_t keep = up ? k[j + 2] : k[j];
-    k[j] = umax64(keep, shfl_xor64(send, 2));
-  }
-  const bool up = (lane & 1) != 0;
-  const uint64_t send = up ? k[0] : k[1];
-  const uint64_t keep = up ? k[1] : k[0];
-  return umax64(keep, shfl_xor64(send, 1));
-}
-
-}  // namespace
 
 __global__ void __launch_bounds__(kLmThreads, 1)
     lmhead_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
@@ -399,20 +277,6 @@ EncodeTiledFn encode_fn() {
   return f;
 }
 
-// A [rows, H] bf16 matrix (row stride ld elements) as 64 x box_rows tiles
-// with the 128-byte swizzle; rows past the end read as zeros.
-bool make_map(CUtensorMap* m, const void* ptr, int H, int rows, int64_t ld, int box_rows) {
-  EncodeTiledFn f = encode_fn();
-  if (!f) return false;
-  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(H), static_cast<cuuint64_t>(rows)};
-  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * 2u};
-  const cuuint32_t box[2] = {static_cast<cuuint32_t>(kLmBK), static_cast<cuuint32_t>(box_rows)};
-  const cuuint32_t estr[2] = {1u, 1u};
-  return f(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, estr,
-           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 uint32_t pow2_cols(int n) {
   uint32_t c = 32u;
   while (c < static_cast<uint32_t>(n)) c <<= 1;
@@ -420,6 +284,29 @@ uint32_t pow2_cols(int n) {
 }
 
 }  // namespace
+
+bool lm_tensor_map(CUtensorMap* m, const void* ptr, int elem_bytes, int inner, int rows, int64_t stride, int box_rows) {
+  EncodeTiledFn f = encode_fn();
+  if (!f) return false;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride)};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / elem_bytes), static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t estr[2] = {1u, 1u};
+  return f(m, elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr),
+           dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+cudaError_t lm_argmax(const uint64_t* part, int B, int G, const int* err, int32_t* out_tok, int32_t* row_status,
+                      cudaStream_t stream) {
+  lmhead_argmax_kernel<<<(B + 7) / 8, 256, 0, stream>>>(part, B, G, err, out_tok, row_status);
+  return cudaGetLastError();
+}
+
+cudaError_t lm_flag(const int* err, int B, int32_t* out_tok, int32_t* row_status, cudaStream_t stream) {
+  lmhead_flag_kernel<<<(B + 255) / 256, 256, 0, stream>>>(err, B, out_tok, row_status);
+  return cudaGetLastError();
+}
 
 // The launch geometry of one batch chunk (B <= 256): exposed for the tests
 // of the host checks.
@@ -454,7 +341,7 @@ rl_status lmhead_launch(rl_sampler* h, const uint16_t* hidden, int64_t ldh, cons
   if (cudaMemsetAsync(h->lm_err, 0, sizeof(int), stream) != cudaSuccess)
     return set_error(RL_ERR_CUDA, "rl_lmhead: cudaMemsetAsync failed");
   CUtensorMap mw;
-  if (!make_map(&mw, weight, H, V, ldw, kLmBM))
+  if (!lm_tensor_map(&mw, weight, 2, H, V, ldw * 2, kLmBM))
     return set_error(RL_ERR_INVALID_ARG, "rl_lmhead: weight tensor map rejected (alignment or stride)");
   for (int b0 = 0; b0 < B; b0 += kLmMaxN) {
     const int Bc = B - b0 < kLmMaxN ? B - b0 : kLmMaxN;
@@ -463,7 +350,7 @@ rl_status lmhead_launch(rl_sampler* h, const uint16_t* hidden, int64_t ldh, cons
     size_t smem = 0;
     lmhead_plan(Bc, H, V, h->num_sms, &a, &grid, &smem);
     CUtensorMap mx;
-    if (!make_map(&mx, hidden + static_cast<int64_t>(b0) * ldh, H, Bc, ldh, a.N))
+    if (!lm_tensor_map(&mx, hidden + static_cast<int64_t>(b0) * ldh, 2, H, Bc, ldh * 2, a.N))
       return set_error(RL_ERR_INVALID_ARG, "rl_lmhead: hidden tensor map rejected (alignment or stride)");
     a.out_f32 = out_f32 ? out_f32 + static_cast<int64_t>(b0) * ldo : nullptr;
     a.out_bf16 = out_bf16 ? out_bf16 + static_cast<int64_t>(b0) * ldo : nullptr;
@@ -474,9 +361,7 @@ rl_status lmhead_launch(rl_sampler* h, const uint16_t* hidden, int64_t ldh, cons
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return set_error(RL_ERR_CUDA, cudaGetErrorString(e));
     if (out_tok) {
-      lmhead_argmax_kernel<<<(Bc + 7) / 8, 256, 0, stream>>>(h->lm_part, Bc, grid, h->lm_err, out_tok + b0,
-                                                             row_status ? row_status + b0 : nullptr);
-      e = cudaGetLastError();
+      e = lm_argmax(h->lm_part, Bc, grid, h->lm_err, out_tok + b0, row_status ? row_status + b0 : nullptr, stream);
       if (e != cudaSuccess) return set_error(RL_ERR_CUDA, cudaGetErrorString(e));
     }
   }
@@ -487,18 +372,7 @@ rl_status lmhead_launch(rl_sampler* h, const uint16_t* hidden, int64_t ldh, cons
 
 namespace {
 
-struct LmDeviceGuard {
-  int prev = -1;
-  bool ok = true;
-  explicit LmDeviceGuard(int dev) {
-    if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
-    if (prev != dev) ok = cudaSetDevice(dev) == cudaSuccess;
-  }
-  ~LmDeviceGuard() {
-    int cur = -1;
-    if (prev >= 0 && cudaGetDevice(&cur) == cudaSuccess && cur != prev) cudaSetDevice(prev);
-  }
-};
+using rl::LmDeviceGuard;
 
 rl_status lm_check(rl_sampler* h, const uint16_t* hidden, int64_t ldh, const uint16_t* weight, int64_t ldw, int B,
                    int H, int V, const char* who) {
@@ -570,8 +444,7 @@ rl_status rl_lmhead_sample(rl_sampler* h, const uint16_t* hidden, int64_t ldh, c
                        out_tok, out_prob, row_status, stream);
   if (st != RL_OK) return st;
   // a GEMM whose wait ran out leaves its rows' logits undefined
-  rl::lmhead_flag_kernel<<<(B + 255) / 256, 256, 0, s>>>(h->lm_err, B, out_tok, row_status);
-  cudaError_t e = cudaGetLastError();
+  cudaError_t e = rl::lm_flag(h->lm_err, B, out_tok, row_status, s);
   if (e != cudaSuccess) return rl::set_error(RL_ERR_CUDA, cudaGetErrorString(e));
   return RL_OK;
 }

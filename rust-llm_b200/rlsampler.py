@@ -70,6 +70,13 @@ class _DistRows(ctypes.Structure):
                 ("cut", ctypes.c_void_p), ("cut_stride", ctypes.c_int64), ("first_row", ctypes.c_void_p)]
 
 
+class _Q4Weight(ctypes.Structure):
+    """rl_q4_weight."""
+
+    _fields_ = [("q", ctypes.c_void_p), ("ldq", ctypes.c_int64), ("scale", ctypes.c_void_p), ("lds", ctypes.c_int64),
+                ("group", ctypes.c_int32)]
+
+
 VERIFY_MAX_NODES = 256  # RL_VERIFY_MAX_NODES
 
 
@@ -182,6 +189,15 @@ def lib():
         L.rl_lmhead_greedy.argtypes = [P, P, I64, P, I64, I, I, I, P, P, P, I64, P]
         L.rl_lmhead_sample.restype = I
         L.rl_lmhead_sample.argtypes = [P, P, I64, P, I64, I, I, I, P, P, I, P, P, P, P, P, P]
+        W = ctypes.POINTER(_Q4Weight)
+        L.rl_lmhead_q4_quantize.restype = I
+        L.rl_lmhead_q4_quantize.argtypes = [P, P, I64, I, I, I, P, I64, P, I64, P]
+        L.rl_lmhead_q4_logits.restype = I
+        L.rl_lmhead_q4_logits.argtypes = [P, P, I64, W, I, I, I, P, I, I64, P]
+        L.rl_lmhead_q4_greedy.restype = I
+        L.rl_lmhead_q4_greedy.argtypes = [P, P, I64, W, I, I, I, P, P, P, I64, P]
+        L.rl_lmhead_q4_sample.restype = I
+        L.rl_lmhead_q4_sample.argtypes = [P, P, I64, W, I, I, I, P, P, I, P, P, P, P, P, P]
         _lib = L
     return _lib
 
@@ -276,6 +292,47 @@ class DistRows:
 def _wrong(who, name, t, dtype, shape, dev):
     return ValueError(f"{who}: {name} must be contiguous {dtype} {tuple(shape)} on {dev}, got {t.dtype} {tuple(t.shape)} "
                       f"on {t.device}")
+
+
+class Q4Weight:
+    """4-bit weights with group scales (rl_q4_weight): q [V, H / 2] uint8 packed
+    codes, scale [V, H / group] bf16; weight = scale * (code - 8)."""
+
+    __slots__ = ("q", "scale", "group", "V", "H", "device", "c")
+
+    def __init__(self, q, scale, group):
+        import torch
+
+        if q.dtype is not torch.uint8 or q.dim() != 2 or (q.shape[1] > 1 and q.stride(1) != 1):
+            raise ValueError("Q4Weight: q must be rows of uint8 codes [V, H / 2]")
+        if scale.dtype is not torch.bfloat16 or scale.dim() != 2 or (scale.shape[1] > 1 and scale.stride(1) != 1):
+            raise ValueError("Q4Weight: scale must be rows of bf16 [V, H / group]")
+        V, H = q.shape[0], 2 * q.shape[1]
+        if scale.shape[0] != V or scale.shape[1] * group != H or scale.device != q.device:
+            raise ValueError(f"Q4Weight: scale {tuple(scale.shape)} on {scale.device} does not fit {V} rows of {H} codes "
+                             f"in groups of {group} on {q.device}")
+        self.q, self.scale, self.group, self.V, self.H, self.device = q, scale, group, V, H, q.device
+        # a single row has no stride to speak of
+        self.c = _Q4Weight(q.data_ptr(), q.stride(0) if V > 1 else (H // 2 + 15) // 16 * 16, scale.data_ptr(),
+                           scale.stride(0) if V > 1 else H // group, group)
+
+
+def q4_pack(codes):
+    """Codes 0 .. 15 [V, H] as the packed bytes [V, H / 2] of rl_q4_weight."""
+    import torch
+
+    V, H = codes.shape
+    shifts = torch.tensor([0, 16, 4, 20, 8, 24, 12, 28], dtype=torch.int64, device=codes.device)
+    word = (codes.to(torch.int64).view(V, H // 8, 8) << shifts).sum(2)
+    return torch.where(word >= 1 << 31, word - (1 << 32), word).to(torch.int32).view(torch.uint8)
+
+
+def q4_unpack(q):
+    """The codes 0 .. 15 [V, H] uint8 of packed bytes [V, H / 2]."""
+    import torch
+
+    shifts = torch.tensor([0, 16, 4, 20, 8, 24, 12, 28], dtype=torch.int32, device=q.device)
+    return ((q.contiguous().view(torch.int32)[:, :, None] >> shifts) & 15).flatten(1).to(torch.uint8)
 
 
 class Sampler:
@@ -669,6 +726,92 @@ class Sampler:
                                      _ptr(out_prob), _ptr(row_status), _stream(stream)),
               "rl_lmhead_sample")
         return out_tok, out_prob, row_status
+
+    # -- LM head, 4-bit weights ------------------------------------------------
+    def lmhead_q4_quantize(self, weight, group=128, stream=None):
+        """rl_lmhead_q4_quantize: a bf16 weight [V, H] as a Q4Weight."""
+        import torch
+
+        if weight.dtype is not torch.bfloat16 or weight.dim() != 2 or weight.stride(1) != 1:
+            raise ValueError("lmhead_q4_quantize: weight must be row-major bf16 [V, H]")
+        V, H = weight.shape
+        if group not in (32, 64, 128) or H % 64 or H % group:
+            raise ValueError("lmhead_q4_quantize: group must be 32, 64 or 128, H a multiple of it and of 64")
+        dev = weight.device
+        q = torch.empty(V, H // 2, dtype=torch.uint8, device=dev)
+        scale = torch.empty(V, H // group, dtype=torch.bfloat16, device=dev)
+        w = Q4Weight(q, scale, group)
+        check(lib().rl_lmhead_q4_quantize(self.h, weight.data_ptr(), weight.stride(0) if V > 1 else max(weight.stride(0), H), H, V,
+                                          group, w.c.q, w.c.ldq, w.c.scale, w.c.lds, _raw_stream(stream, dev)),
+              "rl_lmhead_q4_quantize")
+        return w
+
+    @staticmethod
+    def _q4_operands(hidden, weight):
+        import torch
+
+        if hidden.dtype is not torch.bfloat16 or hidden.dim() != 2 or hidden.stride(1) != 1:
+            raise ValueError("lmhead_q4: hidden must be row-major bf16 [B, H]")
+        B, H = hidden.shape
+        if H != weight.H or hidden.device != weight.device:
+            raise ValueError(f"lmhead_q4: hidden has {H} columns on {hidden.device}, weight {weight.H} on {weight.device}")
+        return B, H, hidden.stride(0) if B > 1 else max(hidden.stride(0), H)
+
+    @staticmethod
+    def _q4_out(out, B, V, dev, dtypes):
+        if out.dtype not in dtypes or out.shape != (B, V) or out.device != dev or (V > 1 and out.stride(1) != 1):
+            raise ValueError(f"lmhead_q4: out must be row-major {dtypes} [{B}, {V}] on {dev}")
+        return out.stride(0) if B > 1 else max(out.stride(0), V)
+
+    def lmhead_q4_logits(self, hidden, weight, out=None, out_dtype=None, stream=None):
+        """rl_lmhead_q4_logits: hidden [B, H] bf16 times a Q4Weight [V, H] into
+        out [B, V] (f32 or bf16)."""
+        import torch
+
+        B, H, ldh = self._q4_operands(hidden, weight)
+        V, dev = weight.V, hidden.device
+        if out is None:
+            out = torch.empty((B, V), dtype=out_dtype or torch.float32, device=dev)
+        ldo = self._q4_out(out, B, V, dev, (torch.float32, torch.bfloat16))
+        check(lib().rl_lmhead_q4_logits(self.h, hidden.data_ptr(), ldh, weight.c, B, H, V, out.data_ptr(),
+                                        RL_BF16 if out.dtype is torch.bfloat16 else RL_F32, ldo, _raw_stream(stream, dev)),
+              "rl_lmhead_q4_logits")
+        return out
+
+    def lmhead_q4_greedy(self, hidden, weight, out_logits=None, stream=None):
+        """rl_lmhead_q4_greedy: the last-maximum argmax of each row's logits.
+        Returns (tokens [B], row_status [B]); out_logits (f32 [B, V],
+        optional) also receives the logits."""
+        import torch
+
+        B, H, ldh = self._q4_operands(hidden, weight)
+        V, dev = weight.V, hidden.device
+        tok = torch.empty(B, dtype=torch.int32, device=dev)
+        st = torch.empty_like(tok)
+        ldo = self._q4_out(out_logits, B, V, dev, (torch.float32,)) if out_logits is not None else V
+        check(lib().rl_lmhead_q4_greedy(self.h, hidden.data_ptr(), ldh, weight.c, B, H, V, tok.data_ptr(), st.data_ptr(),
+                                        out_logits.data_ptr() if out_logits is not None else None, ldo,
+                                        _raw_stream(stream, dev)),
+              "rl_lmhead_q4_greedy")
+        return tok, st
+
+    def lmhead_q4_sample(self, hidden, weight, params, uniforms, hist=None, hist_len=None, stream=None):
+        """rl_lmhead_q4_sample: the 4-bit LM head's logits sampled by the batched
+        sampler (same params / uniforms / history as sample()). Returns
+        (tokens, probs, row_status)."""
+        import torch
+
+        B, H, ldh = self._q4_operands(hidden, weight)
+        dev = hidden.device
+        tok = torch.empty(B, dtype=torch.int32, device=dev)
+        prob = torch.empty(B, dtype=torch.float32, device=dev)
+        st = torch.empty_like(tok)
+        hs = hist.shape[1] if hist is not None else 0
+        check(lib().rl_lmhead_q4_sample(self.h, hidden.data_ptr(), ldh, weight.c, B, H, weight.V, _ptr(hist), _ptr(hist_len),
+                                        hs, _ptr(params), _ptr(uniforms), tok.data_ptr(), prob.data_ptr(), st.data_ptr(),
+                                        _raw_stream(stream, dev)),
+              "rl_lmhead_q4_sample")
+        return tok, prob, st
 
     def sample_host_ptrs(self, logits_p, B, V, params_p, u_p, tok_p, prob_p, hist_p=None, hist_len_p=None,
                          hist_stride=0, mask_p=None, mask_stride=0):
