@@ -6,8 +6,28 @@
 // code - 8 is a whole number in [-8, 7], so code - 8 times a bf16 value is exact
 // in f32; a group's sum is multiplied by its scale once, in f32.
 //
-// A warp takes a vocabulary row, its lanes the row's words, for up to eight
-// batch rows at a time.
+// On the tensor cores: one persistent CTA per SM walks tiles of 128 vocabulary
+// rows (MMA M = 128, N = batch rows padded, K in stages of 64):
+//   warp 0        TMA producer of the codes: [128 rows x 256 codes] a copy, 128
+//                 bytes of a row, 128-byte swizzle
+//   warp 2        TMA producer of the hidden states: [N x 64] a stage
+//   warp 3        copies the scales: [128 rows x 8 groups] a box
+//   warps 4-11    turn codes into bf16 (a thread a row: code | 0x4300 is 128 +
+//                 code, less 136) and store them into TMEM, from where the MMA
+//                 reads them as its A operand: expanded weights never pass
+//                 through shared memory, which would take four times the bytes
+//                 of the codes in and again out
+//   warp 1        tcgen05.mma kind::f16, one accumulator in TMEM for each group
+//   warps 12-...  read a group's accumulator back, times the row's scale (a
+//                 thread a row), into f32 sums in registers; at the tile's end
+//                 logits are stored along the vocabulary, or the rows' running
+//                 maxima kept
+// Multiplying the scale in behind the MMA keeps the operands exact (code - 8
+// has four bits) for scales of any size, at N / group FMAs a weight.
+//
+// Bound: HBM, half a byte a weight, up to about 100 batch rows; beside it the
+// expansion, 11 instructions for 8 weights. Every wait is bounded; where one
+// runs out the error flag is set, copies in flight land and TMEM is freed.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -21,65 +41,385 @@
 namespace rl {
 namespace {
 
-constexpr int kQ4Rows = 256;  // batch rows a launch handles (the size of the argmax workspace)
+constexpr int kBM = 128;        // vocabulary rows of a tile
+constexpr int kQTile = kBM * 128;  // bytes of a copy of codes: 256 codes of each row
+constexpr int kASlots = 4;      // expanded stages in TMEM, 32 columns each
+constexpr int kACols = 32;
+constexpr int kDCols = 512 - kASlots * kACols;  // columns for the accumulators
+constexpr int kDMax = 4;        // accumulator buffers, at most
+constexpr int kSBox = kBM * 16;  // bytes of a box of scales: 8 groups of each row
+constexpr int kSSlots = 8;
+constexpr int kQMax = 8, kXMax = 16;
 
 struct Q4Args {
-  const uint16_t* hidden;
-  int64_t ldh;
-  const uint8_t* q;
-  int64_t ldq;
+  int B, H, V;
+  int gshift;              // log2(group)
+  int ntiles, kstages;     // kstages = H / 64
+  int unit;                // stages between two hand-overs of accumulators (1 or 2)
+  int dbufs, dcols;        // accumulator buffers and their columns
+  int qslots, xslots;
   const uint16_t* scale;
   int64_t lds;
-  int gshift;  // log2(group)
-  int B, H, V;
+  int gran;                // bytes of a copy of scales: 16, 8, 4, or 2 (loads)
   float* out_f32;
   uint16_t* out_bf16;
   int64_t ldo;
-  uint64_t* part;  // [B] packed (value, id) maxima, or null
+  uint64_t* part;          // [B, gridDim.x] packed (value, id) maxima, or null
+  int* err;
 };
 
 __device__ __forceinline__ float bf16_at(uint32_t w, int hi) { return __uint_as_float(hi ? w & 0xffff0000u : w << 16); }
 
-__global__ void __launch_bounds__(256) q4_row_kernel(const __grid_constant__ Q4Args a) {
-  const int v = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (v >= a.V) return;
-  const uint32_t* q = reinterpret_cast<const uint32_t*>(a.q + static_cast<int64_t>(v) * a.ldq);
-  const uint16_t* sc = a.scale + static_cast<int64_t>(v) * a.lds;
-  for (int b0 = 0; b0 < a.B; b0 += 8) {
-    float acc[8] = {};
-    for (int w = lane; w < (a.H >> 3); w += 32) {
-      const uint32_t x = q[w];
-      const float s = bf16_bits_to_f32(sc[(w << 3) >> a.gshift]);
-      float c[8];
+// D (+)= A B^T with A (bf16, M = 128, K = 16) in TMEM columns and B in shared memory.
+__device__ __forceinline__ void umma_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, int acc) {
+  const uint32_t z = 0u;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(acc), "r"(z), "r"(z), "r"(z), "r"(z)
+      : "memory");
+}
+
+// This warp's 32 lanes x 32 columns of TMEM: register j is column j.
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+// Eight codes of a word as bf16 code - 8, in element order.
+__device__ __forceinline__ void expand(uint32_t w, uint32_t* out) {
+  const __nv_bfloat162 c136 = __halves2bfloat162(__ushort_as_bfloat16(0x4308), __ushort_as_bfloat16(0x4308));
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        c[2 * j] = static_cast<float>(static_cast<int>((x >> (4 * j)) & 15u) - 8);
-        c[2 * j + 1] = static_cast<float>(static_cast<int>((x >> (16 + 4 * j)) & 15u) - 8);
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t x = ((w >> (4 * j)) & 0x000f000fu) | 0x43004300u;  // 128 + code
+    __nv_bfloat162 v;
+    *reinterpret_cast<uint32_t*>(&v) = x;
+    v = __hsub2(v, c136);
+    out[j] = *reinterpret_cast<uint32_t*>(&v);
+  }
+}
+
+struct Q4Bars {
+  uint64_t qfull[kQMax], qempty[kQMax];
+  uint64_t xfull[kXMax], xempty[kXMax];
+  uint64_t afull[kASlots], aempty[kASlots];
+  uint64_t dfull[kDMax], dempty[kDMax];
+  uint64_t sfull[kSSlots], sempty[kSSlots];
+  uint64_t done;
+  uint32_t tmem;
+};
+
+// A ring position: slot and the parity of its present use.
+struct Ring {
+  int slot = 0;
+  uint32_t par = 0;
+  __device__ __forceinline__ void next(int n) {
+    if (++slot == n) {
+      slot = 0;
+      par ^= 1u;
+    }
+  }
+};
+
+template <int N, int NEP>  // MMA N; epilogue warps
+__global__ void __launch_bounds__((12 + NEP) * 32, 1)
+    q4_mma_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmX,
+                  const __grid_constant__ Q4Args a) {
+  extern __shared__ uint8_t q4_smem_raw[];
+  __shared__ Q4Bars bars;
+  __shared__ unsigned long long best[N];
+  constexpr int NC = N / (NEP / 4);  // columns of an epilogue warp
+  constexpr uint32_t kXBytes = N * 128;
+  uint8_t* qring = q4_smem_raw + ((1024u - (smem_u32(q4_smem_raw) & 1023u)) & 1023u);
+  uint8_t* xring = qring + a.qslots * kQTile;
+  uint8_t* sring = xring + a.xslots * kXBytes;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < a.qslots; ++i) mbar_init(&bars.qfull[i], 1), mbar_init(&bars.qempty[i], 8);
+    for (int i = 0; i < a.xslots; ++i) mbar_init(&bars.xfull[i], 1), mbar_init(&bars.xempty[i], 1);
+    for (int i = 0; i < kASlots; ++i) mbar_init(&bars.afull[i], 4), mbar_init(&bars.aempty[i], 1);
+    for (int i = 0; i < a.dbufs; ++i) mbar_init(&bars.dfull[i], 1), mbar_init(&bars.dempty[i], NEP);
+    for (int i = 0; i < kSSlots; ++i) mbar_init(&bars.sfull[i], 32), mbar_init(&bars.sempty[i], NEP);
+    mbar_init(&bars.done, 1);
+    fence_mbar_init();
+  }
+  for (int i = threadIdx.x; i < N; i += blockDim.x) best[i] = 0ull;
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars.tmem)), "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    tc_fence_before();
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars.tmem;
+  const uint32_t tmem_a = tmem + kDCols;  // the expanded stages lie behind the accumulators
+  const int qtiles = (a.kstages + 3) >> 2;  // copies of codes a tile
+  const int ngroups = a.H >> a.gshift;
+  bool ok = true;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // ---- codes ----
+      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmQ)) : "memory");
+      const uint64_t pol = lm_policy_first();  // streamed once
+      Ring r;
+      uint32_t it = 0;
+      for (int tile = blockIdx.x; tile < a.ntiles && ok; tile += gridDim.x) {
+        for (int t = 0; t < qtiles; ++t, ++it) {
+          if (!mbar_wait(&bars.qempty[r.slot], r.par ^ 1u, kWaitBudget)) {
+            ok = false;
+            break;
+          }
+          mbar_expect_tx(&bars.qfull[r.slot], kQTile);
+          tma_load_2d(qring + r.slot * kQTile, &tmQ, t * 128, tile * kBM, &bars.qfull[r.slot], pol);
+          r.next(a.qslots);
+        }
       }
+      // every issued copy lands before the CTA may return
+      for (int i = 0; i < a.qslots; ++i) {
+        const uint32_t n = it / a.qslots + (static_cast<uint32_t>(i) < it % a.qslots ? 1u : 0u);
+        if (n > 0 && !mbar_wait(&bars.qfull[i], (n - 1u) & 1u, kWaitBudget)) ok = false;
+      }
+    }
+  } else if (warp == 2) {
+    if (lane == 0) {
+      // ---- hidden states ----
+      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmX)) : "memory");
+      const uint64_t pol = lm_policy_last();  // read by every CTA, for every tile
+      Ring r;
+      uint32_t it = 0;
+      for (int tile = blockIdx.x; tile < a.ntiles && ok; tile += gridDim.x) {
+        for (int kb = 0; kb < a.kstages; ++kb, ++it) {
+          if (!mbar_wait(&bars.xempty[r.slot], r.par ^ 1u, kWaitBudget)) {
+            ok = false;
+            break;
+          }
+          mbar_expect_tx(&bars.xfull[r.slot], kXBytes);
+          tma_load_2d(xring + r.slot * kXBytes, &tmX, kb * 64, 0, &bars.xfull[r.slot], pol);
+          r.next(a.xslots);
+        }
+      }
+      for (int i = 0; i < a.xslots; ++i) {
+        const uint32_t n = it / a.xslots + (static_cast<uint32_t>(i) < it % a.xslots ? 1u : 0u);
+        if (n > 0 && !mbar_wait(&bars.xfull[i], (n - 1u) & 1u, kWaitBudget)) ok = false;
+      }
+    }
+  } else if (warp == 3) {
+    // ---- scales: a lane copies rows lane, lane + 32, ... ----
+    Ring r;
+    for (int tile = blockIdx.x; tile < a.ntiles && ok; tile += gridDim.x) {
+      for (int g0 = 0; g0 < ngroups && ok; g0 += 8) {
+        if (!mbar_wait(&bars.sempty[r.slot], r.par ^ 1u, kWaitBudget)) {
+          ok = false;
+          break;
+        }
+        const int bytes = 2 * min(8, ngroups - g0);
+        uint8_t* box = sring + r.slot * kSBox;
 #pragma unroll
-      for (int b = 0; b < 8; ++b) {
-        if (b0 + b < a.B) {
-          const uint4 h = *reinterpret_cast<const uint4*>(a.hidden + static_cast<int64_t>(b0 + b) * a.ldh + 8 * w);
-          const uint32_t hw[4] = {h.x, h.y, h.z, h.w};
-          float d = 0.0f;
+        for (int i = 0; i < 4; ++i) {
+          const int row = 32 * i + lane;
+          const int64_t v = static_cast<int64_t>(tile) * kBM + row;
+          if (v >= a.V) continue;
+          const uint8_t* src = reinterpret_cast<const uint8_t*>(a.scale + v * a.lds + g0);
+          const uint32_t dst = smem_u32(box + row * 16);
+          if (a.gran == 16) {
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+          } else if (a.gran == 8) {
+            for (int o = 0; o < bytes; o += 8)
+              asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst + o), "l"(src + o) : "memory");
+          } else if (a.gran == 4) {
+            for (int o = 0; o < bytes; o += 4)
+              asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + o), "l"(src + o) : "memory");
+          } else {
+            for (int o = 0; o < bytes; o += 2)
+              *reinterpret_cast<uint16_t*>(box + row * 16 + o) = *reinterpret_cast<const uint16_t*>(src + o);
+          }
+        }
+        // arrives once this lane's copies have landed
+        if (a.gran > 2)
+          asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&bars.sfull[r.slot])) : "memory");
+        else
+          mbar_arrive1(&bars.sfull[r.slot]);
+        r.next(kSSlots);
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else if (warp == 1) {
+    if (lane == 0) {
+      // ---- MMA issuer ----
+      const uint32_t idesc = lm_idesc(N);
+      const int gsteps = 1 << (a.gshift - 4);  // K = 16 steps of a group
+      Ring ra, rx, rd;
+      for (int tile = blockIdx.x; tile < a.ntiles && ok; tile += gridDim.x) {
+        for (int kb = 0; kb < a.kstages && ok; ++kb) {
+          const int in_unit = kb % a.unit;
+          if (in_unit == 0 && !mbar_wait(&bars.dempty[rd.slot], rd.par ^ 1u, kWaitBudget)) {
+            ok = false;
+            break;
+          }
+          if (!mbar_wait(&bars.xfull[rx.slot], rx.par, kWaitBudget) || !mbar_wait(&bars.afull[ra.slot], ra.par, kWaitBudget)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint64_t bd = sw128_desc(smem_u32(xring + rx.slot * kXBytes));
+          const uint32_t at = tmem_a + static_cast<uint32_t>(ra.slot * kACols);
+          const uint32_t d0 = tmem + static_cast<uint32_t>(rd.slot * a.dcols);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) d = fmaf(c[k], bf16_at(hw[k >> 1], k & 1), d);
-          acc[b] = fmaf(s, d, acc[b]);
+          for (int k = 0; k < 4; ++k) {
+            const int step = 4 * in_unit + k;  // of the unit
+            umma_ta(d0 + static_cast<uint32_t>((step / gsteps) * N), at + 8u * k, bd + 2u * k, idesc, step % gsteps != 0);
+          }
+          umma_commit(&bars.aempty[ra.slot]);
+          umma_commit(&bars.xempty[rx.slot]);
+          ra.next(kASlots);
+          rx.next(a.xslots);
+          if (in_unit == a.unit - 1 || kb == a.kstages - 1) {
+            umma_commit(&bars.dfull[rd.slot]);
+            rd.next(a.dbufs);
+          }
+        }
+      }
+      // every MMA of this CTA completes before its TMEM is freed
+      umma_commit(&bars.done);
+      if (!mbar_wait(&bars.done, 0u, kWaitBudget)) ok = false;
+    }
+  } else if (warp < 12) {
+    // ---- codes into bf16: every other stage of this warp's 32 rows ----
+    const int quad = warp & 3, mine = (warp - 4) >> 2;
+    const int row = quad * 32 + lane;
+    Ring rq, ra;
+    uint32_t g = 0;  // stages so far
+    for (int tile = blockIdx.x; tile < a.ntiles && ok; tile += gridDim.x) {
+      for (int t = 0; t < qtiles && ok; ++t) {
+        if (!mbar_wait(&bars.qfull[rq.slot], rq.par, kWaitBudget)) {
+          ok = false;
+          break;
+        }
+        const uint8_t* src = qring + rq.slot * kQTile + row * 128;
+        const int ns = min(4, a.kstages - 4 * t);
+        for (int s = 0; s < ns; ++s, ++g) {
+          if (static_cast<int>(g & 1u) == mine) {
+            const uint4 c0 = *reinterpret_cast<const uint4*>(src + (((2 * s) ^ (row & 7)) << 4));
+            const uint4 c1 = *reinterpret_cast<const uint4*>(src + (((2 * s + 1) ^ (row & 7)) << 4));
+            uint32_t e[32];
+            expand(c0.x, e);
+            expand(c0.y, e + 4);
+            expand(c0.z, e + 8);
+            expand(c0.w, e + 12);
+            expand(c1.x, e + 16);
+            expand(c1.y, e + 20);
+            expand(c1.z, e + 24);
+            expand(c1.w, e + 28);
+            if (!mbar_wait(&bars.aempty[ra.slot], ra.par ^ 1u, kWaitBudget)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            tmem_st32(tmem_a + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(ra.slot * kACols), e);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive1(&bars.afull[ra.slot]);
+          }
+          ra.next(kASlots);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive1(&bars.qempty[rq.slot]);
+        rq.next(a.qslots);
+      }
+    }
+  } else {
+    // ---- epilogue ----
+    const int quad = warp & 3;
+    const int col0 = ((warp - 12) >> 2) * NC;
+    const int row = quad * 32 + lane;
+    Ring rd, rs;
+    for (int tile = blockIdx.x; tile < a.ntiles && ok; tile += gridDim.x) {
+      float acc[NC];
+#pragma unroll
+      for (int j = 0; j < NC; ++j) acc[j] = 0.0f;
+      uint4 sc = {0u, 0u, 0u, 0u};  // the scales of 8 groups
+      int g = 0;
+      for (int kb = 0; kb < a.kstages && ok; kb += a.unit) {
+        const int n_in = (min(a.unit, a.kstages - kb) * 64) >> a.gshift;
+        if (!mbar_wait(&bars.dfull[rd.slot], rd.par, kWaitBudget)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        for (int i = 0; i < n_in; ++i, ++g) {
+          if ((g & 7) == 0) {
+            if (!mbar_wait(&bars.sfull[rs.slot], rs.par, kWaitBudget)) {
+              ok = false;
+              break;
+            }
+            sc = *reinterpret_cast<const uint4*>(sring + rs.slot * kSBox + row * 16);
+            __syncwarp();
+            if (lane == 0) mbar_arrive1(&bars.sempty[rs.slot]);
+            rs.next(kSSlots);
+          }
+          const uint32_t sw = (g & 6) == 0 ? sc.x : (g & 6) == 2 ? sc.y : (g & 6) == 4 ? sc.z : sc.w;
+          const float s = bf16_at(sw, g & 1);
+          const uint32_t at = tmem + (static_cast<uint32_t>(quad * 32) << 16) +
+                              static_cast<uint32_t>(rd.slot * a.dcols + i * N + col0);
+#pragma unroll
+          for (int c = 0; c < NC; c += 16) {
+            uint32_t r[16];
+            tmem_ld16(at + static_cast<uint32_t>(c), r);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) acc[c + j] = fmaf(s, __uint_as_float(r[j]), acc[c + j]);
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive1(&bars.dempty[rd.slot]);
+        rd.next(a.dbufs);
+      }
+      if (!ok) break;
+      const int64_t v = static_cast<int64_t>(tile) * kBM + row;
+      const bool vin = v < a.V;
+      if (vin && a.out_f32) {
+#pragma unroll
+        for (int j = 0; j < NC; ++j)
+          if (col0 + j < a.B) a.out_f32[static_cast<int64_t>(col0 + j) * a.ldo + v] = acc[j];
+      }
+      if (vin && a.out_bf16) {
+#pragma unroll
+        for (int j = 0; j < NC; ++j)
+          if (col0 + j < a.B)
+            a.out_bf16[static_cast<int64_t>(col0 + j) * a.ldo + v] = __bfloat16_as_ushort(__float2bfloat16_rn(acc[j]));
+      }
+      if (a.part) {
+#pragma unroll
+        for (int c = 0; c < NC; c += 16) {
+          uint64_t k[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) k[j] = vin ? lm_key(acc[c + j], static_cast<int>(v)) : 0ull;
+          const uint64_t m = warp_colmax16(k);
+          if (lane < 16 && col0 + c + lane < a.B)
+            atomicMax(&best[col0 + c + lane], static_cast<unsigned long long>(m));
         }
       }
     }
-#pragma unroll
-    for (int b = 0; b < 8; ++b) {
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) acc[b] += __shfl_xor_sync(0xffffffffu, acc[b], o);
-      if (lane == 0 && b0 + b < a.B) {
-        const int64_t at = static_cast<int64_t>(b0 + b) * a.ldo + v;
-        if (a.out_f32) a.out_f32[at] = acc[b];
-        if (a.out_bf16) a.out_bf16[at] = __bfloat16_as_ushort(__float2bfloat16_rn(acc[b]));
-        if (a.part)
-          atomicMax(reinterpret_cast<unsigned long long*>(&a.part[b0 + b]), static_cast<unsigned long long>(lm_key(acc[b], v)));
-      }
-    }
+  }
+  if (!ok) atomicExch(a.err, 1);
+  __syncthreads();
+  if (a.part)
+    for (int b = threadIdx.x; b < a.B; b += blockDim.x) a.part[static_cast<int64_t>(b) * gridDim.x + blockIdx.x] = best[b];
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
   }
 }
 
@@ -166,35 +506,74 @@ rl_status q4_check(rl_sampler* h, const uint16_t* hidden, int64_t ldh, const rl_
   return RL_OK;
 }
 
+// A launch for at most N batch rows.
+template <int N, int NEP>
+cudaError_t q4_run(const CUtensorMap& mq, const CUtensorMap& mx, Q4Args a, int grid, cudaStream_t stream) {
+  const int xbytes = N * 128;
+  a.qslots = kQMax;
+  a.xslots = 64 * 1024 / xbytes < kXMax ? 64 * 1024 / xbytes : kXMax;
+  const int group = 1 << a.gshift;
+  a.unit = group == 128 || 2 * (128 / group) * N <= kDCols ? 2 : 1;
+  a.dcols = N * (64 * a.unit / group);
+  a.dbufs = kDCols / a.dcols < kDMax ? kDCols / a.dcols : kDMax;
+  const size_t smem = 1024 + static_cast<size_t>(a.qslots) * kQTile + static_cast<size_t>(a.xslots) * xbytes + kSSlots * kSBox;
+  static std::atomic<int> configured[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64 || !configured[dev].load(std::memory_order_acquire)) {
+    e = cudaFuncSetAttribute(q4_mma_kernel<N, NEP>, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024);
+    if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64) configured[dev].store(1, std::memory_order_release);
+  }
+  q4_mma_kernel<N, NEP><<<grid, (12 + NEP) * 32, smem, stream>>>(mq, mx, a);
+  return cudaGetLastError();
+}
+
 rl_status q4_launch(rl_sampler* h, const uint16_t* hidden, int64_t ldh, const rl_q4_weight& w, int B, int H, int V,
                     float* out_f32, uint16_t* out_bf16, int64_t ldo, int32_t* out_tok, int32_t* row_status,
                     cudaStream_t stream) {
   if (cudaMemsetAsync(h->lm_err, 0, sizeof(int), stream) != cudaSuccess)
     return set_error(RL_ERR_CUDA, "rl_lmhead_q4: cudaMemsetAsync failed");
-  for (int b0 = 0; b0 < B; b0 += kQ4Rows) {
-    const int Bc = B - b0 < kQ4Rows ? B - b0 : kQ4Rows;
-    Q4Args a = {};
-    a.hidden = hidden + static_cast<int64_t>(b0) * ldh;
-    a.ldh = ldh;
-    a.q = w.q;
-    a.ldq = w.ldq;
-    a.scale = w.scale;
-    a.lds = w.lds;
-    a.gshift = w.group == 32 ? 5 : w.group == 64 ? 6 : 7;
+  CUtensorMap mq;
+  if (!lm_tensor_map(&mq, w.q, 1, H / 2, V, w.ldq, kBM))
+    return set_error(RL_ERR_INVALID_ARG, "rl_lmhead_q4: tensor map of the codes rejected (alignment or stride)");
+  Q4Args a = {};
+  a.H = H;
+  a.V = V;
+  a.gshift = w.group == 32 ? 5 : w.group == 64 ? 6 : 7;
+  a.ntiles = (V + kBM - 1) / kBM;
+  a.kstages = H / 64;
+  a.scale = w.scale;
+  a.lds = w.lds;
+  const uint64_t al = reinterpret_cast<uintptr_t>(w.scale) | static_cast<uint64_t>(w.lds) * 2u |
+                      static_cast<uint64_t>(H / w.group) * 2u;
+  a.gran = al % 16 == 0 ? 16 : al % 8 == 0 ? 8 : al % 4 == 0 ? 4 : 2;
+  a.ldo = ldo;
+  a.err = h->lm_err;
+  const int grid = a.ntiles < h->num_sms ? a.ntiles : h->num_sms;
+  // batch rows a launch: two groups of 32 in a stage take 2 N columns, and two
+  // buffers of them have to fit
+  const int most = w.group == 32 ? 64 : 128;
+  const int chunks = (B + most - 1) / most;
+  const int per = (B + chunks - 1) / chunks;
+  for (int b0 = 0; b0 < B; b0 += per) {
+    const int Bc = B - b0 < per ? B - b0 : per;
     a.B = Bc;
-    a.H = H;
-    a.V = V;
     a.out_f32 = out_f32 ? out_f32 + static_cast<int64_t>(b0) * ldo : nullptr;
     a.out_bf16 = out_bf16 ? out_bf16 + static_cast<int64_t>(b0) * ldo : nullptr;
-    a.ldo = ldo;
     a.part = out_tok ? h->lm_part : nullptr;
-    cudaError_t e = cudaSuccess;
-    if (a.part) e = cudaMemsetAsync(a.part, 0, sizeof(uint64_t) * Bc, stream);
-    if (e != cudaSuccess) return set_error(RL_ERR_CUDA, cudaGetErrorString(e));
-    q4_row_kernel<<<(V + 7) / 8, 256, 0, stream>>>(a);
-    e = cudaGetLastError();
+    const int N = Bc <= 16 ? 16 : Bc <= 32 ? 32 : Bc <= 64 ? 64 : Bc <= 96 ? 96 : 128;
+    CUtensorMap mx;
+    if (!lm_tensor_map(&mx, hidden + static_cast<int64_t>(b0) * ldh, 2, H, Bc, ldh * 2, N))
+      return set_error(RL_ERR_INVALID_ARG, "rl_lmhead_q4: hidden tensor map rejected (alignment or stride)");
+    cudaError_t e = N == 16   ? q4_run<16, 4>(mq, mx, a, grid, stream)
+                    : N == 32 ? q4_run<32, 4>(mq, mx, a, grid, stream)
+                    : N == 64 ? q4_run<64, 8>(mq, mx, a, grid, stream)
+                    : N == 96 ? q4_run<96, 8>(mq, mx, a, grid, stream)
+                              : q4_run<128, 8>(mq, mx, a, grid, stream);
     if (e == cudaSuccess && out_tok)
-      e = lm_argmax(a.part, Bc, 1, h->lm_err, out_tok + b0, row_status ? row_status + b0 : nullptr, stream);
+      e = lm_argmax(h->lm_part, Bc, grid, h->lm_err, out_tok + b0, row_status ? row_status + b0 : nullptr, stream);
     if (e != cudaSuccess) return set_error(RL_ERR_CUDA, cudaGetErrorString(e));
   }
   return RL_OK;
