@@ -7,21 +7,25 @@
 // in f32; a group's sum is multiplied by its scale once, in f32.
 //
 // On the tensor cores: one persistent CTA per SM walks tiles of 128 vocabulary
-// rows (MMA M = 128, N = batch rows padded, K in stages of 64):
+// rows (MMA M = 128, N = batch rows padded, K in blocks of 128):
 //   warp 0        TMA producer of the codes: [128 rows x 256 codes] a copy, 128
 //                 bytes of a row, 128-byte swizzle
-//   warp 2        TMA producer of the hidden states: [N x 64] a stage
+//   warp 2        TMA producer of the hidden states: two [N x 64] a block
 //   warp 3        copies the scales: [128 rows x 8 groups] a box
-//   warps 4-11    turn codes into bf16 (a thread a row: code | 0x4300 is 128 +
-//                 code, less 136) and store them into TMEM, from where the MMA
-//                 reads them as its A operand: expanded weights never pass
-//                 through shared memory, which would take four times the bytes
-//                 of the codes in and again out
-//   warp 1        tcgen05.mma kind::f16, one accumulator in TMEM for each group
-//   warps 12-...  read a group's accumulator back, times the row's scale (a
-//                 thread a row), into f32 sums in registers; at the tile's end
-//                 logits are stored along the vocabulary, or the rows' running
-//                 maxima kept
+//   warps 4-...   (8 or 16) turn codes into bf16 (a thread a row: code | 0x4300
+//                 is 128 + code, less 136) and store them into TMEM, from where
+//                 the MMA reads them as its A operand: expanded weights never
+//                 pass through shared memory, which would take four times the
+//                 bytes of the codes in and again out
+//   warp 1        tcgen05.mma kind::f16, one accumulator in TMEM for each group.
+//                 One thread issues them, eight a block, and at few batch rows
+//                 that is what counts: a block's operands (expanded codes and
+//                 hidden states) share one full and one free barrier, so that
+//                 it waits and commits once for both
+//   the last      (4 or 8) read a group's accumulator back, times the row's
+//                 scale (a thread a row), into f32 sums in registers; at the
+//                 tile's end logits are stored along the vocabulary, or the
+//                 rows' running maxima kept
 // Multiplying the scale in behind the MMA keeps the operands exact (code - 8
 // has four bits) for scales of any size, at N / group FMAs a weight.
 //
@@ -43,21 +47,21 @@ namespace {
 
 constexpr int kBM = 128;        // vocabulary rows of a tile
 constexpr int kQTile = kBM * 128;  // bytes of a copy of codes: 256 codes of each row
-constexpr int kASlots = 4;      // expanded stages in TMEM, 32 columns each
-constexpr int kACols = 32;
-constexpr int kDCols = 512 - kASlots * kACols;  // columns for the accumulators
+constexpr int kSlotCols = 64;   // TMEM columns of a block's expanded codes
+constexpr int kSMax = 6;        // blocks in flight, at most
 constexpr int kDMax = 4;        // accumulator buffers, at most
 constexpr int kSBox = kBM * 16;  // bytes of a box of scales: 8 groups of each row
 constexpr int kSSlots = 8;
-constexpr int kQMax = 8, kXMax = 16;
+constexpr int kQMax = 8;
 
 struct Q4Args {
   int B, H, V;
   int gshift;              // log2(group)
   int ntiles, kstages;     // kstages = H / 64
-  int unit;                // stages between two hand-overs of accumulators (1 or 2)
+  int split;               // accumulators are handed over 1 or 2 times a block
   int dbufs, dcols;        // accumulator buffers and their columns
-  int qslots, xslots;
+  int slots;               // blocks in flight
+  int qslots;
   const uint16_t* scale;
   int64_t lds;
   int gran;                // bytes of a copy of scales: 16, 8, 4, or 2 (loads)
@@ -94,6 +98,16 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
 // Eight codes of a word as bf16 code - 8, in element order.
 __device__ __forceinline__ void expand(uint32_t w, uint32_t* out) {
   const __nv_bfloat162 c136 = __halves2bfloat162(__ushort_as_bfloat16(0x4308), __ushort_as_bfloat16(0x4308));
@@ -109,13 +123,35 @@ __device__ __forceinline__ void expand(uint32_t w, uint32_t* out) {
 
 struct Q4Bars {
   uint64_t qfull[kQMax], qempty[kQMax];
-  uint64_t xfull[kXMax], xempty[kXMax];
-  uint64_t afull[kASlots], aempty[kASlots];
+  uint64_t full[kSMax], free[kSMax];
   uint64_t dfull[kDMax], dempty[kDMax];
   uint64_t sfull[kSSlots], sempty[kSSlots];
   uint64_t done;
   uint32_t tmem;
 };
+
+// mbar_wait, but without its clock where the phase is over already.
+__device__ __forceinline__ bool q4_wait(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return done || mbar_wait(bar, parity, kWaitBudget);
+}
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
 
 // A ring position: slot and the parity of its present use.
 struct Ring {
@@ -129,24 +165,23 @@ struct Ring {
   }
 };
 
-template <int N, int NEP>  // MMA N; epilogue warps
-__global__ void __launch_bounds__((12 + NEP) * 32, 1)
+template <int N, int NDQ, int NEP>  // MMA N; expanding warps (8 or 16); epilogue warps (4 or 8)
+__global__ void __launch_bounds__((4 + NDQ + NEP) * 32, 1)
     q4_mma_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmX,
                   const __grid_constant__ Q4Args a) {
   extern __shared__ uint8_t q4_smem_raw[];
   __shared__ Q4Bars bars;
   __shared__ unsigned long long best[N];
   constexpr int NC = N / (NEP / 4);  // columns of an epilogue warp
-  constexpr uint32_t kXBytes = N * 128;
+  constexpr uint32_t kXBytes = N * 128;  // 64 hidden elements of N rows
   uint8_t* qring = q4_smem_raw + ((1024u - (smem_u32(q4_smem_raw) & 1023u)) & 1023u);
   uint8_t* xring = qring + a.qslots * kQTile;
-  uint8_t* sring = xring + a.xslots * kXBytes;
+  uint8_t* sring = xring + a.slots * 2 * kXBytes;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < a.qslots; ++i) mbar_init(&bars.qfull[i], 1), mbar_init(&bars.qempty[i], 8);
-    for (int i = 0; i < a.xslots; ++i) mbar_init(&bars.xfull[i], 1), mbar_init(&bars.xempty[i], 1);
-    for (int i = 0; i < kASlots; ++i) mbar_init(&bars.afull[i], 4), mbar_init(&bars.aempty[i], 1);
+    for (int i = 0; i < a.qslots; ++i) mbar_init(&bars.qfull[i], 1), mbar_init(&bars.qempty[i], NDQ);
+    for (int i = 0; i < a.slots; ++i) mbar_init(&bars.full[i], NDQ + 1), mbar_init(&bars.free[i], 1);
     for (int i = 0; i < a.dbufs; ++i) mbar_init(&bars.dfull[i], 1), mbar_init(&bars.dempty[i], NEP);
     for (int i = 0; i < kSSlots; ++i) mbar_init(&bars.sfull[i], 32), mbar_init(&bars.sempty[i], NEP);
     mbar_init(&bars.done, 1);
@@ -161,9 +196,10 @@ __global__ void __launch_bounds__((12 + NEP) * 32, 1)
   }
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = bars.tmem;
-  const uint32_t tmem_a = tmem + kDCols;  // the expanded stages lie behind the accumulators
+  const uint32_t tmem = __shfl_sync(0xffffffffu, bars.tmem, 0);
+  const uint32_t tmem_a = tmem + static_cast<uint32_t>(a.dbufs * a.dcols);  // expanded codes lie behind the accumulators
   const int qtiles = (a.kstages + 3) >> 2;  // copies of codes a tile
+  const int blocks = (a.kstages + 1) >> 1;  // the last may be half a block
   const int ngroups = a.H >> a.gshift;
   bool ok = true;
 
@@ -176,7 +212,7 @@ __global__ void __launch_bounds__((12 + NEP) * 32, 1)
       uint32_t it = 0;
       for (int tile = blockIdx.x; tile < a.ntiles && ok; tile += gridDim.x) {
         for (int t = 0; t < qtiles; ++t, ++it) {
-          if (!mbar_wait(&bars.qempty[r.slot], r.par ^ 1u, kWaitBudget)) {
+          if (!q4_wait(&bars.qempty[r.slot], r.par ^ 1u)) {
             ok = false;
             break;
           }
@@ -188,7 +224,7 @@ __global__ void __launch_bounds__((12 + NEP) * 32, 1)
       // every issued copy lands before the CTA may return
       for (int i = 0; i < a.qslots; ++i) {
         const uint32_t n = it / a.qslots + (static_cast<uint32_t>(i) < it % a.qslots ? 1u : 0u);
-        if (n > 0 && !mbar_wait(&bars.qfull[i], (n - 1u) & 1u, kWaitBudget)) ok = false;
+        if (n > 0 && !q4_wait(&bars.qfull[i], (n - 1u) & 1u)) ok = false;
       }
     }
   } else if (warp == 2) {
@@ -199,19 +235,22 @@ __global__ void __launch_bounds__((12 + NEP) * 32, 1)
       Ring r;
       uint32_t it = 0;
       for (int tile = blockIdx.x; tile < a.ntiles && ok; tile += gridDim.x) {
-        for (int kb = 0; kb < a.kstages; ++kb, ++it) {
-          if (!mbar_wait(&bars.xempty[r.slot], r.par ^ 1u, kWaitBudget)) {
+        for (int kb = 0; kb < blocks; ++kb, ++it) {
+          if (!q4_wait(&bars.free[r.slot], r.par ^ 1u)) {
             ok = false;
             break;
           }
-          mbar_expect_tx(&bars.xfull[r.slot], kXBytes);
-          tma_load_2d(xring + r.slot * kXBytes, &tmX, kb * 64, 0, &bars.xfull[r.slot], pol);
-          r.next(a.xslots);
+          const bool two = 2 * kb + 1 < a.kstages;
+          uint8_t* x = xring + r.slot * 2 * kXBytes;
+          mbar_expect_tx(&bars.full[r.slot], two ? 2 * kXBytes : kXBytes);
+          tma_load_2d(x, &tmX, kb * 128, 0, &bars.full[r.slot], pol);
+          if (two) tma_load_2d(x + kXBytes, &tmX, kb * 128 + 64, 0, &bars.full[r.slot], pol);
+          r.next(a.slots);
         }
       }
-      for (int i = 0; i < a.xslots; ++i) {
-        const uint32_t n = it / a.xslots + (static_cast<uint32_t>(i) < it % a.xslots ? 1u : 0u);
-        if (n > 0 && !mbar_wait(&bars.xfull[i], (n - 1u) & 1u, kWaitBudget)) ok = false;
+      for (int i = 0; i < a.slots; ++i) {
+        const uint32_t n = it / a.slots + (static_cast<uint32_t>(i) < it % a.slots ? 1u : 0u);
+        if (n > 0 && !q4_wait(&bars.full[i], (n - 1u) & 1u)) ok = false;
       }
     }
   } else if (warp == 3) {
@@ -219,7 +258,7 @@ __global__ void __launch_bounds__((12 + NEP) * 32, 1)
     Ring r;
     for (int tile = blockIdx.x; tile < a.ntiles && ok; tile += gridDim.x) {
       for (int g0 = 0; g0 < ngroups && ok; g0 += 8) {
-        if (!mbar_wait(&bars.sempty[r.slot], r.par ^ 1u, kWaitBudget)) {
+        if (!q4_wait(&bars.sempty[r.slot], r.par ^ 1u)) {
           ok = false;
           break;
         }
@@ -255,93 +294,105 @@ __global__ void __launch_bounds__((12 + NEP) * 32, 1)
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp == 1) {
-    if (lane == 0) {
-      // ---- MMA issuer ----
-      const uint32_t idesc = lm_idesc(N);
-      const int gsteps = 1 << (a.gshift - 4);  // K = 16 steps of a group
-      Ring ra, rx, rd;
-      for (int tile = blockIdx.x; tile < a.ntiles && ok; tile += gridDim.x) {
-        for (int kb = 0; kb < a.kstages && ok; ++kb) {
-          const int in_unit = kb % a.unit;
-          if (in_unit == 0 && !mbar_wait(&bars.dempty[rd.slot], rd.par ^ 1u, kWaitBudget)) {
-            ok = false;
-            break;
-          }
-          if (!mbar_wait(&bars.xfull[rx.slot], rx.par, kWaitBudget) || !mbar_wait(&bars.afull[ra.slot], ra.par, kWaitBudget)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint64_t bd = sw128_desc(smem_u32(xring + rx.slot * kXBytes));
-          const uint32_t at = tmem_a + static_cast<uint32_t>(ra.slot * kACols);
-          const uint32_t d0 = tmem + static_cast<uint32_t>(rd.slot * a.dcols);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int step = 4 * in_unit + k;  // of the unit
-            umma_ta(d0 + static_cast<uint32_t>((step / gsteps) * N), at + 8u * k, bd + 2u * k, idesc, step % gsteps != 0);
-          }
-          umma_commit(&bars.aempty[ra.slot]);
-          umma_commit(&bars.xempty[rx.slot]);
-          ra.next(kASlots);
-          rx.next(a.xslots);
-          if (in_unit == a.unit - 1 || kb == a.kstages - 1) {
-            umma_commit(&bars.dfull[rd.slot]);
-            rd.next(a.dbufs);
-          }
-        }
-      }
-      // every MMA of this CTA completes before its TMEM is freed
-      umma_commit(&bars.done);
-      if (!mbar_wait(&bars.done, 0u, kWaitBudget)) ok = false;
-    }
-  } else if (warp < 12) {
-    // ---- codes into bf16: every other stage of this warp's 32 rows ----
-    const int quad = warp & 3, mine = (warp - 4) >> 2;
-    const int row = quad * 32 + lane;
-    Ring rq, ra;
-    uint32_t g = 0;  // stages so far
+    // ---- MMA issuer: the warp goes through the blocks together, so that
+    // addresses and descriptors stay uniform; one lane issues ----
+    const uint32_t idesc = lm_idesc(N);
+    const int gsteps = 1 << (a.gshift - 4);  // K = 16 steps of a group
+    const uint32_t x0 = smem_u32(xring);
+    Ring r, rd;
     for (int tile = blockIdx.x; tile < a.ntiles && ok; tile += gridDim.x) {
-      for (int t = 0; t < qtiles && ok; ++t) {
-        if (!mbar_wait(&bars.qfull[rq.slot], rq.par, kWaitBudget)) {
+      for (int kb = 0; kb < blocks && ok; ++kb) {
+        const int nst = min(2, a.kstages - 2 * kb);
+        if (!q4_wait(&bars.full[r.slot], r.par) || !q4_wait(&bars.dempty[rd.slot], rd.par ^ 1u)) {
           ok = false;
           break;
         }
-        const uint8_t* src = qring + rq.slot * kQTile + row * 128;
-        const int ns = min(4, a.kstages - 4 * t);
-        for (int s = 0; s < ns; ++s, ++g) {
-          if (static_cast<int>(g & 1u) == mine) {
-            const uint4 c0 = *reinterpret_cast<const uint4*>(src + (((2 * s) ^ (row & 7)) << 4));
-            const uint4 c1 = *reinterpret_cast<const uint4*>(src + (((2 * s + 1) ^ (row & 7)) << 4));
-            uint32_t e[32];
-            expand(c0.x, e);
-            expand(c0.y, e + 4);
-            expand(c0.z, e + 8);
-            expand(c0.w, e + 12);
-            expand(c1.x, e + 16);
-            expand(c1.y, e + 20);
-            expand(c1.z, e + 24);
-            expand(c1.w, e + 28);
-            if (!mbar_wait(&bars.aempty[ra.slot], ra.par ^ 1u, kWaitBudget)) {
+        tc_fence_after();
+        const uint64_t bd = sw128_desc(x0 + r.slot * 2 * kXBytes);
+        const uint32_t at = tmem_a + static_cast<uint32_t>(r.slot * kSlotCols);
+        int step = 0;  // since the last hand-over of accumulators
+        for (int st = 0; st < nst; ++st) {
+          const uint32_t d0 = tmem + static_cast<uint32_t>(rd.slot * a.dcols);
+          if (elect_one()) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              umma_ta(d0 + static_cast<uint32_t>(((step + k) / gsteps) * N), at + 32u * st + 8u * k,
+                      bd + static_cast<uint64_t>((kXBytes >> 4) * st) + 2u * k, idesc, (step + k) % gsteps != 0);
+            if (st == nst - 1) umma_commit(&bars.free[r.slot]);
+            if (st == nst - 1 || a.split == 2) umma_commit(&bars.dfull[rd.slot]);
+          }
+          __syncwarp();
+          step += 4;
+          if (st == nst - 1 || a.split == 2) {
+            step = 0;
+            rd.next(a.dbufs);
+            if (st < nst - 1 && !q4_wait(&bars.dempty[rd.slot], rd.par ^ 1u)) {
               ok = false;
               break;
             }
             tc_fence_after();
-            tmem_st32(tmem_a + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(ra.slot * kACols), e);
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive1(&bars.afull[ra.slot]);
           }
-          ra.next(kASlots);
         }
+        r.next(a.slots);
+      }
+    }
+    // every MMA of this CTA completes before its TMEM is freed
+    if (elect_one()) umma_commit(&bars.done);
+    __syncwarp();
+    if (!q4_wait(&bars.done, 0u)) ok = false;
+  } else if (warp < 4 + NDQ) {
+    // ---- codes into bf16: this warp's share of a block, for 32 rows ----
+    constexpr int kShare = 128 / (NDQ / 4);  // codes: 64 or 32
+    const int quad = warp & 3, mine = (warp - 4) >> 2;
+    const int row = quad * 32 + lane;
+    const int stage = mine * kShare / 64;  // of the block
+    Ring rq, r;
+    for (int tile = blockIdx.x; tile < a.ntiles && ok; tile += gridDim.x) {
+      for (int kb = 0; kb < blocks && ok; ++kb) {
+        if ((kb & 1) == 0 && !q4_wait(&bars.qfull[rq.slot], rq.par)) {
+          ok = false;
+          break;
+        }
+        const bool have = 2 * kb + stage < a.kstages;
+        uint32_t e[kShare / 2];
+        if (have) {
+          const uint8_t* src = qring + rq.slot * kQTile + row * 128;
+          const int c0 = (kb & 1) * 4 + mine * (kShare / 32);  // 16-byte piece of the row's 128
+#pragma unroll
+          for (int i = 0; i < kShare / 32; ++i) {
+            const uint4 c = *reinterpret_cast<const uint4*>(src + (((c0 + i) ^ (row & 7)) << 4));
+            expand(c.x, e + 16 * i);
+            expand(c.y, e + 16 * i + 4);
+            expand(c.z, e + 16 * i + 8);
+            expand(c.w, e + 16 * i + 12);
+          }
+        }
+        if ((kb & 1) == 1 || kb == blocks - 1) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive1(&bars.qempty[rq.slot]);
+          rq.next(a.qslots);
+        }
+        if (!q4_wait(&bars.free[r.slot], r.par ^ 1u)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        if (have) {
+          const uint32_t to = tmem_a + (static_cast<uint32_t>(quad * 32) << 16) +
+                              static_cast<uint32_t>(r.slot * kSlotCols + mine * (kShare / 2));
+          if constexpr (kShare == 64) tmem_st32(to, e);
+          else tmem_st16(to, e);
+        }
+        tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive1(&bars.qempty[rq.slot]);
-        rq.next(a.qslots);
+        if (lane == 0) mbar_arrive1(&bars.full[r.slot]);
+        r.next(a.slots);
       }
     }
   } else {
     // ---- epilogue ----
     const int quad = warp & 3;
-    const int col0 = ((warp - 12) >> 2) * NC;
+    const int col0 = ((warp - 4 - NDQ) >> 2) * NC;
     const int row = quad * 32 + lane;
     Ring rd, rs;
     for (int tile = blockIdx.x; tile < a.ntiles && ok; tile += gridDim.x) {
@@ -350,16 +401,17 @@ __global__ void __launch_bounds__((12 + NEP) * 32, 1)
       for (int j = 0; j < NC; ++j) acc[j] = 0.0f;
       uint4 sc = {0u, 0u, 0u, 0u};  // the scales of 8 groups
       int g = 0;
-      for (int kb = 0; kb < a.kstages && ok; kb += a.unit) {
-        const int n_in = (min(a.unit, a.kstages - kb) * 64) >> a.gshift;
-        if (!mbar_wait(&bars.dfull[rd.slot], rd.par, kWaitBudget)) {
+      const int unit = 2 / a.split;  // stages of a hand-over
+      for (int kb = 0; kb < a.kstages && ok; kb += unit) {
+        const int n_in = (min(unit, a.kstages - kb) * 64) >> a.gshift;
+        if (!q4_wait(&bars.dfull[rd.slot], rd.par)) {
           ok = false;
           break;
         }
         tc_fence_after();
         for (int i = 0; i < n_in; ++i, ++g) {
           if ((g & 7) == 0) {
-            if (!mbar_wait(&bars.sfull[rs.slot], rs.par, kWaitBudget)) {
+            if (!q4_wait(&bars.sfull[rs.slot], rs.par)) {
               ok = false;
               break;
             }
@@ -507,26 +559,28 @@ rl_status q4_check(rl_sampler* h, const uint16_t* hidden, int64_t ldh, const rl_
 }
 
 // A launch for at most N batch rows.
-template <int N, int NEP>
+template <int N, int NDQ, int NEP>
 cudaError_t q4_run(const CUtensorMap& mq, const CUtensorMap& mx, Q4Args a, int grid, cudaStream_t stream) {
-  const int xbytes = N * 128;
-  a.qslots = kQMax;
-  a.xslots = 64 * 1024 / xbytes < kXMax ? 64 * 1024 / xbytes : kXMax;
-  const int group = 1 << a.gshift;
-  a.unit = group == 128 || 2 * (128 / group) * N <= kDCols ? 2 : 1;
-  a.dcols = N * (64 * a.unit / group);
-  a.dbufs = kDCols / a.dcols < kDMax ? kDCols / a.dcols : kDMax;
-  const size_t smem = 1024 + static_cast<size_t>(a.qslots) * kQTile + static_cast<size_t>(a.xslots) * xbytes + kSSlots * kSBox;
+  const int xbytes = 2 * N * 128, group = 1 << a.gshift;
+  // accumulators take at most half of TMEM, in two buffers or more; the rest
+  // and 64 KB of hidden states (128 KB at the largest N) hold blocks in flight
+  a.split = group == 128 || N * (128 / group) <= 128 ? 1 : 2;
+  a.dcols = N * (128 / group) / a.split;
+  a.dbufs = 256 / a.dcols < kDMax ? 256 / a.dcols : kDMax;
+  a.slots = (512 - a.dbufs * a.dcols) / kSlotCols < kSMax ? (512 - a.dbufs * a.dcols) / kSlotCols : kSMax;
+  const int room = 224 * 1024 - 1024 - kSSlots * kSBox - a.slots * xbytes;
+  a.qslots = room / kQTile < kQMax ? room / kQTile : kQMax;
+  const size_t smem = 1024 + static_cast<size_t>(a.qslots) * kQTile + static_cast<size_t>(a.slots) * xbytes + kSSlots * kSBox;
   static std::atomic<int> configured[64];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev < 0 || dev >= 64 || !configured[dev].load(std::memory_order_acquire)) {
-    e = cudaFuncSetAttribute(q4_mma_kernel<N, NEP>, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024);
+    e = cudaFuncSetAttribute(q4_mma_kernel<N, NDQ, NEP>, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024);
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) configured[dev].store(1, std::memory_order_release);
   }
-  q4_mma_kernel<N, NEP><<<grid, (12 + NEP) * 32, smem, stream>>>(mq, mx, a);
+  q4_mma_kernel<N, NDQ, NEP><<<grid, (4 + NDQ + NEP) * 32, smem, stream>>>(mq, mx, a);
   return cudaGetLastError();
 }
 
@@ -567,11 +621,11 @@ rl_status q4_launch(rl_sampler* h, const uint16_t* hidden, int64_t ldh, const rl
     CUtensorMap mx;
     if (!lm_tensor_map(&mx, hidden + static_cast<int64_t>(b0) * ldh, 2, H, Bc, ldh * 2, N))
       return set_error(RL_ERR_INVALID_ARG, "rl_lmhead_q4: hidden tensor map rejected (alignment or stride)");
-    cudaError_t e = N == 16   ? q4_run<16, 4>(mq, mx, a, grid, stream)
-                    : N == 32 ? q4_run<32, 4>(mq, mx, a, grid, stream)
-                    : N == 64 ? q4_run<64, 8>(mq, mx, a, grid, stream)
-                    : N == 96 ? q4_run<96, 8>(mq, mx, a, grid, stream)
-                              : q4_run<128, 8>(mq, mx, a, grid, stream);
+    cudaError_t e = N == 16   ? q4_run<16, 16, 4>(mq, mx, a, grid, stream)
+                    : N == 32 ? q4_run<32, 16, 4>(mq, mx, a, grid, stream)
+                    : N == 64 ? q4_run<64, 16, 8>(mq, mx, a, grid, stream)
+                    : N == 96 ? q4_run<96, 8, 8>(mq, mx, a, grid, stream)
+                              : q4_run<128, 8, 8>(mq, mx, a, grid, stream);
     if (e == cudaSuccess && out_tok)
       e = lm_argmax(h->lm_part, Bc, grid, h->lm_err, out_tok + b0, row_status ? row_status + b0 : nullptr, stream);
     if (e != cudaSuccess) return set_error(RL_ERR_CUDA, cudaGetErrorString(e));
