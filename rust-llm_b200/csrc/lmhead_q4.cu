@@ -297,8 +297,15 @@ __global__ void __launch_bounds__((4 + NDQ + NEP) * 32, 1)
     // ---- MMA issuer: the warp goes through the blocks together, so that
     // addresses and descriptors stay uniform; one lane issues ----
     const uint32_t idesc = lm_idesc(N);
-    const int gsteps = 1 << (a.gshift - 4);  // K = 16 steps of a group
+    const int gs = a.gshift - 4;  // log2 of a group's steps (K = 16)
     const uint32_t x0 = smem_u32(xring);
+    // four MMAs of a stage, `step` steps behind the hand-over's first
+    const auto issue = [&](uint32_t d0, uint32_t at, uint64_t bd, int step) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        umma_ta(d0 + static_cast<uint32_t>(((step + k) >> gs) * N), at + 8u * k, bd + 2u * k, idesc,
+                ((step + k) & ((1 << gs) - 1)) != 0);
+    };
     Ring r, rd;
     for (int tile = blockIdx.x; tile < a.ntiles && ok; tile += gridDim.x) {
       for (int kb = 0; kb < blocks && ok; ++kb) {
@@ -310,29 +317,37 @@ __global__ void __launch_bounds__((4 + NDQ + NEP) * 32, 1)
         tc_fence_after();
         const uint64_t bd = sw128_desc(x0 + r.slot * 2 * kXBytes);
         const uint32_t at = tmem_a + static_cast<uint32_t>(r.slot * kSlotCols);
-        int step = 0;  // since the last hand-over of accumulators
-        for (int st = 0; st < nst; ++st) {
-          const uint32_t d0 = tmem + static_cast<uint32_t>(rd.slot * a.dcols);
+        const uint32_t d0 = tmem + static_cast<uint32_t>(rd.slot * a.dcols);
+        if (a.split == 1) {
           if (elect_one()) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              umma_ta(d0 + static_cast<uint32_t>(((step + k) / gsteps) * N), at + 32u * st + 8u * k,
-                      bd + static_cast<uint64_t>((kXBytes >> 4) * st) + 2u * k, idesc, (step + k) % gsteps != 0);
-            if (st == nst - 1) umma_commit(&bars.free[r.slot]);
-            if (st == nst - 1 || a.split == 2) umma_commit(&bars.dfull[rd.slot]);
+            issue(d0, at, bd, 0);
+            if (nst == 2) issue(d0, at + 32u, bd + (kXBytes >> 4), 4);
+            umma_commit(&bars.free[r.slot]);
+            umma_commit(&bars.dfull[rd.slot]);
           }
-          __syncwarp();
-          step += 4;
-          if (st == nst - 1 || a.split == 2) {
-            step = 0;
-            rd.next(a.dbufs);
-            if (st < nst - 1 && !q4_wait(&bars.dempty[rd.slot], rd.par ^ 1u)) {
+          rd.next(a.dbufs);
+        } else {
+          if (elect_one()) {
+            issue(d0, at, bd, 0);
+            umma_commit(&bars.dfull[rd.slot]);
+            if (nst == 1) umma_commit(&bars.free[r.slot]);
+          }
+          rd.next(a.dbufs);
+          if (nst == 2) {
+            if (!q4_wait(&bars.dempty[rd.slot], rd.par ^ 1u)) {
               ok = false;
               break;
             }
             tc_fence_after();
+            if (elect_one()) {
+              issue(tmem + static_cast<uint32_t>(rd.slot * a.dcols), at + 32u, bd + (kXBytes >> 4), 0);
+              umma_commit(&bars.dfull[rd.slot]);
+              umma_commit(&bars.free[r.slot]);
+            }
+            rd.next(a.dbufs);
           }
         }
+        __syncwarp();
         r.next(a.slots);
       }
     }
