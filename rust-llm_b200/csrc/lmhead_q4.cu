@@ -12,7 +12,7 @@
 //                 bytes of a row, 128-byte swizzle
 //   warp 2        TMA producer of the hidden states: two [N x 64] a block
 //   warp 3        copies the scales: [128 rows x 8 groups] a box
-//   warps 4-...   (8 or 16) turn codes into bf16 (a thread a row: code | 0x4300
+//   warps 4-...   turn codes into bf16 (a thread a row, a block at a turn: code | 0x4300
 //                 is 128 + code, less 136) and store them into TMEM, from where
 //                 the MMA reads them as its A operand: expanded weights never
 //                 pass through shared memory, which would take four times the
@@ -95,17 +95,6 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
       "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
       "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
-  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-}
-
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
-  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
 // Eight codes of a word as bf16 code - 8, in element order.
@@ -165,7 +154,7 @@ struct Ring {
   }
 };
 
-template <int N, int NDQ, int NEP>  // MMA N; expanding warps (8 or 16); epilogue warps (4 or 8)
+template <int N, int NDQ, int NEP>  // MMA N; expanding warps (a multiple of 4); epilogue warps (4 or 8)
 __global__ void __launch_bounds__((4 + NDQ + NEP) * 32, 1)
     q4_mma_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmX,
                   const __grid_constant__ Q4Args a) {
@@ -181,7 +170,7 @@ __global__ void __launch_bounds__((4 + NDQ + NEP) * 32, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < a.qslots; ++i) mbar_init(&bars.qfull[i], 1), mbar_init(&bars.qempty[i], NDQ);
-    for (int i = 0; i < a.slots; ++i) mbar_init(&bars.full[i], NDQ + 1), mbar_init(&bars.free[i], 1);
+    for (int i = 0; i < a.slots; ++i) mbar_init(&bars.full[i], 4 + 1), mbar_init(&bars.free[i], 1);
     for (int i = 0; i < a.dbufs; ++i) mbar_init(&bars.dfull[i], 1), mbar_init(&bars.dempty[i], NEP);
     for (int i = 0; i < kSSlots; ++i) mbar_init(&bars.sfull[i], 32), mbar_init(&bars.sempty[i], NEP);
     mbar_init(&bars.done, 1);
@@ -356,51 +345,53 @@ __global__ void __launch_bounds__((4 + NDQ + NEP) * 32, 1)
     __syncwarp();
     if (!q4_wait(&bars.done, 0u)) ok = false;
   } else if (warp < 4 + NDQ) {
-    // ---- codes into bf16: this warp's share of a block, for 32 rows ----
-    constexpr int kShare = 128 / (NDQ / 4);  // codes: 64 or 32
-    const int quad = warp & 3, mine = (warp - 4) >> 2;
+    // ---- codes into bf16: every so many blocks of this warp's 32 rows ----
+    constexpr int kTurns = NDQ / 4;
+    const int quad = warp & 3;
     const int row = quad * 32 + lane;
-    const int stage = mine * kShare / 64;  // of the block
+    int turn = (warp - 4) >> 2;  // blocks until this warp's next
     Ring rq, r;
     for (int tile = blockIdx.x; tile < a.ntiles && ok; tile += gridDim.x) {
       for (int kb = 0; kb < blocks && ok; ++kb) {
-        if ((kb & 1) == 0 && !q4_wait(&bars.qfull[rq.slot], rq.par)) {
+        const bool mine = turn == 0;
+        turn = mine ? kTurns - 1 : turn - 1;
+        const bool last = (kb & 1) == 1 || kb == blocks - 1;  // of a copy of codes
+        if ((mine || last) && !q4_wait(&bars.qfull[rq.slot], rq.par)) {
           ok = false;
           break;
         }
-        const bool have = 2 * kb + stage < a.kstages;
-        uint32_t e[kShare / 2];
-        if (have) {
-          const uint8_t* src = qring + rq.slot * kQTile + row * 128;
-          const int c0 = (kb & 1) * 4 + mine * (kShare / 32);  // 16-byte piece of the row's 128
-#pragma unroll
-          for (int i = 0; i < kShare / 32; ++i) {
-            const uint4 c = *reinterpret_cast<const uint4*>(src + (((c0 + i) ^ (row & 7)) << 4));
-            expand(c.x, e + 16 * i);
-            expand(c.y, e + 16 * i + 4);
-            expand(c.z, e + 16 * i + 8);
-            expand(c.w, e + 16 * i + 12);
+        if (mine) {
+          if (!q4_wait(&bars.free[r.slot], r.par ^ 1u)) {
+            ok = false;
+            break;
           }
+          tc_fence_after();
+          const uint8_t* src = qring + rq.slot * kQTile + row * 128;
+          const uint32_t to = tmem_a + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(r.slot * kSlotCols);
+          const int nst = min(2, a.kstages - 2 * kb);
+          for (int st = 0; st < nst; ++st) {
+            const int c0 = (kb & 1) * 4 + st * 2;  // 16-byte piece of the row's 128
+            uint32_t e[32];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const uint4 c = *reinterpret_cast<const uint4*>(src + (((c0 + i) ^ (row & 7)) << 4));
+              expand(c.x, e + 16 * i);
+              expand(c.y, e + 16 * i + 4);
+              expand(c.z, e + 16 * i + 8);
+              expand(c.w, e + 16 * i + 12);
+            }
+            tmem_st32(to + 32u * st, e);
+          }
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive1(&bars.full[r.slot]);
         }
-        if ((kb & 1) == 1 || kb == blocks - 1) {
+        if (last) {
           __syncwarp();
           if (lane == 0) mbar_arrive1(&bars.qempty[rq.slot]);
           rq.next(a.qslots);
         }
-        if (!q4_wait(&bars.free[r.slot], r.par ^ 1u)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        if (have) {
-          const uint32_t to = tmem_a + (static_cast<uint32_t>(quad * 32) << 16) +
-                              static_cast<uint32_t>(r.slot * kSlotCols + mine * (kShare / 2));
-          if constexpr (kShare == 64) tmem_st32(to, e);
-          else tmem_st16(to, e);
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive1(&bars.full[r.slot]);
         r.next(a.slots);
       }
     }
@@ -636,9 +627,9 @@ rl_status q4_launch(rl_sampler* h, const uint16_t* hidden, int64_t ldh, const rl
     CUtensorMap mx;
     if (!lm_tensor_map(&mx, hidden + static_cast<int64_t>(b0) * ldh, 2, H, Bc, ldh * 2, N))
       return set_error(RL_ERR_INVALID_ARG, "rl_lmhead_q4: hidden tensor map rejected (alignment or stride)");
-    cudaError_t e = N == 16   ? q4_run<16, 16, 4>(mq, mx, a, grid, stream)
-                    : N == 32 ? q4_run<32, 16, 4>(mq, mx, a, grid, stream)
-                    : N == 64 ? q4_run<64, 16, 8>(mq, mx, a, grid, stream)
+    cudaError_t e = N == 16   ? q4_run<16, 8, 4>(mq, mx, a, grid, stream)
+                    : N == 32 ? q4_run<32, 8, 4>(mq, mx, a, grid, stream)
+                    : N == 64 ? q4_run<64, 8, 8>(mq, mx, a, grid, stream)
                     : N == 96 ? q4_run<96, 8, 8>(mq, mx, a, grid, stream)
                               : q4_run<128, 8, 8>(mq, mx, a, grid, stream);
     if (e == cudaSuccess && out_tok)
