@@ -29,10 +29,17 @@
 // Multiplying the scale in behind the MMA keeps the operands exact (code - 8
 // has four bits) for scales of any size, at N / group FMAs a weight.
 //
+// Up to 16 batch rows (q4_few_kernel) the hand-overs between those roles cost
+// more than the work: there each warp multiplies what it loads, on its own. It
+// streams the codes of 16 vocabulary rows through a ring of its own and takes
+// them, as f16, straight into mma.sync fragments; the hidden states lie in
+// shared memory in the order of the fragments.
+//
 // Bound: HBM, half a byte a weight, up to about 100 batch rows; beside it the
-// expansion, 11 instructions for 8 weights. Every wait is bounded; where one
-// runs out the error flag is set, copies in flight land and TMEM is freed.
+// expansion, 9 to 13 instructions for 8 weights. Every wait is bounded; where
+// one runs out the error flag is set, copies in flight land and TMEM is freed.
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <atomic>
@@ -482,6 +489,276 @@ __global__ void __launch_bounds__((4 + NDQ + NEP) * 32, 1)
 }
 
 // ---------------------------------------------------------------------------
+// Few batch rows
+// ---------------------------------------------------------------------------
+constexpr int kFewRows = 16;   // vocabulary rows of a tile (MMA M)
+constexpr int kFewWarps = 16;
+constexpr int kFewSlots = 6;   // copies in flight a warp, at most
+constexpr int kFewBox = kFewRows * 128;  // bytes of a copy: 256 codes (two sets) of each row
+constexpr int kFewHidden = 128 * 1024;   // bytes of the hidden states in shared memory, at most
+
+struct FewArgs {
+  const uint16_t* hidden;
+  int64_t ldh;
+  int B, H, V;
+  int gshift;
+  int ntiles, nsets;  // 16-row tiles; sets of K = 128
+  int slots;
+  const uint16_t* scale;
+  int64_t lds;
+  float* out_f32;
+  uint16_t* out_bf16;
+  int64_t ldo;
+  uint64_t* part;
+  int* err;
+};
+
+__device__ __forceinline__ uint32_t h2_bits(__half2 v) { return *reinterpret_cast<uint32_t*>(&v); }
+__device__ __forceinline__ __half2 bits_h2(uint32_t v) { return *reinterpret_cast<__half2*>(&v); }
+
+// Two pairs of codes (elements 0, 1 and 2, 3 of a word's lower byte lanes) as
+// f16 code - 8: 0x6400 | code is 1024 + code, with the code four bits up
+// 1024 + 16 code.
+__device__ __forceinline__ void expand_h(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  lo = h2_bits(__hsub2(bits_h2((w & 0x000f000fu) | 0x64006400u), bits_h2(0x64086408u)));
+  hi = h2_bits(__hfma2(bits_h2((w & 0x00f000f0u) | 0x64006400u), bits_h2(0x2c002c00u), bits_h2(0xd480d480u)));
+}
+
+// D += A B: 16 x 8 f32, A 16 x 16 and B 16 x 8 f16.
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// 2^e, e in [-126, 127].
+__device__ __forceinline__ float pow2f(int e) { return __int_as_float((e + 127) << 23); }
+// The power of two that brings m (>= 0, finite) to [2^k, 2^(k+1)), as an exponent.
+__device__ __forceinline__ int bring_to(float m, int k) {
+  const int e = static_cast<int>(__float_as_uint(m) >> 23) - 127;  // -127 for zero and subnormals
+  return min(max(k - e, -126), 126);
+}
+__device__ __forceinline__ float finite_abs(float x) { return fabsf(x) < RL_POS_INF ? fabsf(x) : 0.0f; }
+
+// Fragments. A row's 16-byte piece holds 32 codes; in a set of K = 128, lane
+// (g, t) = (lane / 4, lane % 4) holds piece t of rows g and g + 8, and hidden
+// elements 32 t .. 32 t + 31 of batch row g. Step j of the set multiplies
+// elements 32 t + 4 j .. + 3 of the four t: K is summed in another order than it
+// lies in memory, alike for both operands.
+//
+// f16 holds code - 8 times a bf16 scale exactly (4 + 8 bits, less the sign's),
+// so where a set has more than one group (Pre) the scale is multiplied in before
+// the MMA, brought near 1 by the power of two of the row's largest scale in the
+// set; a set that is one group is scaled behind it. Either way a set's sum goes
+// into the row's in f32. Hidden states are bf16 brought near 2^10 by the power
+// of two of the batch row's largest. What a power of two drops is below 2^-24 of
+// the largest.
+template <int NT, bool Pre>  // batch tiles of 8
+__global__ void __launch_bounds__(kFewWarps * 32, 1)
+    q4_few_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ FewArgs a) {
+  extern __shared__ uint8_t few_smem_raw[];
+  __shared__ uint64_t full[kFewWarps][kFewSlots];
+  __shared__ unsigned long long best[NT * 8];
+  __shared__ int hexp[NT * 8];  // the batch rows' powers of two
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  uint8_t* base = few_smem_raw + ((1024u - (smem_u32(few_smem_raw) & 1023u)) & 1023u);
+  uint8_t* ring = base + static_cast<size_t>(warp) * a.slots * kFewBox;  // this warp's
+  uint4* hs = reinterpret_cast<uint4*>(base + static_cast<size_t>(kFewWarps) * a.slots * kFewBox);  // [set][NT][4][32]
+  if (lane == 0) {
+    for (int i = 0; i < a.slots; ++i) mbar_init(&full[warp][i], 1);
+    fence_mbar_init();
+  }
+  if (threadIdx.x < NT * 8) best[threadIdx.x] = 0ull;
+  __syncwarp();
+  // ---- this warp's stream of codes ----
+  const int stride = static_cast<int>(gridDim.x) * kFewWarps;
+  const int tile0 = blockIdx.x * kFewWarps + warp;
+  const int boxes = (a.nsets + 1) >> 1;  // copies a tile
+  const uint64_t pol = lm_policy_first();
+  int ctile = tile0, cbox = 0;  // the next copy
+  uint32_t issued = 0;
+  Ring rc;
+  const auto copy = [&] {  // one lane
+    mbar_expect_tx(&full[warp][rc.slot], kFewBox);
+    tma_load_2d(ring + rc.slot * kFewBox, &tmQ, cbox * 128, ctile * kFewRows, &full[warp][rc.slot], pol);
+    rc.next(a.slots);
+    ++issued;
+    if (++cbox == boxes) {
+      cbox = 0;
+      ctile += stride;
+    }
+  };
+  if (lane == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmQ)) : "memory");
+    for (int i = 0; i < a.slots && ctile < a.ntiles; ++i) copy();
+  }
+  // ---- the hidden states, as f16 fragments ----
+  for (int b = warp; b < NT * 8; b += kFewWarps) {
+    float m = 0.0f;
+    if (b < a.B) {
+      const uint4* x = reinterpret_cast<const uint4*>(a.hidden + static_cast<int64_t>(b) * a.ldh);
+      for (int i = lane; i < (a.H >> 3); i += 32) {
+        const uint4 v = __ldg(x + i);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) m = fmaxf(m, fmaxf(finite_abs(bf16_at(w[k], 0)), finite_abs(bf16_at(w[k], 1))));
+      }
+    }
+    m = warp_max(m);
+    if (lane == 0) hexp[b] = bring_to(m, 10);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.nsets * NT * 4 * 32; i += kFewWarps * 32) {
+    // fragment i of lane l: steps 2 jj and 2 jj + 1 of batch tile n in the set
+    const int l = i & 31, jj = (i >> 5) & 3, n = (i >> 7) % NT, set = (i >> 7) / NT;
+    const int b = n * 8 + (l >> 2), k0 = set * 128 + 32 * (l & 3) + 8 * jj;
+    uint4 v = {0u, 0u, 0u, 0u};
+    if (b < a.B && k0 < a.H) v = __ldg(reinterpret_cast<const uint4*>(a.hidden + static_cast<int64_t>(b) * a.ldh + k0));
+    const float f = pow2f(hexp[b]);
+    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = h2_bits(__floats2half2_rn(bf16_at(w[k], 0) * f, bf16_at(w[k], 1) * f));
+    hs[i] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  __syncthreads();
+
+  // ---- tiles ----
+  const int ngroups = a.H >> a.gshift;
+  bool ok = true;
+  Ring r;
+  for (int tile = tile0; tile < a.ntiles && ok; tile += stride) {
+    const int64_t v0 = static_cast<int64_t>(tile) * kFewRows + g, v1 = v0 + 8;
+    const uint16_t* sp0 = a.scale + (v0 < a.V ? v0 : 0) * a.lds;
+    const uint16_t* sp1 = a.scale + (v1 < a.V ? v1 : 0) * a.lds;
+    // this lane's group of a set, rows g and g + 8
+    const auto scales = [&](int set) {
+      const int gi = (set * 128 + 32 * t) >> a.gshift;
+      return gi < ngroups ? static_cast<uint32_t>(__ldg(sp0 + gi)) | static_cast<uint32_t>(__ldg(sp1 + gi)) << 16 : 0u;
+    };
+    float acc[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.0f;
+    uint32_t sc1 = scales(0), sc2 = scales(1);
+    for (int box = 0; box < boxes; ++box) {
+      if (!q4_wait(&full[warp][r.slot], r.par)) {
+        ok = false;
+        break;
+      }
+      const uint8_t* src = ring + r.slot * kFewBox;
+      uint4 c[2][2];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int piece = (s * 4 + t) ^ g;
+        c[s][0] = *reinterpret_cast<const uint4*>(src + g * 128 + piece * 16);
+        c[s][1] = *reinterpret_cast<const uint4*>(src + (g + 8) * 128 + piece * 16);
+      }
+      __syncwarp();
+      if (lane == 0 && ctile < a.ntiles) copy();  // the slot is read: the stream goes on in it
+      r.next(a.slots);
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int set = 2 * box + s;
+        if (set >= a.nsets) break;
+        const float x = bf16_at(sc1, 0), y = bf16_at(sc1, 1);
+        sc1 = sc2;
+        sc2 = scales(set + 2);
+        float d[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) d[n][0] = d[n][1] = d[n][2] = d[n][3] = 0.0f;
+        float up0 = x, up1 = y;
+        __half2 s0, s1;
+        if constexpr (Pre) {
+          float m0 = finite_abs(x), m1 = finite_abs(y);
+          m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, 1));
+          m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, 1));
+          m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, 2));
+          m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, 2));
+          const int e0 = bring_to(m0, 0), e1 = bring_to(m1, 0);
+          s0 = __float2half2_rn(x * pow2f(e0));
+          s1 = __float2half2_rn(y * pow2f(e1));
+          up0 = pow2f(-e0), up1 = pow2f(-e1);
+        }
+        const uint32_t w0[4] = {c[s][0].x, c[s][0].y, c[s][0].z, c[s][0].w};
+        const uint32_t w1[4] = {c[s][1].x, c[s][1].y, c[s][1].z, c[s][1].w};
+        const uint4* h = hs + set * (NT * 4 * 32) + lane;
+#pragma unroll
+        for (int jj = 0; jj < 4; ++jj) {
+          uint32_t e[2][4];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            expand_h(w0[jj] >> (8 * k), e[k][0], e[k][2]);
+            expand_h(w1[jj] >> (8 * k), e[k][1], e[k][3]);
+            if constexpr (Pre) {
+              e[k][0] = h2_bits(__hmul2(bits_h2(e[k][0]), s0));
+              e[k][2] = h2_bits(__hmul2(bits_h2(e[k][2]), s0));
+              e[k][1] = h2_bits(__hmul2(bits_h2(e[k][1]), s1));
+              e[k][3] = h2_bits(__hmul2(bits_h2(e[k][3]), s1));
+            }
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const uint4 hv = h[(n * 4 + jj) * 32];
+            mma_f16(d[n], e[0][0], e[0][1], e[0][2], e[0][3], hv.x, hv.y);
+            mma_f16(d[n], e[1][0], e[1][1], e[1][2], e[1][3], hv.z, hv.w);
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          acc[n][0] = fmaf(up0, d[n][0], acc[n][0]);
+          acc[n][1] = fmaf(up0, d[n][1], acc[n][1]);
+          acc[n][2] = fmaf(up1, d[n][2], acc[n][2]);
+          acc[n][3] = fmaf(up1, d[n][3], acc[n][3]);
+        }
+      }
+    }
+    if (!ok) break;
+    // ---- rows g, g + 8 of batch rows 2 t, 2 t + 1 ----
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int b = n * 8 + 2 * t + k;
+        const float back = pow2f(-hexp[b]);
+        const float y0 = acc[n][k] * back, y1 = acc[n][2 + k] * back;
+        if (b < a.B) {
+          const int64_t at = static_cast<int64_t>(b) * a.ldo;
+          if (a.out_f32) {
+            if (v0 < a.V) a.out_f32[at + v0] = y0;
+            if (v1 < a.V) a.out_f32[at + v1] = y1;
+          }
+          if (a.out_bf16) {
+            if (v0 < a.V) a.out_bf16[at + v0] = __bfloat16_as_ushort(__float2bfloat16_rn(y0));
+            if (v1 < a.V) a.out_bf16[at + v1] = __bfloat16_as_ushort(__float2bfloat16_rn(y1));
+          }
+        }
+        if (a.part) {
+          uint64_t key = v0 < a.V ? lm_key(y0, static_cast<int>(v0)) : 0ull;
+          if (v1 < a.V) key = umax64(key, lm_key(y1, static_cast<int>(v1)));
+#pragma unroll
+          for (int o = 16; o > 2; o >>= 1) key = umax64(key, shfl_xor64(key, o));  // over g
+          if (g == 0 && b < a.B) atomicMax(&best[b], static_cast<unsigned long long>(key));
+        }
+      }
+    }
+  }
+  if (!ok) {
+    // behind a wait that ran out: every issued copy lands before the CTA returns
+    if (lane == 0)
+      for (int i = 0; i < a.slots; ++i) {
+        const uint32_t n = issued / a.slots + (static_cast<uint32_t>(i) < issued % a.slots ? 1u : 0u);
+        if (n > 0) mbar_wait(&full[warp][i], (n - 1u) & 1u, kWaitBudget);
+      }
+    atomicExch(a.err, 1);
+  }
+  __syncthreads();
+  if (a.part && static_cast<int>(threadIdx.x) < a.B)
+    a.part[static_cast<int64_t>(threadIdx.x) * gridDim.x + blockIdx.x] = best[threadIdx.x];
+}
+
+// ---------------------------------------------------------------------------
 // Quantisation: a thread takes eight elements (a word of codes), the lanes of a
 // group find its largest magnitude. Bound by HBM (2.5 bytes an element).
 // ---------------------------------------------------------------------------
@@ -590,11 +867,76 @@ cudaError_t q4_run(const CUtensorMap& mq, const CUtensorMap& mx, Q4Args a, int g
   return cudaGetLastError();
 }
 
+template <int NT, bool Pre>
+cudaError_t few_run(const CUtensorMap& mq, const FewArgs& a, size_t smem, int grid, cudaStream_t stream) {
+  static std::atomic<int> configured[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64 || !configured[dev].load(std::memory_order_acquire)) {
+    e = cudaFuncSetAttribute(q4_few_kernel<NT, Pre>, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024);
+    if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64) configured[dev].store(1, std::memory_order_release);
+  }
+  q4_few_kernel<NT, Pre><<<grid, kFewWarps * 32, smem, stream>>>(mq, a);
+  return cudaGetLastError();
+}
+
+// Whether the hidden states fit shared memory beside the rings (H <= 8192 at
+// 8 batch rows, 4096 at 16).
+size_t few_hidden(int B, int H) { return static_cast<size_t>(B <= 8 ? 8 : 16) * ((H + 127) / 128) * 256; }
+bool is_few(int B, int H) { return B <= 16 && few_hidden(B, H) <= kFewHidden; }
+
+rl_status few_launch(rl_sampler* h, const uint16_t* hidden, int64_t ldh, const rl_q4_weight& w, int B, int H, int V,
+                     float* out_f32, uint16_t* out_bf16, int64_t ldo, uint64_t* part, int* grid_out, cudaStream_t stream) {
+  CUtensorMap mq;
+  if (!lm_tensor_map(&mq, w.q, 1, H / 2, V, w.ldq, kFewRows))
+    return set_error(RL_ERR_INVALID_ARG, "rl_lmhead_q4: tensor map of the codes rejected (alignment or stride)");
+  FewArgs a = {};
+  a.hidden = hidden;
+  a.ldh = ldh;
+  a.B = B;
+  a.H = H;
+  a.V = V;
+  a.gshift = w.group == 32 ? 5 : w.group == 64 ? 6 : 7;
+  a.ntiles = (V + kFewRows - 1) / kFewRows;
+  a.nsets = (H + 127) / 128;
+  a.scale = w.scale;
+  a.lds = w.lds;
+  a.out_f32 = out_f32;
+  a.out_bf16 = out_bf16;
+  a.ldo = ldo;
+  a.part = part;
+  a.err = h->lm_err;
+  const size_t hs = few_hidden(B, H);
+  a.slots = static_cast<int>((224 * 1024 - 1024 - hs) / (kFewWarps * kFewBox));
+  if (a.slots > kFewSlots) a.slots = kFewSlots;
+  const size_t smem = 1024 + static_cast<size_t>(a.slots) * kFewWarps * kFewBox + hs;
+  const int ctas = (a.ntiles + kFewWarps - 1) / kFewWarps;
+  const int grid = ctas < h->num_sms ? ctas : h->num_sms;
+  *grid_out = grid;
+  const bool pre = w.group < 128;
+  const cudaError_t e = B <= 8 ? (pre ? few_run<1, true>(mq, a, smem, grid, stream) : few_run<1, false>(mq, a, smem, grid, stream))
+                               : (pre ? few_run<2, true>(mq, a, smem, grid, stream) : few_run<2, false>(mq, a, smem, grid, stream));
+  if (e != cudaSuccess) return set_error(RL_ERR_CUDA, cudaGetErrorString(e));
+  return RL_OK;
+}
+
 rl_status q4_launch(rl_sampler* h, const uint16_t* hidden, int64_t ldh, const rl_q4_weight& w, int B, int H, int V,
                     float* out_f32, uint16_t* out_bf16, int64_t ldo, int32_t* out_tok, int32_t* row_status,
                     cudaStream_t stream) {
   if (cudaMemsetAsync(h->lm_err, 0, sizeof(int), stream) != cudaSuccess)
     return set_error(RL_ERR_CUDA, "rl_lmhead_q4: cudaMemsetAsync failed");
+  if (is_few(B, H)) {
+    int grid = 0;
+    rl_status st = few_launch(h, hidden, ldh, w, B, H, V, out_f32, out_bf16, ldo, out_tok ? h->lm_part : nullptr, &grid, stream);
+    if (st != RL_OK) return st;
+    if (out_tok) {
+      const cudaError_t e = lm_argmax(h->lm_part, B, grid, h->lm_err, out_tok, row_status, stream);
+      if (e != cudaSuccess) return set_error(RL_ERR_CUDA, cudaGetErrorString(e));
+    }
+    return RL_OK;
+  }
   CUtensorMap mq;
   if (!lm_tensor_map(&mq, w.q, 1, H / 2, V, w.ldq, kBM))
     return set_error(RL_ERR_INVALID_ARG, "rl_lmhead_q4: tensor map of the codes rejected (alignment or stride)");
