@@ -285,16 +285,18 @@ uint32_t pow2_cols(int n) {
 
 }  // namespace
 
-bool lm_tensor_map(CUtensorMap* m, const void* ptr, int elem_bytes, int inner, int rows, int64_t stride, int box_rows) {
+bool lm_tensor_map(CUtensorMap* m, const void* ptr, int elem_bytes, int inner, int rows, int64_t stride, int box_rows,
+                   int box_bytes) {
   EncodeTiledFn f = encode_fn();
   if (!f) return false;
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(rows)};
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride)};
-  const cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / elem_bytes), static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_bytes / elem_bytes), static_cast<cuuint32_t>(box_rows)};
   const cuuint32_t estr[2] = {1u, 1u};
   return f(m, elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr),
-           dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+           dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+           box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 cudaError_t lm_argmax(const uint64_t* part, int B, int G, const int* err, int32_t* out_tok, int32_t* row_status,

@@ -130,9 +130,10 @@ __device__ __forceinline__ uint64_t warp_colmax16(uint64_t (&k)[16]) {
 
 // Host side, in lmhead.cu.
 // A [rows, inner] matrix of 2-byte (bf16) or 1-byte elements at row stride
-// `stride` bytes, as boxes of 128 bytes x box_rows with the 128-byte swizzle;
-// what lies outside reads as zeros.
-bool lm_tensor_map(CUtensorMap* m, const void* ptr, int elem_bytes, int inner, int rows, int64_t stride, int box_rows);
+// `stride` bytes, as boxes of box_bytes (128 or 64) x box_rows with the swizzle
+// of that many bytes; what lies outside reads as zeros.
+bool lm_tensor_map(CUtensorMap* m, const void* ptr, int elem_bytes, int inner, int rows, int64_t stride, int box_rows,
+                   int box_bytes = 128);
 // Row b's token: the largest packed key of part[b, 0 .. G), or -1 and
 // RL_ERR_TIMEOUT where *err is set.
 cudaError_t lm_argmax(const uint64_t* part, int B, int G, const int* err, int32_t* out_tok, int32_t* row_status,

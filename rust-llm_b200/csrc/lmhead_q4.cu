@@ -31,12 +31,14 @@
 //
 // Up to 16 batch rows (q4_few_kernel) the hand-overs between those roles cost
 // more than the work: there each warp multiplies what it loads, on its own. It
-// streams the codes of 16 vocabulary rows through a ring of its own and takes
+// streams the codes of 32 vocabulary rows through a ring of its own and takes
 // them, as f16, straight into mma.sync fragments; the hidden states lie in
-// shared memory in the order of the fragments.
+// shared memory in the order of the fragments. A CTA's warps share its rows'
+// codes evenly, cut where they fall, so that none waits for another; the sums of
+// rows that two warps share are added at the end.
 //
 // Bound: HBM, half a byte a weight, up to about 100 batch rows; beside it the
-// expansion, 9 to 13 instructions for 8 weights. Every wait is bounded; where
+// expansion, 9 (f16) or 11 (bf16) instructions for 8 weights. Every wait is bounded; where
 // one runs out the error flag is set, copies in flight land and TMEM is freed.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -491,10 +493,9 @@ __global__ void __launch_bounds__((4 + NDQ + NEP) * 32, 1)
 // ---------------------------------------------------------------------------
 // Few batch rows
 // ---------------------------------------------------------------------------
-constexpr int kFewRows = 16;   // vocabulary rows of a tile (MMA M)
+constexpr int kFewRows = 32;   // vocabulary rows of a tile (two MMA Ms)
 constexpr int kFewWarps = 16;
-constexpr int kFewSlots = 6;   // copies in flight a warp, at most
-constexpr int kFewBox = kFewRows * 128;  // bytes of a copy: 256 codes (two sets) of each row
+constexpr int kFewSlots = 4;   // copies in flight a warp, at most
 constexpr int kFewHidden = 128 * 1024;   // bytes of the hidden states in shared memory, at most
 
 struct FewArgs {
@@ -502,10 +503,11 @@ struct FewArgs {
   int64_t ldh;
   int B, H, V;
   int gshift;
-  int ntiles, nsets;  // 16-row tiles; sets of K = 128
+  int ntiles, boxes;  // 32-row tiles; copies (boxes) a tile
   int slots;
   const uint16_t* scale;
   int64_t lds;
+  int vec;  // a box's scales of a row may be loaded at once
   float* out_f32;
   uint16_t* out_bf16;
   int64_t ldo;
@@ -524,13 +526,12 @@ __device__ __forceinline__ void expand_h(uint32_t w, uint32_t& lo, uint32_t& hi)
   hi = h2_bits(__hfma2(bits_h2((w & 0x00f000f0u) | 0x64006400u), bits_h2(0x2c002c00u), bits_h2(0xd480d480u)));
 }
 
-// D += A B: 16 x 8 f32, A 16 x 16 and B 16 x 8 f16.
-__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                        uint32_t b1) {
+// D = A B + C: 16 x 8 f32, A 16 x 16 and B 16 x 8 f16.
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
   asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 
 // 2^e, e in [-126, 127].
@@ -542,20 +543,61 @@ __device__ __forceinline__ int bring_to(float m, int k) {
 }
 __device__ __forceinline__ float finite_abs(float x) { return fabsf(x) < RL_POS_INF ? fabsf(x) : 0.0f; }
 
-// Fragments. A row's 16-byte piece holds 32 codes; in a set of K = 128, lane
-// (g, t) = (lane / 4, lane % 4) holds piece t of rows g and g + 8, and hidden
-// elements 32 t .. 32 t + 31 of batch row g. Step j of the set multiplies
-// elements 32 t + 4 j .. + 3 of the four t: K is summed in another order than it
-// lies in memory, alike for both operands.
+// Fragments. K is summed in another order than it lies in memory, alike for both
+// operands, so that a lane's codes lie together and a group is never split over
+// a step: of a group of G codes, lane (g, t) = (lane / 4, lane % 4) holds codes
+// t G / 4 .. of rows g and g + 8, and the same hidden elements of batch row g;
+// step j multiplies 4 j .. 4 j + 3 of those. A group's sum is scaled in f32.
 //
-// f16 holds code - 8 times a bf16 scale exactly (4 + 8 bits, less the sign's),
-// so where a set has more than one group (Pre) the scale is multiplied in before
-// the MMA, brought near 1 by the power of two of the row's largest scale in the
-// set; a set that is one group is scaled behind it. Either way a set's sum goes
-// into the row's in f32. Hidden states are bf16 brought near 2^10 by the power
-// of two of the batch row's largest. What a power of two drops is below 2^-24 of
-// the largest.
-template <int NT, bool Pre>  // batch tiles of 8
+// Hidden states are bf16 brought near 2^10 by the power of two of the batch
+// row's largest, and so exact in f16 but for what is below 2^-24 of the largest.
+template <int GS>
+__device__ __forceinline__ void row_words(const uint8_t* row, int swz, int half, int t, uint32_t (&w)[4]) {
+  // the four words of this lane in K = 128 of a row (64 bytes of a box, whose
+  // 16-byte pieces are swizzled by the row's number)
+  if constexpr (GS == 7) {
+    const uint4 c = *reinterpret_cast<const uint4*>(row + (((half * 4 + t) ^ swz) << 4));
+    w[0] = c.x, w[1] = c.y, w[2] = c.z, w[3] = c.w;
+  } else if constexpr (GS == 6) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint2 c = *reinterpret_cast<const uint2*>(row + (((half * 4 + 2 * i + (t >> 1)) ^ swz) << 4) + 8 * (t & 1));
+      w[2 * i] = c.x, w[2 * i + 1] = c.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      w[i] = *reinterpret_cast<const uint32_t*>(row + (((half * 4 + i) ^ swz) << 4) + 4 * t);
+  }
+}
+
+// The N scales of a box of one row, two to a word.
+template <int N>
+__device__ __forceinline__ void box_scales(const uint16_t* row, int box, int ngroups, bool vec, uint32_t (&w)[(N + 1) / 2]) {
+  const int g0 = box * N;
+  if (vec && N > 1) {  // on 2 N bytes, whole boxes only
+    if constexpr (N == 2) {
+      w[0] = __ldg(reinterpret_cast<const uint32_t*>(row + g0));
+    } else if constexpr (N == 4) {
+      const uint2 c = __ldg(reinterpret_cast<const uint2*>(row + g0));
+      w[0] = c.x, w[1] = c.y;
+    } else if constexpr (N == 8) {
+      const uint4 c = __ldg(reinterpret_cast<const uint4*>(row + g0));
+      w[0] = c.x, w[1] = c.y, w[2] = c.z, w[3] = c.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < (N + 1) / 2; ++i) {
+      const uint32_t lo = g0 + 2 * i < ngroups ? __ldg(row + g0 + 2 * i) : 0;
+      const uint32_t hi = N > 1 && g0 + 2 * i + 1 < ngroups ? __ldg(row + g0 + 2 * i + 1) : 0;
+      w[i] = lo | hi << 16;
+    }
+  }
+}
+
+// Batch tiles of 8; log2(group); halves of K = 128 in a box (a box of two needs
+// half the copies, of one half the room).
+template <int NT, int GS, int HB>
 __global__ void __launch_bounds__(kFewWarps * 32, 1)
     q4_few_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ FewArgs a) {
   extern __shared__ uint8_t few_smem_raw[];
@@ -565,35 +607,38 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   uint8_t* base = few_smem_raw + ((1024u - (smem_u32(few_smem_raw) & 1023u)) & 1023u);
-  uint8_t* ring = base + static_cast<size_t>(warp) * a.slots * kFewBox;  // this warp's
-  uint4* hs = reinterpret_cast<uint4*>(base + static_cast<size_t>(kFewWarps) * a.slots * kFewBox);  // [set][NT][4][32]
+  constexpr int kFewBox = kFewRows * 64 * HB;
+  const int ring_bytes = a.slots * kFewBox;
+  uint8_t* ring = base + static_cast<size_t>(warp) * ring_bytes;  // this warp's
+  uint4* hs = reinterpret_cast<uint4*>(base + static_cast<size_t>(kFewWarps) * ring_bytes);  // [half box][NT][4][32]
   if (lane == 0) {
     for (int i = 0; i < a.slots; ++i) mbar_init(&full[warp][i], 1);
     fence_mbar_init();
   }
   if (threadIdx.x < NT * 8) best[threadIdx.x] = 0ull;
   __syncwarp();
-  // ---- this warp's stream of codes ----
-  const int stride = static_cast<int>(gridDim.x) * kFewWarps;
-  const int tile0 = blockIdx.x * kFewWarps + warp;
-  const int boxes = (a.nsets + 1) >> 1;  // copies a tile
+  // ---- this warp's boxes: an even share of the CTA's tiles ----
+  const int nb = a.boxes;
+  const int tfirst = static_cast<int>(static_cast<int64_t>(a.ntiles) * blockIdx.x / gridDim.x);
+  const int tlast = static_cast<int>(static_cast<int64_t>(a.ntiles) * (blockIdx.x + 1) / gridDim.x);
+  const int64_t units = static_cast<int64_t>(tlast - tfirst) * nb;
+  const int u0 = static_cast<int>(units * warp / kFewWarps), u1 = static_cast<int>(units * (warp + 1) / kFewWarps);
   const uint64_t pol = lm_policy_first();
-  int ctile = tile0, cbox = 0;  // the next copy
-  uint32_t issued = 0;
+  int cu = u0, cbox = u0 % nb, ctile = tfirst + u0 / nb;  // the next copy
   Ring rc;
   const auto copy = [&] {  // one lane
     mbar_expect_tx(&full[warp][rc.slot], kFewBox);
-    tma_load_2d(ring + rc.slot * kFewBox, &tmQ, cbox * 128, ctile * kFewRows, &full[warp][rc.slot], pol);
+    tma_load_2d(ring + rc.slot * kFewBox, &tmQ, cbox * (64 * HB), ctile * kFewRows, &full[warp][rc.slot], pol);
     rc.next(a.slots);
-    ++issued;
-    if (++cbox == boxes) {
+    ++cu;
+    if (++cbox == nb) {
       cbox = 0;
-      ctile += stride;
+      ++ctile;
     }
   };
   if (lane == 0) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmQ)) : "memory");
-    for (int i = 0; i < a.slots && ctile < a.ntiles; ++i) copy();
+    for (int i = 0; i < a.slots && cu < u1; ++i) copy();
   }
   // ---- the hidden states, as f16 fragments ----
   for (int b = warp; b < NT * 8; b += kFewWarps) {
@@ -611,147 +656,184 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1)
     if (lane == 0) hexp[b] = bring_to(m, 10);
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < a.nsets * NT * 4 * 32; i += kFewWarps * 32) {
-    // fragment i of lane l: steps 2 jj and 2 jj + 1 of batch tile n in the set
-    const int l = i & 31, jj = (i >> 5) & 3, n = (i >> 7) % NT, set = (i >> 7) / NT;
-    const int b = n * 8 + (l >> 2), k0 = set * 128 + 32 * (l & 3) + 8 * jj;
+  for (int i = threadIdx.x; i < nb * HB * NT * 4 * 32; i += kFewWarps * 32) {
+    // word w of lane l: eight elements of batch tile n in the hk-th K = 128
+    const int l = i & 31, w = (i >> 5) & 3, n = (i >> 7) % NT, hk = (i >> 7) / NT;
+    constexpr int kWords = 1 << (GS - 5);  // words of a lane's share of a group
+    const int b = n * 8 + (l >> 2), k0 = hk * 128 + (w / kWords << GS) + (l & 3) * (8 * kWords) + 8 * (w % kWords);
     uint4 v = {0u, 0u, 0u, 0u};
     if (b < a.B && k0 < a.H) v = __ldg(reinterpret_cast<const uint4*>(a.hidden + static_cast<int64_t>(b) * a.ldh + k0));
     const float f = pow2f(hexp[b]);
-    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    uint32_t x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int k = 0; k < 4; ++k) w[k] = h2_bits(__floats2half2_rn(bf16_at(w[k], 0) * f, bf16_at(w[k], 1) * f));
-    hs[i] = make_uint4(w[0], w[1], w[2], w[3]);
+    for (int k = 0; k < 4; ++k) x[k] = h2_bits(__floats2half2_rn(bf16_at(x[k], 0) * f, bf16_at(x[k], 1) * f));
+    hs[i] = make_uint4(x[0], x[1], x[2], x[3]);
   }
   __syncthreads();
 
   // ---- tiles ----
-  const int ngroups = a.H >> a.gshift;
+  const int ngroups = a.H >> GS;
+  constexpr int kNs = (128 * HB) >> GS, kSw = (kNs + 1) / 2;  // scales of a box, in words
+  const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   bool ok = true;
   Ring r;
-  for (int tile = tile0; tile < a.ntiles && ok; tile += stride) {
-    const int64_t v0 = static_cast<int64_t>(tile) * kFewRows + g, v1 = v0 + 8;
-    const uint16_t* sp0 = a.scale + (v0 < a.V ? v0 : 0) * a.lds;
-    const uint16_t* sp1 = a.scale + (v1 < a.V ? v1 : 0) * a.lds;
-    // this lane's group of a set, rows g and g + 8
-    const auto scales = [&](int set) {
-      const int gi = (set * 128 + 32 * t) >> a.gshift;
-      return gi < ngroups ? static_cast<uint32_t>(__ldg(sp0 + gi)) | static_cast<uint32_t>(__ldg(sp1 + gi)) << 16 : 0u;
-    };
-    float acc[NT][4];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.0f;
-    uint32_t sc1 = scales(0), sc2 = scales(1);
-    for (int box = 0; box < boxes; ++box) {
-      if (!q4_wait(&full[warp][r.slot], r.par)) {
-        ok = false;
-        break;
-      }
-      const uint8_t* src = ring + r.slot * kFewBox;
-      uint4 c[2][2];
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const int piece = (s * 4 + t) ^ g;
-        c[s][0] = *reinterpret_cast<const uint4*>(src + g * 128 + piece * 16);
-        c[s][1] = *reinterpret_cast<const uint4*>(src + (g + 8) * 128 + piece * 16);
-      }
-      __syncwarp();
-      if (lane == 0 && ctile < a.ntiles) copy();  // the slot is read: the stream goes on in it
-      r.next(a.slots);
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const int set = 2 * box + s;
-        if (set >= a.nsets) break;
-        const float x = bf16_at(sc1, 0), y = bf16_at(sc1, 1);
-        sc1 = sc2;
-        sc2 = scales(set + 2);
-        float d[NT][4];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) d[n][0] = d[n][1] = d[n][2] = d[n][3] = 0.0f;
-        float up0 = x, up1 = y;
-        __half2 s0, s1;
-        if constexpr (Pre) {
-          float m0 = finite_abs(x), m1 = finite_abs(y);
-          m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, 1));
-          m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, 1));
-          m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, 2));
-          m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, 2));
-          const int e0 = bring_to(m0, 0), e1 = bring_to(m1, 0);
-          s0 = __float2half2_rn(x * pow2f(e0));
-          s1 = __float2half2_rn(y * pow2f(e1));
-          up0 = pow2f(-e0), up1 = pow2f(-e1);
-        }
-        const uint32_t w0[4] = {c[s][0].x, c[s][0].y, c[s][0].z, c[s][0].w};
-        const uint32_t w1[4] = {c[s][1].x, c[s][1].y, c[s][1].z, c[s][1].w};
-        const uint4* h = hs + set * (NT * 4 * 32) + lane;
-#pragma unroll
-        for (int jj = 0; jj < 4; ++jj) {
-          uint32_t e[2][4];
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            expand_h(w0[jj] >> (8 * k), e[k][0], e[k][2]);
-            expand_h(w1[jj] >> (8 * k), e[k][1], e[k][3]);
-            if constexpr (Pre) {
-              e[k][0] = h2_bits(__hmul2(bits_h2(e[k][0]), s0));
-              e[k][2] = h2_bits(__hmul2(bits_h2(e[k][2]), s0));
-              e[k][1] = h2_bits(__hmul2(bits_h2(e[k][1]), s1));
-              e[k][3] = h2_bits(__hmul2(bits_h2(e[k][3]), s1));
-            }
-          }
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const uint4 hv = h[(n * 4 + jj) * 32];
-            mma_f16(d[n], e[0][0], e[0][1], e[0][2], e[0][3], hv.x, hv.y);
-            mma_f16(d[n], e[1][0], e[1][1], e[1][2], e[1][3], hv.z, hv.w);
-          }
-        }
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          acc[n][0] = fmaf(up0, d[n][0], acc[n][0]);
-          acc[n][1] = fmaf(up0, d[n][1], acc[n][1]);
-          acc[n][2] = fmaf(up1, d[n][2], acc[n][2]);
-          acc[n][3] = fmaf(up1, d[n][3], acc[n][3]);
-        }
-      }
-    }
-    if (!ok) break;
-    // ---- rows g, g + 8 of batch rows 2 t, 2 t + 1 ----
+  float acc[2][NT][4];
+  // logits of a tile from the fragments of its sums
+  const auto finish = [&](int tile) {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const int b = n * 8 + 2 * t + k;
         const float back = pow2f(-hexp[b]);
-        const float y0 = acc[n][k] * back, y1 = acc[n][2 + k] * back;
-        if (b < a.B) {
-          const int64_t at = static_cast<int64_t>(b) * a.ldo;
-          if (a.out_f32) {
-            if (v0 < a.V) a.out_f32[at + v0] = y0;
-            if (v1 < a.V) a.out_f32[at + v1] = y1;
-          }
-          if (a.out_bf16) {
-            if (v0 < a.V) a.out_bf16[at + v0] = __bfloat16_as_ushort(__float2bfloat16_rn(y0));
-            if (v1 < a.V) a.out_bf16[at + v1] = __bfloat16_as_ushort(__float2bfloat16_rn(y1));
+        uint64_t key = 0ull;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {  // rows g, g + 8, g + 16, g + 24
+          const int64_t v = static_cast<int64_t>(tile) * kFewRows + 8 * i + g;
+          const float y = acc[i >> 1][n][2 * (i & 1) + k] * back;
+          if (v < a.V) {
+            if (b < a.B) {
+              if (a.out_f32) a.out_f32[static_cast<int64_t>(b) * a.ldo + v] = y;
+              if (a.out_bf16) a.out_bf16[static_cast<int64_t>(b) * a.ldo + v] = __bfloat16_as_ushort(__float2bfloat16_rn(y));
+            }
+            key = umax64(key, lm_key(y, static_cast<int>(v)));
           }
         }
         if (a.part) {
-          uint64_t key = v0 < a.V ? lm_key(y0, static_cast<int>(v0)) : 0ull;
-          if (v1 < a.V) key = umax64(key, lm_key(y1, static_cast<int>(v1)));
 #pragma unroll
           for (int o = 16; o > 2; o >>= 1) key = umax64(key, shfl_xor64(key, o));  // over g
           if (g == 0 && b < a.B) atomicMax(&best[b], static_cast<unsigned long long>(key));
         }
       }
     }
+  };
+  // where a tile's sums lie that this warp has a part of: 0 the end of a tile
+  // that began before u0, 1 the beginning of one that ends behind u1
+  float* parts = reinterpret_cast<float*>(ring);  // [2][2 * NT * 4][32], in the ring once it is read
+  int kept = 0;
+  float first[2][NT][4];
+  int u = u0;
+  while (u < u1 && ok) {
+    const int tile = tfirst + u / nb;
+    const int box0 = u % nb, box1 = min(nb, box0 + (u1 - u));
+    const uint16_t* sp[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t v = static_cast<int64_t>(tile) * kFewRows + 8 * i + g;
+      sp[i] = a.scale + (v < a.V ? v : 0) * a.lds;
+    }
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) acc[m][n][0] = acc[m][n][1] = acc[m][n][2] = acc[m][n][3] = 0.0f;
+    uint32_t ahead[4][kSw];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) box_scales<kNs>(sp[i], box0, ngroups, a.vec, ahead[i]);
+    for (int box = box0; box < box1; ++box) {
+      uint32_t sc[4][kSw];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int k = 0; k < kSw; ++k) sc[i][k] = ahead[i][k];
+      if (box + 1 < box1) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) box_scales<kNs>(sp[i], box + 1, ngroups, a.vec, ahead[i]);
+      }
+      if (!q4_wait(&full[warp][r.slot], r.par)) {
+        ok = false;
+        break;
+      }
+      const uint8_t* src = ring + r.slot * kFewBox + g * (64 * HB);
+      const int swz = HB == 2 ? g : g >> 1;  // of rows g, g + 8, ... alike
+#pragma unroll
+      for (int half = 0; half < HB; ++half) {
+        uint32_t w[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) row_words<GS>(src + i * (8 * 64 * HB), swz, half, t, w[i]);
+        if (half == HB - 1) {
+          __syncwarp();
+          if (lane == 0 && cu < u1) copy();  // the slot is read: the stream goes on in it
+          r.next(a.slots);
+        }
+        const uint4* h = hs + (HB * box + half) * (NT * 4 * 32) + lane;
+        constexpr int kWords = 1 << (GS - 5);
+        float d[2][NT][4];
+#pragma unroll
+        for (int jw = 0; jw < 4; ++jw) {
+          uint4 hv[NT];
+#pragma unroll
+          for (int n = 0; n < NT; ++n) hv[n] = h[(n * 4 + jw) * 32];
+          const bool begins = jw % kWords == 0, ends = jw % kWords == kWords - 1;
+#pragma unroll
+          for (int m = 0; m < 2; ++m) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              uint32_t e[4];
+              expand_h(w[2 * m][jw] >> (8 * k), e[0], e[2]);
+              expand_h(w[2 * m + 1][jw] >> (8 * k), e[1], e[3]);
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                if (begins && k == 0) mma_f16(d[m][n], e, hv[n].x, hv[n].y, zero);
+                else mma_f16(d[m][n], e, k ? hv[n].z : hv[n].x, k ? hv[n].w : hv[n].y, d[m][n]);
+              }
+            }
+          }
+          if (ends) {
+            const int gi = (half * 4 + jw) / kWords;  // group of the box
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+              const float x = bf16_at(sc[2 * m][gi >> 1], gi & 1), y = bf16_at(sc[2 * m + 1][gi >> 1], gi & 1);
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                acc[m][n][0] = fmaf(x, d[m][n][0], acc[m][n][0]);
+                acc[m][n][1] = fmaf(x, d[m][n][1], acc[m][n][1]);
+                acc[m][n][2] = fmaf(y, d[m][n][2], acc[m][n][2]);
+                acc[m][n][3] = fmaf(y, d[m][n][3], acc[m][n][3]);
+              }
+            }
+          }
+        }
+      }
+    }
+    if (!ok) break;
+    if (box0 == 0 && box1 == nb) {
+      finish(tile);
+    } else if (box0 > 0) {
+      kept |= 1;
+#pragma unroll
+      for (int i = 0; i < 2 * NT * 4; ++i) first[i / (NT * 4)][(i >> 2) % NT][i & 3] = acc[i / (NT * 4)][(i >> 2) % NT][i & 3];
+    } else {
+      kept |= 2;
+    }
+    u += box1 - box0;
   }
   if (!ok) {
     // behind a wait that ran out: every issued copy lands before the CTA returns
-    if (lane == 0)
-      for (int i = 0; i < a.slots; ++i) {
-        const uint32_t n = issued / a.slots + (static_cast<uint32_t>(i) < issued % a.slots ? 1u : 0u);
-        if (n > 0) mbar_wait(&full[warp][i], (n - 1u) & 1u, kWaitBudget);
-      }
+    const int issued = __shfl_sync(0xffffffffu, cu, 0) - u0;
+    for (int i = 0; i < a.slots; ++i) {
+      const int n = issued / a.slots + (i < issued % a.slots ? 1 : 0);
+      if (n > 0) mbar_wait(&full[warp][i], (n - 1) & 1, kWaitBudget);
+    }
     atomicExch(a.err, 1);
+  }
+  // ---- tiles that warps share: the one that has the beginning adds the rest ----
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 2 * NT * 4; ++i)
+    if (kept & 1) parts[i * 32 + lane] = first[i / (NT * 4)][(i >> 2) % NT][i & 3];
+  __syncthreads();
+  if ((kept & 2) && ok) {
+    const int tile = tfirst + (u1 - 1) / nb;
+    const int end = (tile + 1 - tfirst) * nb;
+    for (int w = warp + 1; w < kFewWarps; ++w) {
+      const int wu0 = static_cast<int>(units * w / kFewWarps), wu1 = static_cast<int>(units * (w + 1) / kFewWarps);
+      if (wu0 >= end) break;
+      if (wu0 == wu1) continue;
+      const float* p = reinterpret_cast<const float*>(base + static_cast<size_t>(w) * ring_bytes);
+#pragma unroll
+      for (int i = 0; i < 2 * NT * 4; ++i) acc[i / (NT * 4)][(i >> 2) % NT][i & 3] += p[i * 32 + lane];
+    }
+    finish(tile);
   }
   __syncthreads();
   if (a.part && static_cast<int>(threadIdx.x) < a.B)
@@ -867,30 +949,41 @@ cudaError_t q4_run(const CUtensorMap& mq, const CUtensorMap& mx, Q4Args a, int g
   return cudaGetLastError();
 }
 
-template <int NT, bool Pre>
+template <int NT, int GS, int HB>
 cudaError_t few_run(const CUtensorMap& mq, const FewArgs& a, size_t smem, int grid, cudaStream_t stream) {
   static std::atomic<int> configured[64];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev < 0 || dev >= 64 || !configured[dev].load(std::memory_order_acquire)) {
-    e = cudaFuncSetAttribute(q4_few_kernel<NT, Pre>, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024);
+    e = cudaFuncSetAttribute(q4_few_kernel<NT, GS, HB>, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024);
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) configured[dev].store(1, std::memory_order_release);
   }
-  q4_few_kernel<NT, Pre><<<grid, kFewWarps * 32, smem, stream>>>(mq, a);
+  q4_few_kernel<NT, GS, HB><<<grid, kFewWarps * 32, smem, stream>>>(mq, a);
   return cudaGetLastError();
+}
+
+template <int NT, int HB>
+cudaError_t few_run(const CUtensorMap& mq, const FewArgs& a, int group, size_t smem, int grid, cudaStream_t stream) {
+  return group == 32   ? few_run<NT, 5, HB>(mq, a, smem, grid, stream)
+         : group == 64 ? few_run<NT, 6, HB>(mq, a, smem, grid, stream)
+                       : few_run<NT, 7, HB>(mq, a, smem, grid, stream);
 }
 
 // Whether the hidden states fit shared memory beside the rings (H <= 8192 at
 // 8 batch rows, 4096 at 16).
-size_t few_hidden(int B, int H) { return static_cast<size_t>(B <= 8 ? 8 : 16) * ((H + 127) / 128) * 256; }
+size_t few_hidden(int B, int H) { return static_cast<size_t>(B <= 8 ? 8 : 16) * ((H + 255) / 256) * 512; }
 bool is_few(int B, int H) { return B <= 16 && few_hidden(B, H) <= kFewHidden; }
 
 rl_status few_launch(rl_sampler* h, const uint16_t* hidden, int64_t ldh, const rl_q4_weight& w, int B, int H, int V,
                      float* out_f32, uint16_t* out_bf16, int64_t ldo, uint64_t* part, int* grid_out, cudaStream_t stream) {
+  // boxes of K = 256 where two of them a warp fit beside the hidden states
+  const size_t hs = few_hidden(B, H), room = 224 * 1024 - 1024 - hs;
+  const int hb = room / (kFewWarps * kFewRows * 128) >= 2 ? 2 : 1;
+  const size_t box = static_cast<size_t>(kFewRows) * 64 * hb;
   CUtensorMap mq;
-  if (!lm_tensor_map(&mq, w.q, 1, H / 2, V, w.ldq, kFewRows))
+  if (!lm_tensor_map(&mq, w.q, 1, H / 2, V, w.ldq, kFewRows, 64 * hb))
     return set_error(RL_ERR_INVALID_ARG, "rl_lmhead_q4: tensor map of the codes rejected (alignment or stride)");
   FewArgs a = {};
   a.hidden = hidden;
@@ -900,7 +993,7 @@ rl_status few_launch(rl_sampler* h, const uint16_t* hidden, int64_t ldh, const r
   a.V = V;
   a.gshift = w.group == 32 ? 5 : w.group == 64 ? 6 : 7;
   a.ntiles = (V + kFewRows - 1) / kFewRows;
-  a.nsets = (H + 127) / 128;
+  a.boxes = (H + 128 * hb - 1) / (128 * hb);
   a.scale = w.scale;
   a.lds = w.lds;
   a.out_f32 = out_f32;
@@ -908,16 +1001,18 @@ rl_status few_launch(rl_sampler* h, const uint16_t* hidden, int64_t ldh, const r
   a.ldo = ldo;
   a.part = part;
   a.err = h->lm_err;
-  const size_t hs = few_hidden(B, H);
-  a.slots = static_cast<int>((224 * 1024 - 1024 - hs) / (kFewWarps * kFewBox));
+  const int scales = 128 * hb / w.group;  // of a box
+  a.vec = H % (128 * hb) == 0 &&
+          (reinterpret_cast<uintptr_t>(w.scale) | static_cast<uint64_t>(w.lds) * 2u) % (2u * static_cast<unsigned>(scales)) == 0;
+  a.slots = static_cast<int>(room / (kFewWarps * box));
   if (a.slots > kFewSlots) a.slots = kFewSlots;
-  const size_t smem = 1024 + static_cast<size_t>(a.slots) * kFewWarps * kFewBox + hs;
-  const int ctas = (a.ntiles + kFewWarps - 1) / kFewWarps;
-  const int grid = ctas < h->num_sms ? ctas : h->num_sms;
+  const size_t smem = 1024 + static_cast<size_t>(a.slots) * kFewWarps * box + hs;
+  const int grid = a.ntiles < h->num_sms ? a.ntiles : h->num_sms;
   *grid_out = grid;
-  const bool pre = w.group < 128;
-  const cudaError_t e = B <= 8 ? (pre ? few_run<1, true>(mq, a, smem, grid, stream) : few_run<1, false>(mq, a, smem, grid, stream))
-                               : (pre ? few_run<2, true>(mq, a, smem, grid, stream) : few_run<2, false>(mq, a, smem, grid, stream));
+  const cudaError_t e = B <= 8 ? (hb == 2 ? few_run<1, 2>(mq, a, w.group, smem, grid, stream)
+                                          : few_run<1, 1>(mq, a, w.group, smem, grid, stream))
+                               : (hb == 2 ? few_run<2, 2>(mq, a, w.group, smem, grid, stream)
+                                          : few_run<2, 1>(mq, a, w.group, smem, grid, stream));
   if (e != cudaSuccess) return set_error(RL_ERR_CUDA, cudaGetErrorString(e));
   return RL_OK;
 }
