@@ -22,7 +22,7 @@
 //                 that is what counts: a block's operands (expanded codes and
 //                 hidden states) share one full and one free barrier, so that
 //                 it waits and commits once for both
-//   the last      (4 or 8) read a group's accumulator back, times the row's
+//   the last      read a group's accumulator back, times the row's
 //                 scale (a thread a row), into f32 sums in registers; at the
 //                 tile's end logits are stored along the vocabulary, or the
 //                 rows' running maxima kept
@@ -128,8 +128,7 @@ struct Q4Bars {
   uint32_t tmem;
 };
 
-// mbar_wait, but without its clock where the phase is over already.
-__device__ __forceinline__ bool q4_wait(uint64_t* bar, uint32_t parity) {
+__device__ __forceinline__ bool q4_try(uint64_t* bar, uint32_t parity) {
   uint32_t done;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
@@ -138,7 +137,19 @@ __device__ __forceinline__ bool q4_wait(uint64_t* bar, uint32_t parity) {
       : "=r"(done)
       : "r"(smem_u32(bar)), "r"(parity)
       : "memory");
-  return done || mbar_wait(bar, parity, kWaitBudget);
+  return done != 0;
+}
+// A bounded wait as mbar_wait, but without its clock where the phase is over
+// already, and asleep between tries: here most warps wait most of the time, and
+// their tries would take the issue slots of those that work.
+__device__ __forceinline__ bool q4_wait(uint64_t* bar, uint32_t parity) {
+  if (q4_try(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (true) {
+    __nanosleep(32);
+    if (q4_try(bar, parity)) return true;
+    if (clock64() - t0 > kWaitBudget) return false;
+  }
 }
 // One lane of a converged warp.
 __device__ __forceinline__ bool elect_one() {
@@ -161,9 +172,16 @@ struct Ring {
       par ^= 1u;
     }
   }
+  __device__ __forceinline__ void skip(int d, int n) {
+    slot += d;
+    while (slot >= n) {
+      slot -= n;
+      par ^= 1u;
+    }
+  }
 };
 
-template <int N, int NDQ, int NEP>  // MMA N; expanding warps (a multiple of 4); epilogue warps (4 or 8)
+template <int N, int NDQ, int NEP>  // MMA N; expanding warps, epilogue warps (multiples of 4)
 __global__ void __launch_bounds__((4 + NDQ + NEP) * 32, 1)
     q4_mma_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmX,
                   const __grid_constant__ Q4Args a) {
@@ -178,7 +196,7 @@ __global__ void __launch_bounds__((4 + NDQ + NEP) * 32, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < a.qslots; ++i) mbar_init(&bars.qfull[i], 1), mbar_init(&bars.qempty[i], NDQ);
+    for (int i = 0; i < a.qslots; ++i) mbar_init(&bars.qfull[i], 1), mbar_init(&bars.qempty[i], 8);
     for (int i = 0; i < a.slots; ++i) mbar_init(&bars.full[i], 4 + 1), mbar_init(&bars.free[i], 1);
     for (int i = 0; i < a.dbufs; ++i) mbar_init(&bars.dfull[i], 1), mbar_init(&bars.dempty[i], NEP);
     for (int i = 0; i < kSSlots; ++i) mbar_init(&bars.sfull[i], 32), mbar_init(&bars.sempty[i], NEP);
@@ -358,51 +376,63 @@ __global__ void __launch_bounds__((4 + NDQ + NEP) * 32, 1)
     constexpr int kTurns = NDQ / 4;
     const int quad = warp & 3;
     const int row = quad * 32 + lane;
-    int turn = (warp - 4) >> 2;  // blocks until this warp's next
+    const uint8_t* qrow = qring + row * 128;
+    const uint32_t to0 = tmem_a + (static_cast<uint32_t>(quad * 32) << 16);
+    const int swz = row & 7;
     Ring rq, r;
-    for (int tile = blockIdx.x; tile < a.ntiles && ok; tile += gridDim.x) {
-      for (int kb = 0; kb < blocks && ok; ++kb) {
-        const bool mine = turn == 0;
-        turn = mine ? kTurns - 1 : turn - 1;
-        const bool last = (kb & 1) == 1 || kb == blocks - 1;  // of a copy of codes
-        if ((mine || last) && !q4_wait(&bars.qfull[rq.slot], rq.par)) {
-          ok = false;
-          break;
-        }
-        if (mine) {
-          if (!q4_wait(&bars.free[r.slot], r.par ^ 1u)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint8_t* src = qring + rq.slot * kQTile + row * 128;
-          const uint32_t to = tmem_a + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(r.slot * kSlotCols);
-          const int nst = min(2, a.kstages - 2 * kb);
-          for (int st = 0; st < nst; ++st) {
-            const int c0 = (kb & 1) * 4 + st * 2;  // 16-byte piece of the row's 128
-            uint32_t e[32];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const uint4 c = *reinterpret_cast<const uint4*>(src + (((c0 + i) ^ (row & 7)) << 4));
-              expand(c.x, e + 16 * i);
-              expand(c.y, e + 16 * i + 4);
-              expand(c.z, e + 16 * i + 8);
-              expand(c.w, e + 16 * i + 12);
-            }
-            tmem_st32(to + 32u * st, e);
-          }
-          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive1(&bars.full[r.slot]);
-        }
-        if (last) {
-          __syncwarp();
-          if (lane == 0) mbar_arrive1(&bars.qempty[rq.slot]);
-          rq.next(a.qslots);
-        }
-        r.next(a.slots);
+    int tile = blockIdx.x, kb = (warp - 4) >> 2;
+    r.skip(kb, a.slots);
+    rq.skip(kb >> 1, a.qslots);
+    while (kb >= blocks) {  // (few blocks a tile)
+      kb -= blocks;
+      tile += gridDim.x;
+    }
+    if (blocks < kTurns) {  // the copies of the tiles passed over
+      rq = Ring();
+      rq.skip(((tile - static_cast<int>(blockIdx.x)) / static_cast<int>(gridDim.x)) * qtiles + (kb >> 1), a.qslots);
+    }
+    while (tile < a.ntiles && ok) {
+      if (!q4_wait(&bars.qfull[rq.slot], rq.par) || !q4_wait(&bars.free[r.slot], r.par ^ 1u)) {
+        ok = false;
+        break;
       }
+      tc_fence_after();
+      const uint8_t* src = qrow + rq.slot * kQTile;
+      const uint32_t to = to0 + static_cast<uint32_t>(r.slot * kSlotCols);
+      const int nst = min(2, a.kstages - 2 * kb);
+      for (int st = 0; st < nst; ++st) {
+        const int c0 = (kb & 1) * 4 + st * 2;  // 16-byte piece of the row's 128
+        uint32_t e[32];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint4 c = *reinterpret_cast<const uint4*>(src + (((c0 + i) ^ swz) << 4));
+          expand(c.x, e + 16 * i);
+          expand(c.y, e + 16 * i + 4);
+          expand(c.z, e + 16 * i + 8);
+          expand(c.w, e + 16 * i + 12);
+        }
+        tmem_st32(to + 32u * st, e);
+      }
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive1(&bars.full[r.slot]);
+        // a copy of codes is free once the four quadrants have read both of its
+        // blocks (eight arrivals; its only block counts twice)
+        mbar_arrive1(&bars.qempty[rq.slot]);
+        if ((kb & 1) == 0 && kb == blocks - 1) mbar_arrive1(&bars.qempty[rq.slot]);
+      }
+      // on to this warp's next block
+      r.skip(kTurns, a.slots);
+      int copies = -(kb >> 1);
+      kb += kTurns;
+      while (kb >= blocks) {
+        kb -= blocks;
+        tile += gridDim.x;
+        copies += qtiles;
+      }
+      rq.skip(copies + (kb >> 1), a.qslots);
     }
   } else {
     // ---- epilogue ----
@@ -439,6 +469,8 @@ __global__ void __launch_bounds__((4 + NDQ + NEP) * 32, 1)
           const float s = bf16_at(sw, g & 1);
           const uint32_t at = tmem + (static_cast<uint32_t>(quad * 32) << 16) +
                               static_cast<uint32_t>(rd.slot * a.dcols + i * N + col0);
+          // sixteen columns at a time: wider loads keep the MMAs from TMEM (128
+          // batch rows, H 4096, V 128256: 157 us, with 32 columns 200)
 #pragma unroll
           for (int c = 0; c < NC; c += 16) {
             uint32_t r[16];
@@ -1018,9 +1050,10 @@ rl_status few_launch(rl_sampler* h, const uint16_t* hidden, int64_t ldh, const r
 }
 
 rl_status q4_launch(rl_sampler* h, const uint16_t* hidden, int64_t ldh, const rl_q4_weight& w, int B, int H, int V,
-                    float* out_f32, uint16_t* out_bf16, int64_t ldo, int32_t* out_tok, int32_t* row_status,
+                    float* out_f32, uint16_t* out_bf16, int64_t ldo, int32_t* out_tok, int32_t* row_status, bool flagged,
                     cudaStream_t stream) {
-  if (cudaMemsetAsync(h->lm_err, 0, sizeof(int), stream) != cudaSuccess)
+  // the flag is read where there are statuses to give
+  if (flagged && cudaMemsetAsync(h->lm_err, 0, sizeof(int), stream) != cudaSuccess)
     return set_error(RL_ERR_CUDA, "rl_lmhead_q4: cudaMemsetAsync failed");
   if (is_few(B, H)) {
     int grid = 0;
@@ -1065,7 +1098,7 @@ rl_status q4_launch(rl_sampler* h, const uint16_t* hidden, int64_t ldh, const rl
     if (!lm_tensor_map(&mx, hidden + static_cast<int64_t>(b0) * ldh, 2, H, Bc, ldh * 2, N))
       return set_error(RL_ERR_INVALID_ARG, "rl_lmhead_q4: hidden tensor map rejected (alignment or stride)");
     cudaError_t e = N == 16   ? q4_run<16, 8, 4>(mq, mx, a, grid, stream)
-                    : N == 32 ? q4_run<32, 8, 4>(mq, mx, a, grid, stream)
+                    : N == 32 ? q4_run<32, 8, 8>(mq, mx, a, grid, stream)
                     : N == 64 ? q4_run<64, 8, 8>(mq, mx, a, grid, stream)
                     : N == 96 ? q4_run<96, 8, 8>(mq, mx, a, grid, stream)
                               : q4_run<128, 8, 8>(mq, mx, a, grid, stream);
@@ -1110,7 +1143,7 @@ rl_status rl_lmhead_q4_logits(rl_sampler* h, const uint16_t* hidden, int64_t ldh
   rl::LmDeviceGuard g(h->device);
   if (!g.ok) return rl::set_error(RL_ERR_CUDA, "rl_lmhead_q4_logits: cudaSetDevice failed");
   return rl::q4_launch(h, hidden, ldh, *weight, B, H, V, out_dtype == RL_F32 ? static_cast<float*>(out_logits) : nullptr,
-                       out_dtype == RL_BF16 ? static_cast<uint16_t*>(out_logits) : nullptr, ldo, nullptr, nullptr,
+                       out_dtype == RL_BF16 ? static_cast<uint16_t*>(out_logits) : nullptr, ldo, nullptr, nullptr, false,
                        static_cast<cudaStream_t>(stream));
 }
 
@@ -1124,7 +1157,7 @@ rl_status rl_lmhead_q4_greedy(rl_sampler* h, const uint16_t* hidden, int64_t ldh
   if (B == 0) return RL_OK;
   rl::LmDeviceGuard g(h->device);
   if (!g.ok) return rl::set_error(RL_ERR_CUDA, "rl_lmhead_q4_greedy: cudaSetDevice failed");
-  return rl::q4_launch(h, hidden, ldh, *weight, B, H, V, out_logits, nullptr, ldo, out_tok, row_status,
+  return rl::q4_launch(h, hidden, ldh, *weight, B, H, V, out_logits, nullptr, ldo, out_tok, row_status, true,
                        static_cast<cudaStream_t>(stream));
 }
 
@@ -1142,7 +1175,7 @@ rl_status rl_lmhead_q4_sample(rl_sampler* h, const uint16_t* hidden, int64_t ldh
   rl::LmDeviceGuard g(h->device);
   if (!g.ok) return rl::set_error(RL_ERR_CUDA, "rl_lmhead_q4_sample: cudaSetDevice failed");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  st = rl::q4_launch(h, hidden, ldh, *weight, B, H, V, h->stage_logits, nullptr, V, nullptr, nullptr, s);
+  st = rl::q4_launch(h, hidden, ldh, *weight, B, H, V, h->stage_logits, nullptr, V, nullptr, nullptr, true, s);
   if (st != RL_OK) return st;
   st = rl_sample_batch(h, h->stage_logits, RL_F32, B, V, V, hist, hist_len, hist_stride, nullptr, 0, params, uniforms,
                        out_tok, out_prob, row_status, stream);
