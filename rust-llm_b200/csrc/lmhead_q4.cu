@@ -57,19 +57,13 @@ namespace {
 constexpr int kBM = 128;        // vocabulary rows of a tile
 constexpr int kQTile = kBM * 128;  // bytes of a copy of codes: 256 codes of each row
 constexpr int kSlotCols = 64;   // TMEM columns of a block's expanded codes
-constexpr int kSMax = 6;        // blocks in flight, at most
-constexpr int kDMax = 4;        // accumulator buffers, at most
 constexpr int kSBox = kBM * 16;  // bytes of a box of scales: 8 groups of each row
 constexpr int kSSlots = 8;
 constexpr int kQMax = 8;
 
 struct Q4Args {
   int B, H, V;
-  int gshift;              // log2(group)
-  int ntiles, kstages;     // kstages = H / 64
-  int split;               // accumulators are handed over 1 or 2 times a block
-  int dbufs, dcols;        // accumulator buffers and their columns
-  int slots;               // blocks in flight
+  int ntiles, kstages;  // kstages = H / 64
   int qslots;
   const uint16_t* scale;
   int64_t lds;
@@ -121,8 +115,8 @@ __device__ __forceinline__ void expand(uint32_t w, uint32_t* out) {
 
 struct Q4Bars {
   uint64_t qfull[kQMax], qempty[kQMax];
-  uint64_t full[kSMax], free[kSMax];
-  uint64_t dfull[kDMax], dempty[kDMax];
+  uint64_t full[6], free[6];
+  uint64_t dfull[4], dempty[4];
   uint64_t sfull[kSSlots], sempty[kSSlots];
   uint64_t done;
   uint32_t tmem;
@@ -181,24 +175,40 @@ struct Ring {
   }
 };
 
-template <int N, int NDQ, int NEP>  // MMA N; expanding warps, epilogue warps (multiples of 4)
+// How a launch of N batch rows and groups of 2^GS lays out TMEM: accumulators
+// are handed over kSplit times a block, in kDBufs buffers of kDCols columns that
+// take at most half of it; the rest holds kSlots blocks of expanded codes (the
+// hidden states of as many lie in shared memory).
+template <int N, int GS>
+struct Q4Plan {
+  static constexpr int kSplit = N * (128 >> GS) <= 128 ? 1 : 2;
+  static constexpr int kNg = (128 >> GS) / kSplit;  // groups of a hand-over
+  static constexpr int kDCols = N * kNg;
+  static constexpr int kDBufs = 256 / kDCols < 4 ? 256 / kDCols : 4;
+  static constexpr int kRoom = (512 - kDBufs * kDCols) / kSlotCols;
+  static constexpr int kSlots = kRoom < 6 ? kRoom : 6;
+};
+
+template <int N, int GS, int NDQ, int NEP>  // expanding warps, epilogue warps (multiples of 4)
 __global__ void __launch_bounds__((4 + NDQ + NEP) * 32, 1)
     q4_mma_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmX,
                   const __grid_constant__ Q4Args a) {
   extern __shared__ uint8_t q4_smem_raw[];
   __shared__ Q4Bars bars;
   __shared__ unsigned long long best[N];
+  using P = Q4Plan<N, GS>;
+  constexpr int kSplit = P::kSplit, kNg = P::kNg, kDCols = P::kDCols, kDBufs = P::kDBufs, kSlots = P::kSlots;
   constexpr int NC = N / (NEP / 4);  // columns of an epilogue warp
   constexpr uint32_t kXBytes = N * 128;  // 64 hidden elements of N rows
   uint8_t* qring = q4_smem_raw + ((1024u - (smem_u32(q4_smem_raw) & 1023u)) & 1023u);
   uint8_t* xring = qring + a.qslots * kQTile;
-  uint8_t* sring = xring + a.slots * 2 * kXBytes;
+  uint8_t* sring = xring + kSlots * 2 * kXBytes;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < a.qslots; ++i) mbar_init(&bars.qfull[i], 1), mbar_init(&bars.qempty[i], 8);
-    for (int i = 0; i < a.slots; ++i) mbar_init(&bars.full[i], 4 + 1), mbar_init(&bars.free[i], 1);
-    for (int i = 0; i < a.dbufs; ++i) mbar_init(&bars.dfull[i], 1), mbar_init(&bars.dempty[i], NEP);
+    for (int i = 0; i < kSlots; ++i) mbar_init(&bars.full[i], 4 + 1), mbar_init(&bars.free[i], 1);
+    for (int i = 0; i < kDBufs; ++i) mbar_init(&bars.dfull[i], 1), mbar_init(&bars.dempty[i], NEP);
     for (int i = 0; i < kSSlots; ++i) mbar_init(&bars.sfull[i], 32), mbar_init(&bars.sempty[i], NEP);
     mbar_init(&bars.done, 1);
     fence_mbar_init();
@@ -213,10 +223,10 @@ __global__ void __launch_bounds__((4 + NDQ + NEP) * 32, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, bars.tmem, 0);
-  const uint32_t tmem_a = tmem + static_cast<uint32_t>(a.dbufs * a.dcols);  // expanded codes lie behind the accumulators
+  const uint32_t tmem_a = tmem + static_cast<uint32_t>(kDBufs * kDCols);  // expanded codes lie behind the accumulators
   const int qtiles = (a.kstages + 3) >> 2;  // copies of codes a tile
   const int blocks = (a.kstages + 1) >> 1;  // the last may be half a block
-  const int ngroups = a.H >> a.gshift;
+  const int ngroups = a.H >> GS;
   bool ok = true;
 
   if (warp == 0) {
@@ -261,11 +271,11 @@ __global__ void __launch_bounds__((4 + NDQ + NEP) * 32, 1)
           mbar_expect_tx(&bars.full[r.slot], two ? 2 * kXBytes : kXBytes);
           tma_load_2d(x, &tmX, kb * 128, 0, &bars.full[r.slot], pol);
           if (two) tma_load_2d(x + kXBytes, &tmX, kb * 128 + 64, 0, &bars.full[r.slot], pol);
-          r.next(a.slots);
+          r.next(kSlots);
         }
       }
-      for (int i = 0; i < a.slots; ++i) {
-        const uint32_t n = it / a.slots + (static_cast<uint32_t>(i) < it % a.slots ? 1u : 0u);
+      for (int i = 0; i < kSlots; ++i) {
+        const uint32_t n = it / kSlots + (static_cast<uint32_t>(i) < it % kSlots ? 1u : 0u);
         if (n > 0 && !q4_wait(&bars.full[i], (n - 1u) & 1u)) ok = false;
       }
     }
@@ -313,7 +323,7 @@ __global__ void __launch_bounds__((4 + NDQ + NEP) * 32, 1)
     // ---- MMA issuer: the warp goes through the blocks together, so that
     // addresses and descriptors stay uniform; one lane issues ----
     const uint32_t idesc = lm_idesc(N);
-    const int gs = a.gshift - 4;  // log2 of a group's steps (K = 16)
+    constexpr int gs = GS - 4;  // log2 of a group's steps (K = 16)
     const uint32_t x0 = smem_u32(xring);
     // four MMAs of a stage, `step` steps behind the hand-over's first
     const auto issue = [&](uint32_t d0, uint32_t at, uint64_t bd, int step) {
@@ -333,22 +343,22 @@ __global__ void __launch_bounds__((4 + NDQ + NEP) * 32, 1)
         tc_fence_after();
         const uint64_t bd = sw128_desc(x0 + r.slot * 2 * kXBytes);
         const uint32_t at = tmem_a + static_cast<uint32_t>(r.slot * kSlotCols);
-        const uint32_t d0 = tmem + static_cast<uint32_t>(rd.slot * a.dcols);
-        if (a.split == 1) {
+        const uint32_t d0 = tmem + static_cast<uint32_t>(rd.slot * kDCols);
+        if constexpr (kSplit == 1) {
           if (elect_one()) {
             issue(d0, at, bd, 0);
             if (nst == 2) issue(d0, at + 32u, bd + (kXBytes >> 4), 4);
             umma_commit(&bars.free[r.slot]);
             umma_commit(&bars.dfull[rd.slot]);
           }
-          rd.next(a.dbufs);
+          rd.next(kDBufs);
         } else {
           if (elect_one()) {
             issue(d0, at, bd, 0);
             umma_commit(&bars.dfull[rd.slot]);
             if (nst == 1) umma_commit(&bars.free[r.slot]);
           }
-          rd.next(a.dbufs);
+          rd.next(kDBufs);
           if (nst == 2) {
             if (!q4_wait(&bars.dempty[rd.slot], rd.par ^ 1u)) {
               ok = false;
@@ -356,15 +366,15 @@ __global__ void __launch_bounds__((4 + NDQ + NEP) * 32, 1)
             }
             tc_fence_after();
             if (elect_one()) {
-              issue(tmem + static_cast<uint32_t>(rd.slot * a.dcols), at + 32u, bd + (kXBytes >> 4), 0);
+              issue(tmem + static_cast<uint32_t>(rd.slot * kDCols), at + 32u, bd + (kXBytes >> 4), 0);
               umma_commit(&bars.dfull[rd.slot]);
               umma_commit(&bars.free[r.slot]);
             }
-            rd.next(a.dbufs);
+            rd.next(kDBufs);
           }
         }
         __syncwarp();
-        r.next(a.slots);
+        r.next(kSlots);
       }
     }
     // every MMA of this CTA completes before its TMEM is freed
@@ -381,7 +391,7 @@ __global__ void __launch_bounds__((4 + NDQ + NEP) * 32, 1)
     const int swz = row & 7;
     Ring rq, r;
     int tile = blockIdx.x, kb = (warp - 4) >> 2;
-    r.skip(kb, a.slots);
+    r.skip(kb, kSlots);
     rq.skip(kb >> 1, a.qslots);
     while (kb >= blocks) {  // (few blocks a tile)
       kb -= blocks;
@@ -424,7 +434,7 @@ __global__ void __launch_bounds__((4 + NDQ + NEP) * 32, 1)
         if ((kb & 1) == 0 && kb == blocks - 1) mbar_arrive1(&bars.qempty[rq.slot]);
       }
       // on to this warp's next block
-      r.skip(kTurns, a.slots);
+      r.skip(kTurns, kSlots);
       int copies = -(kb >> 1);
       kb += kTurns;
       while (kb >= blocks) {
@@ -439,50 +449,50 @@ __global__ void __launch_bounds__((4 + NDQ + NEP) * 32, 1)
     const int quad = warp & 3;
     const int col0 = ((warp - 4 - NDQ) >> 2) * NC;
     const int row = quad * 32 + lane;
+    const uint32_t from = tmem + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(col0);
     Ring rd, rs;
     for (int tile = blockIdx.x; tile < a.ntiles && ok; tile += gridDim.x) {
       float acc[NC];
 #pragma unroll
       for (int j = 0; j < NC; ++j) acc[j] = 0.0f;
-      uint4 sc = {0u, 0u, 0u, 0u};  // the scales of 8 groups
-      int g = 0;
-      const int unit = 2 / a.split;  // stages of a hand-over
-      for (int kb = 0; kb < a.kstages && ok; kb += unit) {
-        const int n_in = (min(unit, a.kstages - kb) * 64) >> a.gshift;
-        if (!q4_wait(&bars.dfull[rd.slot], rd.par)) {
+      for (int g0 = 0; g0 < ngroups && ok; g0 += 8) {  // a box of scales
+        if (!q4_wait(&bars.sfull[rs.slot], rs.par)) {
           ok = false;
           break;
         }
-        tc_fence_after();
-        for (int i = 0; i < n_in; ++i, ++g) {
-          if ((g & 7) == 0) {
-            if (!q4_wait(&bars.sfull[rs.slot], rs.par)) {
-              ok = false;
-              break;
-            }
-            sc = *reinterpret_cast<const uint4*>(sring + rs.slot * kSBox + row * 16);
-            __syncwarp();
-            if (lane == 0) mbar_arrive1(&bars.sempty[rs.slot]);
-            rs.next(kSSlots);
-          }
-          const uint32_t sw = (g & 6) == 0 ? sc.x : (g & 6) == 2 ? sc.y : (g & 6) == 4 ? sc.z : sc.w;
-          const float s = bf16_at(sw, g & 1);
-          const uint32_t at = tmem + (static_cast<uint32_t>(quad * 32) << 16) +
-                              static_cast<uint32_t>(rd.slot * a.dcols + i * N + col0);
-          // sixteen columns at a time: wider loads keep the MMAs from TMEM (128
-          // batch rows, H 4096, V 128256: 157 us, with 32 columns 200)
-#pragma unroll
-          for (int c = 0; c < NC; c += 16) {
-            uint32_t r[16];
-            tmem_ld16(at + static_cast<uint32_t>(c), r);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) acc[c + j] = fmaf(s, __uint_as_float(r[j]), acc[c + j]);
-          }
-        }
-        tc_fence_before();
+        const uint4 sc = *reinterpret_cast<const uint4*>(sring + rs.slot * kSBox + row * 16);
+        const uint32_t sw[4] = {sc.x, sc.y, sc.z, sc.w};
         __syncwarp();
-        if (lane == 0) mbar_arrive1(&bars.dempty[rd.slot]);
-        rd.next(a.dbufs);
+        if (lane == 0) mbar_arrive1(&bars.sempty[rs.slot]);
+        rs.next(kSSlots);
+#pragma unroll
+        for (int h0 = 0; h0 < 8; h0 += kNg) {  // a hand-over
+          if (g0 + h0 >= ngroups) break;
+          if (!q4_wait(&bars.dfull[rd.slot], rd.par)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t at = from + static_cast<uint32_t>(rd.slot * kDCols);
+#pragma unroll
+          for (int i = 0; i < kNg; ++i) {
+            if (i > 0 && g0 + h0 + i >= ngroups) break;  // half a block, the tile's last
+            const float s = bf16_at(sw[(h0 + i) >> 1], (h0 + i) & 1);
+            // sixteen columns at a time: wider loads keep the MMAs from TMEM (128
+            // batch rows, H 4096, V 128256: 157 us, with 32 columns 200)
+#pragma unroll
+            for (int c = 0; c < NC; c += 16) {
+              uint32_t r[16];
+              tmem_ld16(at + static_cast<uint32_t>(i * N + c), r);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) acc[c + j] = fmaf(s, __uint_as_float(r[j]), acc[c + j]);
+            }
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive1(&bars.dempty[rd.slot]);
+          rd.next(kDBufs);
+        }
       }
       if (!ok) break;
       const int64_t v = static_cast<int64_t>(tile) * kBM + row;
@@ -956,29 +966,32 @@ rl_status q4_check(rl_sampler* h, const uint16_t* hidden, int64_t ldh, const rl_
 }
 
 // A launch for at most N batch rows.
-template <int N, int NDQ, int NEP>
+template <int N, int GS, int NDQ, int NEP>
 cudaError_t q4_run(const CUtensorMap& mq, const CUtensorMap& mx, Q4Args a, int grid, cudaStream_t stream) {
-  const int xbytes = 2 * N * 128, group = 1 << a.gshift;
-  // accumulators take at most half of TMEM, in two buffers or more; the rest
-  // and 64 KB of hidden states (128 KB at the largest N) hold blocks in flight
-  a.split = group == 128 || N * (128 / group) <= 128 ? 1 : 2;
-  a.dcols = N * (128 / group) / a.split;
-  a.dbufs = 256 / a.dcols < kDMax ? 256 / a.dcols : kDMax;
-  a.slots = (512 - a.dbufs * a.dcols) / kSlotCols < kSMax ? (512 - a.dbufs * a.dcols) / kSlotCols : kSMax;
-  const int room = 224 * 1024 - 1024 - kSSlots * kSBox - a.slots * xbytes;
-  a.qslots = room / kQTile < kQMax ? room / kQTile : kQMax;
-  const size_t smem = 1024 + static_cast<size_t>(a.qslots) * kQTile + static_cast<size_t>(a.slots) * xbytes + kSSlots * kSBox;
+  constexpr int kFixed = 1024 + kSSlots * kSBox + Q4Plan<N, GS>::kSlots * 2 * N * 128;
+  constexpr int kRoom = (224 * 1024 - kFixed) / kQTile;
+  a.qslots = kRoom < kQMax ? kRoom : kQMax;
+  const size_t smem = kFixed + static_cast<size_t>(a.qslots) * kQTile;
   static std::atomic<int> configured[64];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev < 0 || dev >= 64 || !configured[dev].load(std::memory_order_acquire)) {
-    e = cudaFuncSetAttribute(q4_mma_kernel<N, NDQ, NEP>, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024);
+    e = cudaFuncSetAttribute(q4_mma_kernel<N, GS, NDQ, NEP>, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024);
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) configured[dev].store(1, std::memory_order_release);
   }
-  q4_mma_kernel<N, NDQ, NEP><<<grid, (4 + NDQ + NEP) * 32, smem, stream>>>(mq, mx, a);
+  q4_mma_kernel<N, GS, NDQ, NEP><<<grid, (4 + NDQ + NEP) * 32, smem, stream>>>(mq, mx, a);
   return cudaGetLastError();
+}
+template <int N, int NEP>
+cudaError_t q4_run(const CUtensorMap& mq, const CUtensorMap& mx, const Q4Args& a, int group, int grid, cudaStream_t stream) {
+  // groups of 32 go up to 64 batch rows a launch: two buffers of two groups
+  if constexpr (N <= 64)
+    if (group == 32) return q4_run<N, 5, 8, NEP>(mq, mx, a, grid, stream);
+  if (group == 64) return q4_run<N, 6, 8, NEP>(mq, mx, a, grid, stream);
+  if (group == 128) return q4_run<N, 7, 8, NEP>(mq, mx, a, grid, stream);
+  return cudaErrorInvalidValue;
 }
 
 template <int NT, int GS, int HB>
@@ -1071,7 +1084,6 @@ rl_status q4_launch(rl_sampler* h, const uint16_t* hidden, int64_t ldh, const rl
   Q4Args a = {};
   a.H = H;
   a.V = V;
-  a.gshift = w.group == 32 ? 5 : w.group == 64 ? 6 : 7;
   a.ntiles = (V + kBM - 1) / kBM;
   a.kstages = H / 64;
   a.scale = w.scale;
@@ -1097,11 +1109,11 @@ rl_status q4_launch(rl_sampler* h, const uint16_t* hidden, int64_t ldh, const rl
     CUtensorMap mx;
     if (!lm_tensor_map(&mx, hidden + static_cast<int64_t>(b0) * ldh, 2, H, Bc, ldh * 2, N))
       return set_error(RL_ERR_INVALID_ARG, "rl_lmhead_q4: hidden tensor map rejected (alignment or stride)");
-    cudaError_t e = N == 16   ? q4_run<16, 8, 4>(mq, mx, a, grid, stream)
-                    : N == 32 ? q4_run<32, 8, 8>(mq, mx, a, grid, stream)
-                    : N == 64 ? q4_run<64, 8, 8>(mq, mx, a, grid, stream)
-                    : N == 96 ? q4_run<96, 8, 8>(mq, mx, a, grid, stream)
-                              : q4_run<128, 8, 8>(mq, mx, a, grid, stream);
+    cudaError_t e = N == 16   ? q4_run<16, 4>(mq, mx, a, w.group, grid, stream)
+                    : N == 32 ? q4_run<32, 8>(mq, mx, a, w.group, grid, stream)
+                    : N == 64 ? q4_run<64, 8>(mq, mx, a, w.group, grid, stream)
+                    : N == 96 ? q4_run<96, 8>(mq, mx, a, w.group, grid, stream)
+                              : q4_run<128, 8>(mq, mx, a, w.group, grid, stream);
     if (e == cudaSuccess && out_tok)
       e = lm_argmax(h->lm_part, Bc, grid, h->lm_err, out_tok + b0, row_status ? row_status + b0 : nullptr, stream);
     if (e != cudaSuccess) return set_error(RL_ERR_CUDA, cudaGetErrorString(e));
