@@ -613,26 +613,33 @@ __device__ __forceinline__ void row_words(const uint8_t* row, int swz, int half,
   }
 }
 
-// The N scales of a box of one row, two to a word.
+// The N scales of a box of four rows, two to a word; sp[i] is row i's first
+// scale, at element offset g0 <= ngroups - 1.
 template <int N>
-__device__ __forceinline__ void box_scales(const uint16_t* row, int box, int ngroups, bool vec, uint32_t (&w)[(N + 1) / 2]) {
-  const int g0 = box * N;
-  if (vec && N > 1) {  // on 2 N bytes, whole boxes only
-    if constexpr (N == 2) {
-      w[0] = __ldg(reinterpret_cast<const uint32_t*>(row + g0));
-    } else if constexpr (N == 4) {
-      const uint2 c = __ldg(reinterpret_cast<const uint2*>(row + g0));
-      w[0] = c.x, w[1] = c.y;
-    } else if constexpr (N == 8) {
-      const uint4 c = __ldg(reinterpret_cast<const uint4*>(row + g0));
-      w[0] = c.x, w[1] = c.y, w[2] = c.z, w[3] = c.w;
+__device__ __forceinline__ void box_scales(const uint16_t* const (&sp)[4], int g0, int ngroups, bool vec,
+                                           uint32_t (&w)[4][(N + 1) / 2]) {
+  if (N > 1 && vec) {  // on 2 N bytes, whole boxes only
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (N == 2) {
+        w[i][0] = __ldg(reinterpret_cast<const uint32_t*>(sp[i] + g0));
+      } else if constexpr (N == 4) {
+        const uint2 c = __ldg(reinterpret_cast<const uint2*>(sp[i] + g0));
+        w[i][0] = c.x, w[i][1] = c.y;
+      } else if constexpr (N == 8) {
+        const uint4 c = __ldg(reinterpret_cast<const uint4*>(sp[i] + g0));
+        w[i][0] = c.x, w[i][1] = c.y, w[i][2] = c.z, w[i][3] = c.w;
+      }
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < (N + 1) / 2; ++i) {
-      const uint32_t lo = g0 + 2 * i < ngroups ? __ldg(row + g0 + 2 * i) : 0;
-      const uint32_t hi = N > 1 && g0 + 2 * i + 1 < ngroups ? __ldg(row + g0 + 2 * i + 1) : 0;
-      w[i] = lo | hi << 16;
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int k = 0; k < (N + 1) / 2; ++k) {
+        const uint32_t lo = g0 + 2 * k < ngroups ? __ldg(sp[i] + g0 + 2 * k) : 0;
+        const uint32_t hi = N > 1 && g0 + 2 * k + 1 < ngroups ? __ldg(sp[i] + g0 + 2 * k + 1) : 0;
+        w[i][k] = lo | hi << 16;
+      }
     }
   }
 }
@@ -717,6 +724,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1)
   const int ngroups = a.H >> GS;
   constexpr int kNs = (128 * HB) >> GS, kSw = (kNs + 1) / 2;  // scales of a box, in words
   const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  const bool vec = a.vec != 0;
   bool ok = true;
   Ring r;
   float acc[2][NT][4];
@@ -769,18 +777,14 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1)
 #pragma unroll
       for (int n = 0; n < NT; ++n) acc[m][n][0] = acc[m][n][1] = acc[m][n][2] = acc[m][n][3] = 0.0f;
     uint32_t ahead[4][kSw];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) box_scales<kNs>(sp[i], box0, ngroups, a.vec, ahead[i]);
+    box_scales<kNs>(sp, box0 * kNs, ngroups, vec, ahead);
     for (int box = box0; box < box1; ++box) {
       uint32_t sc[4][kSw];
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int k = 0; k < kSw; ++k) sc[i][k] = ahead[i][k];
-      if (box + 1 < box1) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) box_scales<kNs>(sp[i], box + 1, ngroups, a.vec, ahead[i]);
-      }
+      if (box + 1 < box1) box_scales<kNs>(sp, (box + 1) * kNs, ngroups, vec, ahead);
       if (!q4_wait(&full[warp][r.slot], r.par)) {
         ok = false;
         break;
@@ -1112,8 +1116,8 @@ rl_status q4_launch(rl_sampler* h, const uint16_t* hidden, int64_t ldh, const rl
     cudaError_t e = N == 16   ? q4_run<16, 4>(mq, mx, a, w.group, grid, stream)
                     : N == 32 ? q4_run<32, 8>(mq, mx, a, w.group, grid, stream)
                     : N == 64 ? q4_run<64, 8>(mq, mx, a, w.group, grid, stream)
-                    : N == 96 ? q4_run<96, 8>(mq, mx, a, w.group, grid, stream)
-                              : q4_run<128, 8>(mq, mx, a, w.group, grid, stream);
+                    : N == 96 ? q4_run<96, 12>(mq, mx, a, w.group, grid, stream)
+                              : q4_run<128, 16>(mq, mx, a, w.group, grid, stream);
     if (e == cudaSuccess && out_tok)
       e = lm_argmax(h->lm_part, Bc, grid, h->lm_err, out_tok + b0, row_status ? row_status + b0 : nullptr, stream);
     if (e != cudaSuccess) return set_error(RL_ERR_CUDA, cudaGetErrorString(e));
