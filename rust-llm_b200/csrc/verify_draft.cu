@@ -22,7 +22,7 @@
 // What bounds it is HBM for many rows and, for few, the dependent steps of the
 // walk. While the cluster joins its sums and decides, the rows of the node's
 // first child are fetched into L2; a pass then runs on L2, a warp's next chunk
-// loaded as soon as the registers of the last are free, 24 warps an SM.
+// loaded as soon as the registers of the last are free.
 //
 // Precision. A weight is 2^(x c - F): one FMA and ex2.approx, relative error
 // about 2^-22 with no bias that two ids would not share; c = log2(e) / T in
@@ -69,7 +69,7 @@ struct VdArgs {
   VdSide p, q;
   int has_q;
   int V, N;                // N: nodes of the widest sequence (outputs' row stride)
-  int part;                // ids of a warp's part (a multiple of 8)
+  int part;                // ids of a warp's part (whole chunks)
   const int32_t* tokens;   // node i's token and uniform at b * tok_stride + i - tok_off
   const float* accept_u;
   int tok_stride, tok_off;
@@ -365,30 +365,33 @@ __device__ __forceinline__ void join_parts(const Part* parts, int np, bool greed
   Q.s = sb;
 }
 
-// Loads the chunk of ids [c0, c0 + kChunk) cut at `end` into x: unit i of the
-// lane holds ids c0 + 128 i + 4 lane ... A row that does not start on a unit's
-// boundary is loaded id by id.
+// Loads the ids [c0, c0 + kChunk) into x: unit i of the lane holds ids c0 +
+// 128 i + 4 lane ... A row that does not start on a unit's boundary is loaded id
+// by id.
 template <bool Plain, typename T>
-__device__ __forceinline__ void chunk_load(const Row<T>& r, int c0, int end, float (&x)[4][4]) {
-  const int lane = threadIdx.x & 31;
-  const bool whole = end - c0 >= kChunk;
-  const T* at = r.x + c0 + 4 * lane;
+__device__ __forceinline__ void chunk_load(const Row<T>& r, int c0, float (&x)[4][4]) {
+  const T* at = r.x + c0 + 4 * (static_cast<int>(threadIdx.x) & 31);
   if (Plain || (reinterpret_cast<uintptr_t>(r.x) & (4 * sizeof(T) - 1)) == 0) {
-    if (whole) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) unit(at + 128 * i, x[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int j = c0 + 128 * i + 4 * lane;
-        x[i][0] = x[i][1] = x[i][2] = x[i][3] = RL_NEG_INF;
-        if (j + 4 <= end) unit(at + 128 * i, x[i]);
-        else if (j < end) unit_guarded(r.x, j, end, x[i]);
-      }
-    }
+    for (int i = 0; i < 4; ++i) unit(at + 128 * i, x[i]);
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) unit_guarded(r.x, c0 + 128 * i + 4 * lane, end, x[i]);
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[i][k] = to_f(__ldg(at + 128 * i + k));
+  }
+}
+// The same of a row's last ids, cut at `end`. Parts are whole chunks, so this
+// is one warp's; a function with an array of its own, which keeps its cases out
+// of the other warps' loops.
+template <typename T>
+__device__ __noinline__ void chunk_cut(const T* row, int c0, int end, float* x) {
+#pragma unroll 1
+  for (int i = 0; i < 4; ++i) {
+    float v[4];
+    unit_guarded(row, c0 + 128 * i + 4 * (static_cast<int>(threadIdx.x) & 31), end, v);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[4 * i + k] = v[k];
   }
 }
 template <bool Plain, typename T>
@@ -407,47 +410,76 @@ __device__ __forceinline__ void chunk_keep(const Row<T>& r, int c0, int end, flo
 // chunk, logits). The next chunk is loaded as soon as f is done with the last.
 template <bool Plain, typename T, typename F>
 __device__ __forceinline__ void pass(const Row<T>& r, int j0, int j1, F f) {
-  float x[4][4];
-  if (j0 < j1) chunk_load<Plain>(r, j0, j1, x);
-  for (int c0 = j0; c0 < j1; c0 += kChunk) {
-    chunk_keep<Plain>(r, c0, j1, x);
-    f(c0, x);
-    if (c0 + kChunk < j1) chunk_load<Plain>(r, c0 + kChunk, j1, x);
+  const int whole = j1 - (j1 - j0) % kChunk;
+  if (j0 < whole) {
+    float x[4][4];
+    chunk_load<Plain>(r, j0, x);
+    for (int c0 = j0; c0 < whole; c0 += kChunk) {
+      chunk_keep<Plain>(r, c0, j1, x);
+      f(c0, x);
+      if (c0 + kChunk < whole) chunk_load<Plain>(r, c0 + kChunk, x);
+    }
+  }
+  if (whole < j1) {
+    float t[4][4];
+    chunk_cut(r.x, whole, j1, &t[0][0]);
+    chunk_keep<Plain>(r, whole, j1, t);
+    f(whole, t);
   }
 }
 // f on the target's chunk, g on the draft's.
 template <bool Plain, typename TP, typename TQ, typename F, typename G>
 __device__ __forceinline__ void pass_two(const Row<TP>& rp, const Row<TQ>& rq, int j0, int j1, F f, G g) {
-  float x[4][4], y[4][4];
-  if (j0 < j1) {
-    chunk_load<Plain>(rp, j0, j1, x);
-    chunk_load<Plain>(rq, j0, j1, y);
+  const int whole = j1 - (j1 - j0) % kChunk;
+  if (j0 < whole) {
+    float x[4][4], y[4][4];
+    chunk_load<Plain>(rp, j0, x);
+    chunk_load<Plain>(rq, j0, y);
+    for (int c0 = j0; c0 < whole; c0 += kChunk) {
+      const bool more = c0 + kChunk < whole;
+      chunk_keep<Plain>(rp, c0, j1, x);
+      f(c0, x);
+      if (more) chunk_load<Plain>(rp, c0 + kChunk, x);
+      chunk_keep<Plain>(rq, c0, j1, y);
+      g(c0, y);
+      if (more) chunk_load<Plain>(rq, c0 + kChunk, y);
+    }
   }
-  for (int c0 = j0; c0 < j1; c0 += kChunk) {
-    chunk_keep<Plain>(rp, c0, j1, x);
-    f(c0, x);
-    if (c0 + kChunk < j1) chunk_load<Plain>(rp, c0 + kChunk, j1, x);
-    chunk_keep<Plain>(rq, c0, j1, y);
-    g(c0, y);
-    if (c0 + kChunk < j1) chunk_load<Plain>(rq, c0 + kChunk, j1, y);
+  if (whole < j1) {
+    float t[4][4];
+    chunk_cut(rp.x, whole, j1, &t[0][0]);
+    chunk_keep<Plain>(rp, whole, j1, t);
+    f(whole, t);
+    chunk_cut(rq.x, whole, j1, &t[0][0]);
+    chunk_keep<Plain>(rq, whole, j1, t);
+    g(whole, t);
   }
 }
 // f on both.
 template <bool Plain, typename TP, typename TQ, typename F>
 __device__ __forceinline__ void pass_both(const Row<TP>& rp, const Row<TQ>& rq, int j0, int j1, F f) {
-  float x[4][4], y[4][4];
-  if (j0 < j1) {
-    chunk_load<Plain>(rp, j0, j1, x);
-    chunk_load<Plain>(rq, j0, j1, y);
-  }
-  for (int c0 = j0; c0 < j1; c0 += kChunk) {
-    chunk_keep<Plain>(rp, c0, j1, x);
-    chunk_keep<Plain>(rq, c0, j1, y);
-    f(x, y);
-    if (c0 + kChunk < j1) {
-      chunk_load<Plain>(rp, c0 + kChunk, j1, x);
-      chunk_load<Plain>(rq, c0 + kChunk, j1, y);
+  const int whole = j1 - (j1 - j0) % kChunk;
+  if (j0 < whole) {
+    float x[4][4], y[4][4];
+    chunk_load<Plain>(rp, j0, x);
+    chunk_load<Plain>(rq, j0, y);
+    for (int c0 = j0; c0 < whole; c0 += kChunk) {
+      chunk_keep<Plain>(rp, c0, j1, x);
+      chunk_keep<Plain>(rq, c0, j1, y);
+      f(x, y);
+      if (c0 + kChunk < whole) {
+        chunk_load<Plain>(rp, c0 + kChunk, x);
+        chunk_load<Plain>(rq, c0 + kChunk, y);
+      }
     }
+  }
+  if (whole < j1) {
+    float t[4][4], u[4][4];
+    chunk_cut(rp.x, whole, j1, &t[0][0]);
+    chunk_cut(rq.x, whole, j1, &u[0][0]);
+    chunk_keep<Plain>(rp, whole, j1, t);
+    chunk_keep<Plain>(rq, whole, j1, u);
+    f(t, u);
   }
 }
 
@@ -497,6 +529,81 @@ __device__ __forceinline__ void find_owner(Ctl& sh, const double (&w)[kPerLane],
     sh.rest = t - before;
     sh.at = INT_MAX;
   }
+}
+
+// The passes are functions of their own: what the walk keeps stays out of their
+// registers, and a warp's loads in flight are what a pass lives on.
+template <bool Plain, typename T>
+__device__ __noinline__ Seen see_row(Row<T> r, int j0, int j1, float c, bool greedy) {
+  Seen z = unseen();
+  const int lane = threadIdx.x & 31;
+  if (greedy) pass<Plain>(r, j0, j1, [&](int c0, const float (&x)[4][4]) { see_max(z, x, c0 + 4 * lane); });
+  else pass<Plain>(r, j0, j1, [&](int, const float (&x)[4][4]) { see(z, x, c); });
+  return z;
+}
+struct Seen2 {
+  Seen p, q;
+};
+template <bool Plain, typename TP, typename TQ>
+__device__ __noinline__ Seen2 see_rows(Row<TP> rp, Row<TQ> rq, int j0, int j1, float cp, float cq) {
+  Seen zp = unseen(), zq = unseen();
+  pass_two<Plain>(rp, rq, j0, j1, [&](int, const float (&x)[4][4]) { see(zp, x, cp); },
+                  [&](int, const float (&y)[4][4]) { see(zq, y, cq); });
+  return {zp, zq};
+}
+// The frames and factors of w = max(p rho - q, 0).
+struct Resid {
+  float cp, cq, Pm, Qm, Fp, Fq, rhi, rlo;
+};
+// A lane's sum of w over its part.
+template <bool Plain, typename TP, typename TQ>
+__device__ __noinline__ double sum_resid(Row<TP> rp, Row<TQ> rq, int j0, int j1, Resid f) {
+  double s = 0.0;
+  pass_both<Plain>(rp, rq, j0, j1, [&](const float (&x)[4][4], const float (&y)[4][4]) {
+    float w = 0.0f;
+    if (fabsf(f.Fp) < RL_POS_INF && fabsf(f.Fq) < RL_POS_INF) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float ep = weight(x[i][k], f.cp, f.Fp), eq = weight(y[i][k], f.cq, f.Fq);
+          v[k] = fmaxf(__fmaf_rn(ep, f.rhi, __fmaf_rn(ep, f.rlo, -eq)), 0.0f);
+        }
+        w += (v[0] + v[1]) + (v[2] + v[3]);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        const float ep = weight(x[k >> 2][k & 3], f.Pm, f.cp, f.Fp), eq = weight(y[k >> 2][k & 3], f.Qm, f.cq, f.Fq);
+        w += fmaxf(__fmaf_rn(ep, f.rhi, __fmaf_rn(ep, f.rlo, -eq)), 0.0f);
+      }
+    }
+    s += static_cast<double>(w);
+  });
+  return s;
+}
+// A lane's sum of p over its part without the refused given tokens.
+template <bool Plain, typename T>
+__device__ __noinline__ double sum_kept(Row<T> r, int j0, int j1, float c, float m, float F, const Ctl* sh, const Node* nodes,
+                                        int nrem) {
+  double s = 0.0;
+  const int lane = threadIdx.x & 31;
+  pass<Plain>(r, j0, j1, [&](int c0, float (&x)[4][4]) {
+    for (int k = 0; k < nrem; ++k) {
+      const int t = nodes[sh->removed[k]].tok - c0;  // its lane takes it out
+      if (t >= 0 && t < kChunk && ((t >> 2) & 31) == lane) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (i == ((t >> 7) << 2 | (t & 3))) x[i >> 2][i & 3] = RL_NEG_INF;
+      }
+    }
+    float w = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w += weight(x[i >> 2][i & 3], m, c, F);
+    s += static_cast<double>(w);
+  });
+  return s;
 }
 
 template <typename T>
@@ -629,13 +736,13 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
     if (Plain || (no_mask & 2)) rq.mask = nullptr;
     if (Plain) rp.cut = rq.cut = -1;
     // ---- this warp's sums of both rows, into every CTA of the cluster ----
-    Seen zp = unseen(), zq = unseen();
-    const auto see_p = [&](int c0, const float (&x)[4][4]) {
-      if (greedy) see_max(zp, x, c0 + 4 * lane);
-      else see(zp, x, cp);
-    };
-    if (with_q) pass_two<Plain>(rp, rq, j0, j1, see_p, [&](int, const float (&y)[4][4]) { see(zq, y, cq); });
-    else pass<Plain>(rp, j0, j1, see_p);
+    Seen zp, zq = unseen();
+    if (with_q) {
+      const Seen2 z = see_rows<Plain>(rp, rq, j0, j1, cp, cq);
+      zp = z.p, zq = z.q;
+    } else {
+      zp = see_row<Plain>(rp, j0, j1, cp, greedy);
+    }
     if (firstc != INT_MAX && (drawn || greedy)) {  // likely to be accepted
       fetch(px0 + firstc * a.p.ld, j0, j1);
       if (drawn && nodes[firstc].first != INT_MAX) fetch(qx0 + firstc * a.q.ld, j0, j1);
@@ -754,29 +861,7 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
       rhi = static_cast<float>(rho);
       rlo = static_cast<float>(rho - static_cast<double>(rhi));
       const float Pm = sh.Pm, Qm = sh.Qm, Fp = frame(Pm, cp), Fq = frame(Qm, cq);
-      double s = 0.0;
-      pass_both<Plain>(rp, rq, j0, j1, [&](const float (&x)[4][4], const float (&y)[4][4]) {
-        float w = 0.0f;
-        if (fabsf(Fp) < RL_POS_INF && fabsf(Fq) < RL_POS_INF) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float v[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float ep = weight(x[i][k], cp, Fp), eq = weight(y[i][k], cq, Fq);
-              v[k] = fmaxf(__fmaf_rn(ep, rhi, __fmaf_rn(ep, rlo, -eq)), 0.0f);
-            }
-            w += (v[0] + v[1]) + (v[2] + v[3]);
-          }
-        } else {
-#pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            const float ep = weight(x[k >> 2][k & 3], Pm, cp, Fp), eq = weight(y[k >> 2][k & 3], Qm, cq, Fq);
-            w += fmaxf(__fmaf_rn(ep, rhi, __fmaf_rn(ep, rlo, -eq)), 0.0f);
-          }
-        }
-        s += static_cast<double>(w);
-      });
+      double s = sum_resid<Plain>(rp, rq, j0, j1, Resid{cp, cq, Pm, Qm, Fp, Fq, rhi, rlo});
       s = warp_sum_d(s);
       if (lane < C) (C > 1 ? cl.map_shared_rank(&sh.w[par][0], lane) : &sh.w[par][0])[mypart] = s;
       if (C > 1) cl.sync();
@@ -859,21 +944,7 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
         again |= t >= j0 && t < j1;
       }
       if (again) {
-        double s = 0.0;
-        pass<Plain>(rp, j0, j1, [&](int c0, float (&x)[4][4]) {
-          for (int k = 0; k < nrem; ++k) {
-            const int t = nodes[sh.removed[k]].tok - c0;  // its lane takes it out
-            if (t >= 0 && t < kChunk && ((t >> 2) & 31) == lane) {
-#pragma unroll
-              for (int i = 0; i < 16; ++i)
-                if (i == ((t >> 7) << 2 | (t & 3))) x[i >> 2][i & 3] = RL_NEG_INF;
-            }
-          }
-          float w = 0.0f;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) w += weight(x[i >> 2][i & 3], Pm, cp, Fp);
-          s += static_cast<double>(w);
-        });
+        const double s = sum_kept<Plain>(rp, j0, j1, cp, Pm, Fp, &sh, nodes, nrem);
         f = warp_sum_d(s);
       }
       if (lane < C) (C > 1 ? cl.map_shared_rank(&sh.w[par][0], lane) : &sh.w[par][0])[mypart] = f;
@@ -1043,9 +1114,10 @@ rl_status side_of(const rl_dist_rows* d, int V, int per_seq, VdSide* s) {
 // CTAs of a sequence's cluster. A walk's steps follow one another and only its
 // rows can be split: eight where they find room on the GPU at once (two CTAs an
 // SM), four where there are sequences enough, and at least 2048 ids a CTA,
-// below which the join costs more than it saves. us a call at 2 / 4 / 8 / 16
-// CTAs: 64 x 4 x 128256 f32 115 / 81 / 94 / 142, 16 trees of 29 nodes x 128256
-// 86 / 53 / 39 / 41, one chain of 3 x 32000 18.0 / 14.2 / 13.0 / 14.1.
+// below which the join costs more than it saves. us a call at 2 / 4 / 8 CTAs:
+// 64 x 4 x 128256 f32 100 / 72 / 80, 128 x 7 x 151936 bf16 180 / 116 / 123, 16
+// trees of 29 nodes x 128256 70 / 43 / 32, one chain of 3 x 32000 15.9 / 12.3 /
+// 12.3 (an earlier form at 16 CTAs: 142 where 4 took 81).
 int cluster_size(int B, int V) {
   int C = 1;
   while (C < kMaxCluster && (C < 4 || static_cast<int64_t>(B) * C * 2 <= 256) && V / (2 * C) >= 2048) C *= 2;
@@ -1071,8 +1143,9 @@ rl_status verify(rl_sampler* h, int B, int V, VdArgs& a, const rl_dist_rows* tar
   VdGuard g(h->device);
   if (!g.ok) return set_error(RL_ERR_CUDA, "rl_specdec_verify: cudaSetDevice failed");
   const int C = cluster_size(B, V);
-  // parts in whole groups of eight ids: they start on 16-byte boundaries
-  a.part = static_cast<int>(((static_cast<int64_t>(V) + C * kVW - 1) / (C * kVW) + 7) & ~int64_t(7));
+  // parts of whole chunks, so that only the row's end is cut
+  const int64_t even = (static_cast<int64_t>(V) + C * kVW - 1) / (C * kVW);
+  a.part = static_cast<int>((even + kChunk - 1) / kChunk * kChunk);
   const bool plain = is_plain(target) && (!draft || is_plain(draft));
   using bf = __nv_bfloat16;
   const cudaError_t e = pb ? (qb ? launch<bf, bf>(a, B, C, plain, stream) : launch<bf, float>(a, B, C, plain, stream))

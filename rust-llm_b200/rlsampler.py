@@ -229,12 +229,16 @@ def _stream(stream):
 
 
 def _raw_stream(stream, device):
-    """The stream's handle: the device's current stream where none is given."""
-    if stream is None:
-        import torch
+    """The stream's handle: the device's current stream where none is given
+    (asked of torch without making a Stream object, where it can be)."""
+    if stream is not None:
+        return stream.cuda_stream
+    import torch
 
-        stream = torch.cuda.current_stream(device)
-    return stream.cuda_stream
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    if raw is not None and device.index is not None:
+        return raw(device.index)
+    return torch.cuda.current_stream(device).cuda_stream
 
 
 class DistRows:
