@@ -302,8 +302,8 @@ rl_status rl_specdec_verify(rl_sampler* h, const float* logits, int B, int V, in
  *   first_row[B]    the sequence's first row (NULL: sequences follow one
  *                   another at the widest number of rows); `rows` is the
  *                   number of rows that may be read.
- * -inf logits have probability 0. Weights below 2^-126 of the row's largest
- * count as 0. 1e-30 and 3e38 bound 1 / T.
+ * -inf logits have probability 0. Weights below 2^-125 of the row's largest may
+ * count as 0. 1e-30 and 3e38 bound log2(e) / T.
  *
  * rl_specdec_verify_draft -- a chain. Sequence b has n_draft[b] in [0,
  * max_draft] drafts drafts[b, i], target rows first_row + 0 .. n_draft and
@@ -341,8 +341,9 @@ rl_status rl_specdec_verify(rl_sampler* h, const float* logits, int B, int V, in
  *                   a non-finite T; RL_ERR_INVALID_ARG for a count or a row
  *                   outside its range. Such a sequence gets out_accepted -1,
  *                   tokens and nodes -1 and probabilities 0.
- * Rows behind the last accepted node are not read. No workspace: calls may
- * overlap on one handle, and may be captured.
+ * What stands in rows behind the last accepted node has no effect (a part of
+ * them may be brought into cache). No workspace: calls may overlap on one handle,
+ * and may be captured.
  */
 typedef struct {
   const void* logits;
@@ -462,7 +463,8 @@ rl_status rl_lmhead_sample(rl_sampler* h, const uint16_t* hidden, int64_t ldh, c
  *   scale  bf16 [V, lds], lds >= H / group
  *   group  32, 64 or 128; H a multiple of group and of 64
  * Products are exact in f32 and sums are f32; a group's sum is multiplied by
- * its scale in f32.
+ * its scale in f32 (scales of magnitudes up to 2^90). Up to 16 batch rows, hidden
+ * elements below 2^-27 of their row's largest are rounded to 2^-35 of it.
  *
  * rl_lmhead_q4_quantize: such a weight from the bf16 one that rl_lmhead_*
  *   takes (read once, laid out once): per group scale = -m / 8 for the element
@@ -470,7 +472,9 @@ rl_status rl_lmhead_sample(rl_sampler* h, const uint16_t* hidden, int64_t ldh, c
  *   round-half-even(w / scale) + 8 clamped to 0 .. 15; an all-zero group has
  *   scale 0 and codes 8. A group that holds NaN or an infinity gets a NaN scale.
  * rl_lmhead_q4_logits / _greedy / _sample: rl_lmhead_logits / _greedy /
- *   _sample on it (same outputs, same limits on hidden and B).
+ *   _sample on it (same outputs, same limits on hidden and B). _greedy and
+ *   _sample use buffers of the handle: one call at a time per handle, as for
+ *   rl_lmhead_greedy and _sample.
  */
 typedef struct {
   const uint8_t* q;

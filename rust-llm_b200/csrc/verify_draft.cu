@@ -131,11 +131,13 @@ __device__ __forceinline__ float weight_2(float x, float m, float c, float F) {
   return ex2(t) * ex2(__fadd_rn(e, f));
 }
 // What a sum relative to frame F (of logit m) is multiplied by to be relative
-// to frame G (of logit M >= m); more than 126 binades apart it drops out.
-__device__ __forceinline__ float rebase(float m, float F, float M, float G) {
+// to frame G (of logit M >= m); more than 125 binades apart it drops out. What
+// stays holds an id, m's, whose own weight in G's frame is not 0, so that a draw
+// that falls in it finds an id.
+__device__ __forceinline__ float rebase(float m, float F, float M, float G, float c) {
   if (m == M) return 1.0f;
   const float t = F - G;
-  return t >= -126.0f ? ex2(t) : 0.0f;
+  return fminf(t, __fmaf_rn(m, c, -G)) >= -125.0f ? ex2(t) : 0.0f;
 }
 
 // A row of logits with what decides which of its ids are kept.
@@ -274,7 +276,7 @@ __device__ __forceinline__ void see(Seen& z, const float (&x)[4][4], float c) {
     if (gm != gm) z.s = __longlong_as_double(0x7ff8000000000000LL);
     if (gm > z.m) {
       const float F = frame(gm, c);
-      if (z.m > RL_NEG_INF) z.s *= static_cast<double>(rebase(z.m, z.F, gm, F));
+      if (z.m > RL_NEG_INF) z.s *= static_cast<double>(rebase(z.m, z.F, gm, F, c));
       z.m = gm;
       z.F = F;
     }
@@ -301,8 +303,8 @@ __device__ __forceinline__ void warp_parts(const Seen& a, float ca, const Seen& 
   pb.m = warp_fmax(b.m);
   pa.id = static_cast<int>(__reduce_min_sync(0xffffffffu, static_cast<unsigned>(a.m == pa.m ? a.id : INT_MAX)));
   pb.id = 0;
-  const float fa = greedy ? 1.0f : a.m > RL_NEG_INF ? rebase(a.m, a.F, pa.m, frame(pa.m, ca)) : 0.0f;
-  const float fb = b.m > RL_NEG_INF ? rebase(b.m, b.F, pb.m, frame(pb.m, cb)) : 0.0f;
+  const float fa = greedy ? 1.0f : a.m > RL_NEG_INF ? rebase(a.m, a.F, pa.m, frame(pa.m, ca), ca) : 0.0f;
+  const float fb = b.m > RL_NEG_INF ? rebase(b.m, b.F, pb.m, frame(pb.m, cb), cb) : 0.0f;
   double sa = a.s == a.s ? a.s * static_cast<double>(fa) : a.s;
   double sb = b.s == b.s ? b.s * static_cast<double>(fb) : b.s;
 #pragma unroll
@@ -347,8 +349,8 @@ __device__ __forceinline__ void join_parts(const Part* parts, int np, bool greed
   for (int k = 0; k < kPerLane; ++k) {
     if (k >= per) continue;
     if (a[k].m == P.m) id = min(id, static_cast<unsigned>(a[k].id));
-    const float fa = greedy ? 1.0f : a[k].m > RL_NEG_INF ? rebase(a[k].m, frame(a[k].m, cp), P.m, Ga) : 0.0f;
-    const float fb = b[k].m > RL_NEG_INF ? rebase(b[k].m, frame(b[k].m, cq), Q.m, Gb) : 0.0f;
+    const float fa = greedy ? 1.0f : a[k].m > RL_NEG_INF ? rebase(a[k].m, frame(a[k].m, cp), P.m, Ga, cp) : 0.0f;
+    const float fb = b[k].m > RL_NEG_INF ? rebase(b[k].m, frame(b[k].m, cq), Q.m, Gb, cq) : 0.0f;
     w[k] = a[k].s == a[k].s ? a[k].s * static_cast<double>(fa) : a[k].s;
     sa += w[k];
     sb += b[k].s == b[k].s ? b[k].s * static_cast<double>(fb) : b[k].s;
@@ -937,7 +939,7 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
       // the parts that hold refused given tokens sum again (taking a weight
       // off a sum would leave its rounding)
       const Part me = sh.part[par ^ 1][0][mypart];
-      double f = me.m > RL_NEG_INF ? me.s * static_cast<double>(rebase(me.m, frame(me.m, cp), Pm, Fp)) : 0.0;
+      double f = me.m > RL_NEG_INF ? me.s * static_cast<double>(rebase(me.m, frame(me.m, cp), Pm, Fp, cp)) : 0.0;
       bool again = false;
       for (int k = 0; k < nrem; ++k) {
         const int t = nodes[sh.removed[k]].tok;

@@ -466,3 +466,34 @@ def test_cutoffs_from_the_sampler(smp):
     assert np.array_equal(got[1].cpu().numpy(), want[2])
     c.check(want)
     s.close()
+
+
+@pytest.mark.parametrize("pad,first", [("given", 600), ("drawn", 600), ("given", 5000), ("drawn", 5000)])
+def test_first_ids_at_the_edge_of_the_weights(smp, pad, first):
+    """A draw with u = 0 where the row's first ids weigh about 2^-126 of its
+    largest, in steps around that: whatever counts there, the token is an id of
+    the row and none before it has any weight by its own."""
+    B, V = 400, 20000
+    rng = np.random.default_rng(40)
+    m = rng.choice([0.0, 3.3, -7.1, 400.7, -9000.3], B)
+    x = np.full((B, V), -np.inf, np.float32)
+    x[:, V - 5] = m
+    gap = (126.0 + np.linspace(-1.5, 1.5, B)) * np.log(2.0)
+    x[:, :first] = (x[:, V - 5].astype(np.float64) - gap)[:, None]
+    rows = torch.from_numpy(x).to(DEV)
+    zero = torch.zeros(B, device=DEV)
+    n = torch.zeros(B, dtype=torch.int32, device=DEV)
+    none = torch.empty(B, 0, dtype=torch.int32, device=DEV)
+    kw = {}
+    if pad == "drawn":  # one draft that the target refuses: the token comes from max(p - q, 0)
+        n += 1
+        none = torch.full((B, 1), V - 3, dtype=torch.int32, device=DEV)
+        q = torch.full((B, V), -np.inf, device=DEV)
+        q[:, V - 3] = 1.0
+        kw["draft"] = rlsampler.DistRows(q)
+        rows = rows.repeat_interleave(2, 0).contiguous()
+    acc, tok, prob, st = smp.specdec_verify_draft(rlsampler.DistRows(rows), none, n, torch.zeros(none.shape, device=DEV), zero, **kw)
+    tok = tok[:, 0].cpu().numpy()
+    assert (st == 0).all() and (acc == 0).all()
+    assert np.isin(tok, [0, V - 5]).all(), tok[~np.isin(tok, [0, V - 5])]
+    assert (tok[gap < 124.5 * np.log(2.0)] == 0).all()
