@@ -145,6 +145,9 @@ __device__ __forceinline__ bool q4_wait(uint64_t* bar, uint32_t parity) {
     if (clock64() - t0 > kWaitBudget) return false;
   }
 }
+// The outcome of a converged warp's waits, alike for its lanes: one whose wait
+// runs out leaves no others behind at an instruction of the whole warp.
+__device__ __forceinline__ bool all_ok(bool ok) { return __all_sync(0xffffffffu, ok) != 0; }
 // One lane of a converged warp.
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;
@@ -284,7 +287,7 @@ __global__ void __launch_bounds__((4 + NDQ + NEP) * 32, 1)
     Ring r;
     for (int tile = blockIdx.x; tile < a.ntiles && ok; tile += gridDim.x) {
       for (int g0 = 0; g0 < ngroups && ok; g0 += 8) {
-        if (!q4_wait(&bars.sempty[r.slot], r.par ^ 1u)) {
+        if (!all_ok(q4_wait(&bars.sempty[r.slot], r.par ^ 1u))) {
           ok = false;
           break;
         }
@@ -336,7 +339,7 @@ __global__ void __launch_bounds__((4 + NDQ + NEP) * 32, 1)
     for (int tile = blockIdx.x; tile < a.ntiles && ok; tile += gridDim.x) {
       for (int kb = 0; kb < blocks && ok; ++kb) {
         const int nst = min(2, a.kstages - 2 * kb);
-        if (!q4_wait(&bars.full[r.slot], r.par) || !q4_wait(&bars.dempty[rd.slot], rd.par ^ 1u)) {
+        if (!all_ok(q4_wait(&bars.full[r.slot], r.par) && q4_wait(&bars.dempty[rd.slot], rd.par ^ 1u))) {
           ok = false;
           break;
         }
@@ -360,7 +363,7 @@ __global__ void __launch_bounds__((4 + NDQ + NEP) * 32, 1)
           }
           rd.next(kDBufs);
           if (nst == 2) {
-            if (!q4_wait(&bars.dempty[rd.slot], rd.par ^ 1u)) {
+            if (!all_ok(q4_wait(&bars.dempty[rd.slot], rd.par ^ 1u))) {
               ok = false;
               break;
             }
@@ -381,6 +384,7 @@ __global__ void __launch_bounds__((4 + NDQ + NEP) * 32, 1)
     if (elect_one()) umma_commit(&bars.done);
     __syncwarp();
     if (!q4_wait(&bars.done, 0u)) ok = false;
+    __syncwarp();
   } else if (warp < 4 + NDQ) {
     // ---- codes into bf16: every so many blocks of this warp's 32 rows ----
     constexpr int kTurns = NDQ / 4;
@@ -402,7 +406,7 @@ __global__ void __launch_bounds__((4 + NDQ + NEP) * 32, 1)
       rq.skip(((tile - static_cast<int>(blockIdx.x)) / static_cast<int>(gridDim.x)) * qtiles + (kb >> 1), a.qslots);
     }
     while (tile < a.ntiles && ok) {
-      if (!q4_wait(&bars.qfull[rq.slot], rq.par) || !q4_wait(&bars.free[r.slot], r.par ^ 1u)) {
+      if (!all_ok(q4_wait(&bars.qfull[rq.slot], rq.par) && q4_wait(&bars.free[r.slot], r.par ^ 1u))) {
         ok = false;
         break;
       }
@@ -456,10 +460,7 @@ __global__ void __launch_bounds__((4 + NDQ + NEP) * 32, 1)
 #pragma unroll
       for (int j = 0; j < NC; ++j) acc[j] = 0.0f;
       for (int g0 = 0; g0 < ngroups && ok; g0 += 8) {  // a box of scales
-        if (!q4_wait(&bars.sfull[rs.slot], rs.par)) {
-          ok = false;
-          break;
-        }
+        const bool in = q4_wait(&bars.sfull[rs.slot], rs.par);
         const uint4 sc = *reinterpret_cast<const uint4*>(sring + rs.slot * kSBox + row * 16);
         const uint32_t sw[4] = {sc.x, sc.y, sc.z, sc.w};
         __syncwarp();
@@ -468,7 +469,7 @@ __global__ void __launch_bounds__((4 + NDQ + NEP) * 32, 1)
 #pragma unroll
         for (int h0 = 0; h0 < 8; h0 += kNg) {  // a hand-over
           if (g0 + h0 >= ngroups) break;
-          if (!q4_wait(&bars.dfull[rd.slot], rd.par)) {
+          if (!all_ok(in && q4_wait(&bars.dfull[rd.slot], rd.par))) {
             ok = false;
             break;
           }
@@ -544,7 +545,6 @@ struct FewArgs {
   const uint16_t* hidden;
   int64_t ldh;
   int B, H, V;
-  int gshift;
   int ntiles, boxes;  // 32-row tiles; copies (boxes) a tile
   int slots;
   const uint16_t* scale;
@@ -757,10 +757,9 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1)
       }
     }
   };
-  // where a tile's sums lie that this warp has a part of: 0 the end of a tile
-  // that began before u0, 1 the beginning of one that ends behind u1
-  float* parts = reinterpret_cast<float*>(ring);  // [2][2 * NT * 4][32], in the ring once it is read
-  int kept = 0;
+  // the sums of the end of a tile that began before u0, in the ring once it is read
+  float* parts = reinterpret_cast<float*>(ring);  // [2 * NT * 4][32]
+  int kept = 0;  // 1: `first` holds those; 2: acc holds a tile that ends behind u1
   float first[2][NT][4];
   int u = u0;
   while (u < u1 && ok) {
@@ -785,7 +784,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1)
 #pragma unroll
         for (int k = 0; k < kSw; ++k) sc[i][k] = ahead[i][k];
       if (box + 1 < box1) box_scales<kNs>(sp, (box + 1) * kNs, ngroups, vec, ahead);
-      if (!q4_wait(&full[warp][r.slot], r.par)) {
+      if (!all_ok(q4_wait(&full[warp][r.slot], r.par))) {
         ok = false;
         break;
       }
@@ -1020,8 +1019,10 @@ cudaError_t few_run(const CUtensorMap& mq, const FewArgs& a, int group, size_t s
                        : few_run<NT, 7, HB>(mq, a, smem, grid, stream);
 }
 
-// Whether the hidden states fit shared memory beside the rings (H <= 8192 at
-// 8 batch rows, 4096 at 16).
+// Up to 16 batch rows, where the hidden states fit shared memory beside the rings
+// (H <= 8192 at 8 batch rows, 4096 at 16). us a call, few rows' kernel / the
+// tensor cores' roles: 1 x 4096 x 128256 64 / 103, 12 rows of it 102 / 113, 1 x
+// 2048 x 32000 15 / 19; behind 16 rows it would load each code again for every 16.
 size_t few_hidden(int B, int H) { return static_cast<size_t>(B <= 8 ? 8 : 16) * ((H + 255) / 256) * 512; }
 bool is_few(int B, int H) { return B <= 16 && few_hidden(B, H) <= kFewHidden; }
 
@@ -1040,7 +1041,6 @@ rl_status few_launch(rl_sampler* h, const uint16_t* hidden, int64_t ldh, const r
   a.B = B;
   a.H = H;
   a.V = V;
-  a.gshift = w.group == 32 ? 5 : w.group == 64 ? 6 : 7;
   a.ntiles = (V + kFewRows - 1) / kFewRows;
   a.boxes = (H + 128 * hb - 1) / (128 * hb);
   a.scale = w.scale;

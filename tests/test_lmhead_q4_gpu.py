@@ -266,3 +266,39 @@ def test_argument_errors(smp):
         smp.lmhead_q4_sample(torch.empty(1, 64, dtype=torch.bfloat16, device="cuda"), big, torch.zeros(24, dtype=torch.uint8, device="cuda"),
                              torch.zeros(1, device="cuda"))
     assert e.value.status == rlsampler.RL_ERR_SHAPE
+
+
+@pytest.mark.parametrize("B", [3, 40])
+def test_offsets_past_32_bits(smp, B):
+    """Codes and scales of the last rows lie beyond 2^32 bytes; logits too."""
+    H, V, G = 256, 70, 64
+    hidden, codes, w = make(B, H, V, G, 41)
+    ldq, lds = 1 << 26, (1 << 25) + 8
+    q = torch.empty(V * ldq, dtype=torch.uint8, device="cuda").as_strided((V, H // 2), (ldq, 1))
+    s = torch.empty(V * lds, dtype=torch.bfloat16, device="cuda").as_strided((V, H // G), (lds, 1))
+    q.copy_(w.q)
+    s.copy_(w.scale)
+    want = smp.lmhead_q4_logits(hidden, w)
+    got = smp.lmhead_q4_logits(hidden, rlsampler.Q4Weight(q, s, G))
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+    del q, s
+    ldo = (1 << 30) + 1 if B < 8 else 1 << 27
+    out = torch.empty(B * ldo, dtype=torch.float32, device="cuda").as_strided((B, V), (ldo, 1))
+    smp.lmhead_q4_logits(hidden, w, out=out)
+    assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("B", [4, 30])
+@pytest.mark.parametrize("H,G", [(256, 32), (512, 64), (1024, 128), (256, 128)])
+@pytest.mark.parametrize("lead,pad", [(0, 0), (1, 0), (2, 2), (4, 4), (0, 1), (8, 8)])
+def test_scales_on_any_boundary(smp, B, H, G, lead, pad):
+    """Scales that start at any element and at any row stride."""
+    V = 333
+    hidden, codes, w = make(B, H, V, G, 42)
+    n = H // G
+    buf = torch.full((lead + V * (n + pad),), float("nan"), dtype=torch.bfloat16, device="cuda")
+    s = buf[lead:].as_strided((V, n), (n + pad, 1), lead)
+    s.copy_(w.scale)
+    got = smp.lmhead_q4_logits(hidden, rlsampler.Q4Weight(w.q, s, G))
+    assert torch.equal(got, smp.lmhead_q4_logits(hidden, w))
