@@ -14,6 +14,11 @@ device (one row per live sequence, in the order `live()` returns):
   semantics "spec": rl_sample_batch with each sequence's optional top_k and
       penalties over its last HISTORY tokens (the batched pipeline).
 
+SpeculativeStep is the sampling part of SpeculativeDecoder::generate
+(src/inference.rs:260-333) for a batch of sequences, with the drafts verified
+against both models' distributions (rl_specdec_verify_draft) in place of the
+reference's comparison of the target's probability with itself.
+
 SequenceState mirrors src/inference.rs:31-40 and carries the optional
 sampler fields the batched path adds (all off by default).
 """
@@ -134,6 +139,85 @@ class BatchStep:
         if not act:
             return {}
         return apply(act, self.sample(act, logits, uniforms))
+
+    def close(self):
+        self.sampler.close()
+
+
+def apply_tokens(states, tokens) -> dict:
+    """apply() for several tokens a sequence (rows of a [B, n] array, -1 behind a
+    row's last): a sequence takes its tokens until it is finished. Returns
+    {seq_id: [tokens taken]}."""
+    out = {}
+    for s, row in zip(states, tokens):
+        taken = out.setdefault(s.seq_id, [])
+        for t in row:
+            if t < 0 or not s.live():
+                break
+            apply([s], [t])
+            taken.append(int(t))
+    return out
+
+
+class SpeculativeStep:
+    """Draft and verify for the live sequences of a batch: `draft` draws one
+    token a sequence from the draft model's logits (called once for each
+    position of the drafts), `verify` checks the drafts against the target's
+    logits and gives each sequence its accepted drafts and one more token,
+    distributed as the target's own samples are. Both models sample at the
+    sequences' temperatures (top-p and penalties are not applied here: verify
+    takes whole distributions)."""
+
+    def __init__(self, vocab: int, max_batch: int, max_draft: int, device: int = 0, uniform=None):
+        if max_draft < 1 or max_draft + 1 > rlsampler.VERIFY_MAX_NODES:
+            raise ValueError(f"max_draft {max_draft}")
+        self.V, self.K, self.device = vocab, max_draft, device
+        self.sampler = rlsampler.Sampler(device, max_batch=max_batch, max_vocab=vocab, max_history=1)
+        rng = np.random.Generator(np.random.PCG64())
+        self.uniform = uniform or (lambda n: (rng.random(n) * (1.0 - 2.0 ** -24)).astype(np.float32))
+
+    def _params(self, states, dev):
+        p = np.zeros(len(states), rlsampler.ROW_PARAMS_DTYPE)
+        p["temperature"], p["top_p"], p["repeat_penalty"] = [s.temperature for s in states], 1.0, 1.0
+        return rlsampler.params_tensor(p, dev)
+
+    def _uniforms(self, shape, dev):
+        import torch
+
+        return torch.from_numpy(np.ascontiguousarray(self.uniform(int(np.prod(shape))), np.float32).reshape(shape)).to(dev)
+
+    def draft(self, states, logits):
+        """One drafted token [B] (device) a sequence from draft logits [B, V]."""
+        if tuple(logits.shape) != (len(states), self.V):
+            raise ValueError(f"draft logits {tuple(logits.shape)} for {len(states)} sequences of vocabulary {self.V}")
+        tok, _, _ = self.sampler.sample(logits, self._params(states, logits.device), self._uniforms((len(states),), logits.device))
+        return tok
+
+    def verify(self, states, target_logits, drafts, draft_logits=None, n_draft=None):
+        """target_logits [B * (K + 1), V] (a sequence's rows after 0 .. K drafts),
+        drafts [B, K] int32 and the logits [B * K, V] they were drawn from
+        (None: given drafts), n_draft [B] of them (None: K). Returns the
+        device tensors (accepted [B], tokens [B, K + 1]); the states are not
+        changed."""
+        import torch
+
+        B, dev = len(states), target_logits.device
+        if tuple(drafts.shape) != (B, self.K) or tuple(target_logits.shape) != (B * (self.K + 1), self.V):
+            raise ValueError(f"drafts {tuple(drafts.shape)} and target logits {tuple(target_logits.shape)} for {B} sequences")
+        T = torch.tensor([s.temperature for s in states], dtype=torch.float32, device=dev)
+        n = torch.full((B,), self.K, dtype=torch.int32, device=dev) if n_draft is None else n_draft
+        acc, tok, _, st = self.sampler.specdec_verify_draft(
+            rlsampler.DistRows(target_logits, T), drafts, n, self._uniforms((B, self.K), dev), self._uniforms((B,), dev),
+            draft=None if draft_logits is None else rlsampler.DistRows(draft_logits, T))
+        bad = st.cpu().numpy()
+        if (bad != 0).any():
+            i = int(np.flatnonzero(bad)[0])
+            raise rlsampler.RLError(int(bad[i]), f"sequence {states[i].seq_id}: row status {int(bad[i])}")
+        return acc, tok
+
+    def step(self, states, target_logits, drafts, draft_logits=None, n_draft=None) -> dict:
+        """verify() and the per-sequence updates; returns {seq_id: [tokens]}."""
+        return apply_tokens(states, self.verify(states, target_logits, drafts, draft_logits, n_draft)[1].cpu().numpy())
 
     def close(self):
         self.sampler.close()
