@@ -302,7 +302,7 @@ rl_status rl_specdec_verify(rl_sampler* h, const float* logits, int B, int V, in
  *   first_row[B]    the sequence's first row (NULL: sequences follow one
  *                   another at the widest number of rows); `rows` is the
  *                   number of rows that may be read.
- * -inf logits have probability 0. Weights below 2^-125 of the row's largest may
+ * -inf logits have probability 0. Weights below 2^-60 of the row's largest may
  * count as 0. 1e-30 and 3e38 bound log2(e) / T.
  *
  * rl_specdec_verify_draft -- a chain. Sequence b has n_draft[b] in [0,

@@ -27,9 +27,9 @@
 // Precision. A weight is 2^(x c - F): one FMA and ex2.approx, relative error
 // about 2^-22 with no bias that two ids would not share; c = log2(e) / T in
 // single precision tilts a row by at most 2^-25 |t|. A lane's F is the product
-// max c of the first logits it sees, moved only where a later logit lies 64
+// x c of the first logit it sees, moved only where a later logit lies 64
 // binades above: any F does, as long as the sums are joined with it, and no
-// running maximum has to be kept. Sums are doubles, and draws are compared in
+// maximum has to be found. Sums are doubles, and draws are compared in
 // doubles: a token can differ from the exact one only where the draw lies
 // within about 1e-8 of a border.
 #include <cooperative_groups.h>
@@ -110,22 +110,28 @@ __device__ __forceinline__ float ex2(float t) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
   return r;
 }
-// Where a row's largest logit m lies in the exponent's domain: F = m c. A
-// product beyond the range of floats (a row of lowest values, say) is marked
-// by an infinite F; there any two logits that differ are infinitely far apart.
-__device__ __forceinline__ float frame(float m, float c) { return m * c; }
-// The weight of x relative to the frame; 0 for x = -inf, NaN for NaN.
-__device__ __forceinline__ float weight(float x, float c, float F) { return ex2(__fmaf_rn(x, c, -F)); }
-__device__ __forceinline__ float weight(float x, float m, float c, float F) {
-  const float e = weight(x, c, F);
-  const float f = x == m ? 1.0f : (x != x ? x : 0.0f);
-  return fabsf(F) < RL_POS_INF ? e : f;
+// Where a logit m lies in the exponent's domain: F = m c. From 2^24 on the
+// product's rounding would be binades (and it can leave the range of floats): such
+// frames are marked by NaN, and weights are taken from the difference x - m.
+__device__ __forceinline__ float frame(float m, float c) {
+  const float F = m * c;
+  return fabsf(F) < 16777216.0f ? F : __int_as_float(0x7fc00000);
 }
+__device__ __forceinline__ bool is_near(float F) { return F == F; }
+// The exponent of x relative to the frame of logit m.
+__device__ __forceinline__ float exponent(float x, float m, float c, float F) {
+  return is_near(F) ? __fmaf_rn(x, c, -F) : (x - m) * c;
+}
+// The weight of x; 0 for x = -inf, NaN for NaN. Of the first two the one without m
+// is for frames that are known to be near, and NaN for others.
+__device__ __forceinline__ float weight(float x, float c, float F) { return ex2(__fmaf_rn(x, c, -F)); }
+__device__ __forceinline__ float weight(float x, float m, float c, float F) { return ex2(exponent(x, m, c, F)); }
 // The same with the exponent in two floats.
 __device__ __forceinline__ float weight_2(float x, float m, float c, float F) {
   if (!(x > RL_NEG_INF)) return 0.0f;
-  if (!(fabsf(F) < RL_POS_INF)) return x == m ? 1.0f : 0.0f;
+  if (!is_near(F)) return weight(x, m, c, F);
   const float p = __fmul_rn(x, c), e = __fmaf_rn(x, c, -p);
+  if (!(fabsf(p) < RL_POS_INF)) return ex2(__fmaf_rn(x, c, -F));
   const float t = __fadd_rn(p, -F), v = __fadd_rn(t, -p);
   const float f = __fadd_rn(__fadd_rn(p, -__fadd_rn(t, -v)), __fadd_rn(-F, -v));  // p - F = t + f
   return ex2(t) * ex2(__fadd_rn(e, f));
@@ -136,8 +142,9 @@ __device__ __forceinline__ float weight_2(float x, float m, float c, float F) {
 // that falls in it finds an id.
 __device__ __forceinline__ float rebase(float m, float F, float M, float G, float c) {
   if (m == M) return 1.0f;
-  const float t = F - G;
-  return fminf(t, __fmaf_rn(m, c, -G)) >= -125.0f ? ex2(t) : 0.0f;
+  const float w = exponent(m, M, c, G);
+  const float t = !is_near(F) ? w : is_near(G) ? F - G : -__fmaf_rn(M, c, -F);
+  return fminf(t, w) >= -125.0f ? ex2(t) : 0.0f;
 }
 
 // A row of logits with what decides which of its ids are kept.
@@ -199,7 +206,7 @@ __device__ __forceinline__ void keep4(const Row<T>& r, int j0, uint32_t bits, fl
 
 struct __align__(16) Part {
   double s;  // sum of weights relative to m's frame (T <= 0: NaN marks a NaN)
-  float m;   // a logit of the part, near its largest (T <= 0: the largest)
+  float m;   // a logit of the part, at most 64 binades below its largest (T <= 0: the largest)
   int id;    // T <= 0: lowest id at m
 };
 
@@ -250,7 +257,7 @@ struct Seen {
   int id;
 };
 __device__ __forceinline__ Seen unseen() {
-  return {RL_NEG_INF, __int_as_float(0x7fc00000), 0.0, INT_MAX};  // a frame of NaN: the first chunk sets it
+  return {RL_NEG_INF, 0.0f, 0.0, INT_MAX};
 }
 
 __device__ __forceinline__ void see_max(Seen& z, const float (&x)[4][4], int j0) {
@@ -265,30 +272,33 @@ __device__ __forceinline__ void see_max(Seen& z, const float (&x)[4][4], int j0)
 }
 
 __device__ __forceinline__ void see(Seen& z, const float (&x)[4][4], float c) {
+  if (!(z.m > RL_NEG_INF)) {  // nothing seen yet: the first logit's frame
+    z.m = x[0][0];
+    z.F = frame(z.m, c);
+  }
   float e[4];
 #pragma unroll
   for (int u = 0; u < 4; ++u)
     e[u] = (weight(x[u][0], c, z.F) + weight(x[u][1], c, z.F)) + (weight(x[u][2], c, z.F) + weight(x[u][3], c, z.F));
   float sum = (e[0] + e[1]) + (e[2] + e[3]);
   if (!(sum < kHigh)) {
-    // no frame yet, one that is far too low, an infinite one, or a NaN
+    // a frame that is far too low, one that is not near 0, or a NaN
     const float gm = max16(x);
     if (gm != gm) z.s = __longlong_as_double(0x7ff8000000000000LL);
     if (gm > z.m) {
-      const float F = frame(gm, c);
-      if (z.m > RL_NEG_INF) z.s *= static_cast<double>(rebase(z.m, z.F, gm, F, c));
+      if (z.m > RL_NEG_INF) z.s *= static_cast<double>(rebase(z.m, z.F, gm, frame(gm, c), c));
       z.m = gm;
-      z.F = F;
+      z.F = frame(gm, c);
     }
     sum = 0.0f;
     if (z.m > RL_NEG_INF) {
-      if (fabsf(z.F) < RL_POS_INF) {
+      if (is_near(z.F)) {
 #pragma unroll
         for (int u = 0; u < 4; ++u)
           sum += (weight(x[u][0], c, z.F) + weight(x[u][1], c, z.F)) + (weight(x[u][2], c, z.F) + weight(x[u][3], c, z.F));
       } else {
 #pragma unroll
-        for (int k = 0; k < 16; ++k) sum += x[k >> 2][k & 3] == z.m ? 1.0f : 0.0f;
+        for (int k = 0; k < 16; ++k) sum += weight(x[k >> 2][k & 3], z.m, c, z.F);
       }
     }
   }
@@ -383,18 +393,42 @@ __device__ __forceinline__ void chunk_load(const Row<T>& r, int c0, float (&x)[4
       for (int k = 0; k < 4; ++k) x[i][k] = to_f(__ldg(at + 128 * i + k));
   }
 }
-// The same of a row's last ids, cut at `end`. Parts are whole chunks, so this
-// is one warp's; a function with an array of its own, which keeps its cases out
+// The same of the last ids of a row or of two, cut at `end`. Parts are whole
+// chunks, so this is one warp's, and all others wait for it: all of its loads are
+// in flight at once. A function with arrays of its own, which keeps its cases out
 // of the other warps' loops.
-template <typename T>
-__device__ __noinline__ void chunk_cut(const T* row, int c0, int end, float* x) {
-#pragma unroll 1
-  for (int i = 0; i < 4; ++i) {
-    float v[4];
-    unit_guarded(row, c0 + 128 * i + 4 * (static_cast<int>(threadIdx.x) & 31), end, v);
+template <bool Plain, typename T>
+__device__ __forceinline__ void load_cut(const T* row, int j0, int end, float (&v)[4][4]) {
+  const bool units = Plain || (reinterpret_cast<uintptr_t>(row) & (4 * sizeof(T) - 1)) == 0;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) x[4 * i + k] = v[k];
+  for (int i = 0; i < 4; ++i) {
+    const int j = j0 + 128 * i;
+    v[i][0] = v[i][1] = v[i][2] = v[i][3] = RL_NEG_INF;
+    if (units && j + 4 <= end) unit(row + j, v[i]);
   }
+  if (!units || (end & 3)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (!units || j0 + 128 * i + 4 > end) unit_guarded(row, j0 + 128 * i, end, v[i]);
+  }
+}
+template <bool Plain, typename T>
+__device__ __noinline__ void chunk_cut(const T* row, int c0, int end, float* x) {
+  float v[4][4];
+  load_cut<Plain>(row, c0 + 4 * (static_cast<int>(threadIdx.x) & 31), end, v);
+#pragma unroll
+  for (int k = 0; k < 16; ++k) x[k] = v[k >> 2][k & 3];
+}
+template <bool Plain, typename TP, typename TQ>
+__device__ __noinline__ void chunk_cut(const TP* rp, const TQ* rq, int c0, int end, float* x, float* y) {
+  float v[4][4], w[4][4];
+  const int j0 = c0 + 4 * (static_cast<int>(threadIdx.x) & 31);
+  load_cut<Plain>(rp, j0, end, v);
+  load_cut<Plain>(rq, j0, end, w);
+#pragma unroll
+  for (int k = 0; k < 16; ++k) x[k] = v[k >> 2][k & 3];
+#pragma unroll
+  for (int k = 0; k < 16; ++k) y[k] = w[k >> 2][k & 3];
 }
 template <bool Plain, typename T>
 __device__ __forceinline__ void chunk_keep(const Row<T>& r, int c0, int end, float (&x)[4][4]) {
@@ -424,7 +458,7 @@ __device__ __forceinline__ void pass(const Row<T>& r, int j0, int j1, F f) {
   }
   if (whole < j1) {
     float t[4][4];
-    chunk_cut(r.x, whole, j1, &t[0][0]);
+    chunk_cut<Plain>(r.x, whole, j1, &t[0][0]);
     chunk_keep<Plain>(r, whole, j1, t);
     f(whole, t);
   }
@@ -448,13 +482,12 @@ __device__ __forceinline__ void pass_two(const Row<TP>& rp, const Row<TQ>& rq, i
     }
   }
   if (whole < j1) {
-    float t[4][4];
-    chunk_cut(rp.x, whole, j1, &t[0][0]);
+    float t[4][4], u[4][4];
+    chunk_cut<Plain>(rp.x, rq.x, whole, j1, &t[0][0], &u[0][0]);
     chunk_keep<Plain>(rp, whole, j1, t);
     f(whole, t);
-    chunk_cut(rq.x, whole, j1, &t[0][0]);
-    chunk_keep<Plain>(rq, whole, j1, t);
-    g(whole, t);
+    chunk_keep<Plain>(rq, whole, j1, u);
+    g(whole, u);
   }
 }
 // f on both.
@@ -477,8 +510,7 @@ __device__ __forceinline__ void pass_both(const Row<TP>& rp, const Row<TQ>& rq, 
   }
   if (whole < j1) {
     float t[4][4], u[4][4];
-    chunk_cut(rp.x, whole, j1, &t[0][0]);
-    chunk_cut(rq.x, whole, j1, &u[0][0]);
+    chunk_cut<Plain>(rp.x, rq.x, whole, j1, &t[0][0], &u[0][0]);
     chunk_keep<Plain>(rp, whole, j1, t);
     chunk_keep<Plain>(rq, whole, j1, u);
     f(t, u);
@@ -563,7 +595,7 @@ __device__ __noinline__ double sum_resid(Row<TP> rp, Row<TQ> rq, int j0, int j1,
   double s = 0.0;
   pass_both<Plain>(rp, rq, j0, j1, [&](const float (&x)[4][4], const float (&y)[4][4]) {
     float w = 0.0f;
-    if (fabsf(f.Fp) < RL_POS_INF && fabsf(f.Fq) < RL_POS_INF) {
+    if (is_near(f.Fp) && is_near(f.Fq)) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         float v[4];
@@ -619,26 +651,27 @@ __device__ __forceinline__ Row<T> make_row(const VdSide& a, int64_t row, int cut
 }
 
 // One side's share of a node's entry: the token's logit (-inf outside the row)
-// and mask bit in the parent's row, the node's own row's cutoff.
+// and mask bit in the parent's row,
 template <typename T>
-__device__ __forceinline__ void read_node(const VdSide& a, int64_t row0, int V, int node, int parent, int tok, bool own_row,
-                                          float& logit, uint8_t& bit, int& cut, float& xcut) {
+__device__ __forceinline__ void read_token(const VdSide& a, int64_t row0, int V, int parent, int tok, float& logit, uint8_t& bit) {
   logit = RL_NEG_INF;
   bit = 1;
-  cut = -1;
-  xcut = 0.0f;
-  const T* x = static_cast<const T*>(a.logits);
   if (parent >= 0 && static_cast<unsigned>(tok) < static_cast<unsigned>(V)) {
     const int64_t row = row0 + parent;
-    logit = to_f(x[row * a.ld + tok]);
+    logit = to_f(static_cast<const T*>(a.logits)[row * a.ld + tok]);
     if (a.mask) bit = (a.mask[row * a.mask_stride + (tok >> 5)] >> (tok & 31)) & 1u;
   }
-  if (a.cut && own_row) {
-    const int64_t row = row0 + node;
+}
+// and the node's own row's cutoff.
+template <typename T>
+__device__ __forceinline__ void read_cut(const VdSide& a, int64_t row, int V, int& cut, float& xcut) {
+  cut = -1;
+  xcut = 0.0f;
+  if (a.cut) {
     const int c = a.cut[row * a.cut_stride];
     if (static_cast<unsigned>(c) < static_cast<unsigned>(V)) {
       cut = c;
-      xcut = to_f(x[row * a.ld + c]);
+      xcut = to_f(static_cast<const T*>(a.logits)[row * a.ld + c]);
     }
   }
 }
@@ -673,6 +706,15 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
   int32_t* out_path = a.out_path ? a.out_path + static_cast<int64_t>(b) * N : nullptr;
   float* out_prob = a.out_prob ? a.out_prob + static_cast<int64_t>(b) * N : nullptr;
 
+  // ---- a thread a node ----
+  static_assert(RL_VERIFY_MAX_NODES <= kVT, "a thread a node");
+  const bool has_entry = tid >= a.tok_off && tid < N;  // a chain's node 0 has none
+  const int64_t entry = static_cast<int64_t>(b) * a.tok_stride + tid - a.tok_off;
+  const int my_tok = has_entry ? a.tokens[entry] : -1;
+  const float my_u = has_entry ? a.accept_u[entry] : 0.0f;
+  int my_parent = tid - 1;
+  if (tree) my_parent = has_entry ? a.parent[entry] : -1;
+  if (my_parent < 0 || my_parent >= tid) my_parent = -1;
   // ---- the sequence's numbers, checked ----
   const int n = a.count[b] + a.count_add;
   const float Tp = a.p.T ? a.p.T[b] : 1.0f;
@@ -699,25 +741,20 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
     if (drawn && n > 1) fetch(qx0, j0, j1);
   }
   if (C > 1) cgx::this_cluster().barrier_arrive();
-  for (int i = tid; i < N; i += kVT) {
-    const int64_t at = static_cast<int64_t>(b) * a.tok_stride + i - a.tok_off;
-    const bool is = i >= a.tok_off;  // a chain's node 0 has no entry
-    Node& nd = nodes[i];
-    nd.tok = is ? a.tokens[at] : -1;
-    nd.u = is ? a.accept_u[at] : 0.0f;
-    int f = tree ? a.parent[at] : i - 1;
-    if (f < 0 || f >= i) f = -1;
-    nd.parent = static_cast<int16_t>(f);
-    nd.first = !tree && i + 1 < n ? i + 1 : INT_MAX;
-    if (status == RL_OK && i < n) {
-      read_node<TP>(a.p, p0, V, i, f, nd.tok, true, nd.lp, nd.bit[0], nd.cut[0], nd.xcut[0]);
-      if (drawn) read_node<TQ>(a.q, q0, V, i, f, nd.tok, tree || i + 1 < n, nd.lq, nd.bit[1], nd.cut[1], nd.xcut[1]);
+  if (tid < N) {
+    Node& nd = nodes[tid];
+    nd.tok = my_tok;
+    nd.u = my_u;
+    nd.parent = static_cast<int16_t>(my_parent);
+    nd.first = !tree && tid + 1 < n ? tid + 1 : INT_MAX;
+    if (!Plain && status == RL_OK && tid < n) {
+      read_cut<TP>(a.p, p0 + tid, V, nd.cut[0], nd.xcut[0]);
+      if (drawn && (tree || tid + 1 < n)) read_cut<TQ>(a.q, q0 + tid, V, nd.cut[1], nd.xcut[1]);
     }
   }
   __syncthreads();
   if (tree && status == RL_OK) {
-    for (int i = tid; i < n; i += kVT)
-      if (nodes[i].parent >= 0) atomicMin(&nodes[nodes[i].parent].first, i);
+    if (tid < n && my_parent >= 0) atomicMin(&nodes[my_parent].first, tid);
     __syncthreads();
   }
 
@@ -729,14 +766,13 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
   while (status == RL_OK) {
     // ---- the node's rows and its children ----
     const Node& nd = nodes[node];
-    Row<TP> rp = make_row<TP>(a.p, p0 + node, nd.cut[0], nd.xcut[0]);
+    Row<TP> rp = make_row<TP>(a.p, p0 + node, Plain ? -1 : nd.cut[0], Plain ? 0.0f : nd.xcut[0]);
     const int firstc = nd.first;
     const bool with_q = drawn && firstc != INT_MAX;
     Row<TQ> rq = {};
-    if (with_q) rq = make_row<TQ>(a.q, q0 + node, nd.cut[1], nd.xcut[1]);
+    if (with_q) rq = make_row<TQ>(a.q, q0 + node, Plain ? -1 : nd.cut[1], Plain ? 0.0f : nd.xcut[1]);
     if (Plain || (no_mask & 1)) rp.mask = nullptr;
     if (Plain || (no_mask & 2)) rq.mask = nullptr;
-    if (Plain) rp.cut = rq.cut = -1;
     // ---- this warp's sums of both rows, into every CTA of the cluster ----
     Seen zp, zq = unseen();
     if (with_q) {
@@ -754,14 +790,23 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
       warp_parts(zp, cp, zq, cq, greedy, pp, pq);
       // every CTA of the cluster has started: its shared memory may be written
       if (C > 1 && !started) cgx::this_cluster().barrier_wait();
-      started = true;
       if (lane < C) {
         Part* to = C > 1 ? cl.map_shared_rank(&sh.part[par][0][0], lane) : &sh.part[par][0][0];
         to[mypart] = pp;
         if (with_q) to[kParts + mypart] = pq;
       }
     }
-    if (C > 1) cl.sync();
+    if (C > 1) cgx::this_cluster().barrier_arrive();
+    if (!started) {  // meanwhile: the nodes' logits
+      if (tid < n) {
+        Node& me = nodes[tid];
+        read_token<TP>(a.p, p0, V, my_parent, my_tok, me.lp, me.bit[0]);
+        if (drawn) read_token<TQ>(a.q, q0, V, my_parent, my_tok, me.lq, me.bit[1]);
+      }
+      __syncthreads();
+      started = true;
+    }
+    if (C > 1) cgx::this_cluster().barrier_wait();
     else __syncthreads();
     // ---- joined by warp 0 of every CTA ----
     double wp[kPerLane];

@@ -497,3 +497,53 @@ def test_first_ids_at_the_edge_of_the_weights(smp, pad, first):
     assert (st == 0).all() and (acc == 0).all()
     assert np.isin(tok, [0, V - 5]).all(), tok[~np.isin(tok, [0, V - 5])]
     assert (tok[gap < 124.5 * np.log(2.0)] == 0).all()
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("drawn", [False, True])
+def test_products_beyond_the_range_of_floats(smp, sign, drawn):
+    """At a temperature of 1e-38 logits times 1 / T leave the range of floats:
+    all of a row's probability is on its largest logit, wherever that lies."""
+    V, places = 128256, [0, 3, 700, 1100, 1537, 64000, 128255]
+    B = len(places)
+    rng = np.random.default_rng(41)
+    x = (rng.random((B, V)) * 8 + (10 if sign > 0 else -40)).astype(np.float32)
+    for b, j in enumerate(places):
+        x[b, j] = 19.0 if sign > 0 else -5.0
+    T = torch.full((B,), 1e-38, device=DEV)
+    rows = torch.from_numpy(x).to(DEV)
+    du = torch.tensor([0.0, 0.3, 0.6, 0.9, 0.99, 0.5, 0.1], device=DEV)
+    K = 1 if drawn else 0
+    drafts = torch.tensor([[(j + 1) % V] for j in places], dtype=torch.int32, device=DEV)[:, :K].contiguous()
+    kw = {}
+    if drawn:
+        y = x.copy()
+        y[np.arange(B), [(j + 1) % V for j in places]] = 20.0
+        kw["draft"] = rlsampler.DistRows(torch.from_numpy(y).to(DEV), T)
+        rows = rows.repeat_interleave(2, 0).contiguous()
+    acc, tok, prob, st = smp.specdec_verify_draft(rlsampler.DistRows(rows, T), drafts, torch.full((B,), K, dtype=torch.int32, device=DEV),
+                                                  torch.full((B, K), 0.5, device=DEV), du, **kw)
+    assert (st == 0).all() and (acc == 0).all()
+    assert tok[:, 0].tolist() == places and (prob[:, 0] == 1).all()
+
+
+@pytest.mark.parametrize("T", [1e-4, 1e-6, 1e-7, 1e-8, 1e-9, 1e-12, 1e-20, 1e-30, 1e-37, 2e-38])
+@pytest.mark.parametrize("shift", [-40.0, -3.0, 0.0, 12.0, 900.0])
+def test_small_temperatures_at_any_level(smp, T, shift):
+    """Logits over T far above 1, where products lose the fractions that decide:
+    a few ids lie within a few T of the largest (as far as f32 can tell them
+    apart), the others below."""
+    B, V = 12, 9000
+    rng = np.random.default_rng(43)
+    c = Case(rng, B, V, K=2, T=np.full(B, T), sigma=2.0)
+    step = np.abs(np.spacing(np.float32(abs(shift) + 8)))
+    for rows in (c.pr, c.qr):
+        x = rows.cpu().numpy() * np.float32(0.5)
+        x = np.minimum(x, 6.0).astype(np.float32)
+        for r in range(len(x)):
+            near = rng.choice(V, 6, replace=False)
+            x[r, near] = 8.0 - np.round(rng.random(6) * 5) * max(step, np.float32(T))
+        rows.copy_(torch.from_numpy((x.astype(np.float64) + shift).astype(np.float32)))
+    c.x, c.y = c.pr.cpu().numpy(), c.qr.cpu().numpy()
+    c.tok[:] = np.argmax(c.x.reshape(B, 3, V)[:, :2], 2).reshape(c.tok.shape)
+    c.check(c.call(smp), ok=0.9)
