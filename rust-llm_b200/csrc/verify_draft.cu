@@ -86,6 +86,11 @@ struct VdArgs {
 
 // log2(e) / T.
 __device__ __forceinline__ float scale_of(float T) {
+  if (T > 1e-30f && T < 1e30f) {  // a quotient and its remainder: nearest but for 2^-30
+    constexpr float hi = 1.44269504f, lo = static_cast<float>(1.4426950408889634074 - static_cast<double>(hi));
+    const float y = __frcp_rn(T), q = __fmul_rn(hi, y);
+    return __fmaf_rn(__fadd_rn(__fmaf_rn(-q, T, hi), lo), y, q);
+  }
   return static_cast<float>(fmin(fmax(1.4426950408889634074 / static_cast<double>(T), 1e-30), 3e38));
 }
 
@@ -203,6 +208,25 @@ __device__ __forceinline__ void keep4(const Row<T>& r, int j0, uint32_t bits, fl
       if (x[k] < r.xcut || (x[k] == r.xcut && j0 + k > r.cut)) x[k] = RL_NEG_INF;
   }
 }
+// The words of a chunk's mask, loaded with its logits.
+template <bool Plain>
+struct Bits {
+  uint32_t w[4];
+  template <typename T>
+  __device__ __forceinline__ void load(const Row<T>& r, int c0, int end) {
+    if (!r.mask) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int j = c0 + 128 * i + 4 * (static_cast<int>(threadIdx.x) & 31);
+      w[i] = j < end ? __ldg(r.mask + (j >> 5)) : 0u;
+    }
+  }
+};
+template <>
+struct Bits<true> {
+  template <typename T>
+  __device__ __forceinline__ void load(const Row<T>&, int, int) {}
+};
 
 struct __align__(16) Part {
   double s;  // sum of weights relative to m's frame (T <= 0: NaN marks a NaN)
@@ -431,14 +455,12 @@ __device__ __noinline__ void chunk_cut(const TP* rp, const TQ* rq, int c0, int e
   for (int k = 0; k < 16; ++k) y[k] = w[k >> 2][k & 3];
 }
 template <bool Plain, typename T>
-__device__ __forceinline__ void chunk_keep(const Row<T>& r, int c0, int end, float (&x)[4][4]) {
+__device__ __forceinline__ void chunk_keep(const Row<T>& r, int c0, const Bits<Plain>& m, float (&x)[4][4]) {
   if constexpr (!Plain) {
     if (!r.mask && r.cut < 0) return;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int j = c0 + 128 * i + 4 * (static_cast<int>(threadIdx.x) & 31);
-      keep4(r, j, r.mask ? bits4(r.mask, j, end) : 0u, x[i]);
-    }
+    for (int i = 0; i < 4; ++i)
+      keep4(r, c0 + 128 * i + 4 * (static_cast<int>(threadIdx.x) & 31), m.w[i] >> (4 * (threadIdx.x & 7)), x[i]);
   }
 }
 
@@ -447,19 +469,25 @@ __device__ __forceinline__ void chunk_keep(const Row<T>& r, int c0, int end, flo
 template <bool Plain, typename T, typename F>
 __device__ __forceinline__ void pass(const Row<T>& r, int j0, int j1, F f) {
   const int whole = j1 - (j1 - j0) % kChunk;
+  Bits<Plain> m;
   if (j0 < whole) {
     float x[4][4];
+    m.load(r, j0, j1);
     chunk_load<Plain>(r, j0, x);
     for (int c0 = j0; c0 < whole; c0 += kChunk) {
-      chunk_keep<Plain>(r, c0, j1, x);
+      chunk_keep<Plain>(r, c0, m, x);
       f(c0, x);
-      if (c0 + kChunk < whole) chunk_load<Plain>(r, c0 + kChunk, x);
+      if (c0 + kChunk < whole) {
+        m.load(r, c0 + kChunk, j1);
+        chunk_load<Plain>(r, c0 + kChunk, x);
+      }
     }
   }
   if (whole < j1) {
     float t[4][4];
+    m.load(r, whole, j1);
     chunk_cut<Plain>(r.x, whole, j1, &t[0][0]);
-    chunk_keep<Plain>(r, whole, j1, t);
+    chunk_keep<Plain>(r, whole, m, t);
     f(whole, t);
   }
 }
@@ -467,26 +495,37 @@ __device__ __forceinline__ void pass(const Row<T>& r, int j0, int j1, F f) {
 template <bool Plain, typename TP, typename TQ, typename F, typename G>
 __device__ __forceinline__ void pass_two(const Row<TP>& rp, const Row<TQ>& rq, int j0, int j1, F f, G g) {
   const int whole = j1 - (j1 - j0) % kChunk;
+  Bits<Plain> m, n;
   if (j0 < whole) {
     float x[4][4], y[4][4];
+    m.load(rp, j0, j1);
+    n.load(rq, j0, j1);
     chunk_load<Plain>(rp, j0, x);
     chunk_load<Plain>(rq, j0, y);
     for (int c0 = j0; c0 < whole; c0 += kChunk) {
       const bool more = c0 + kChunk < whole;
-      chunk_keep<Plain>(rp, c0, j1, x);
+      chunk_keep<Plain>(rp, c0, m, x);
       f(c0, x);
-      if (more) chunk_load<Plain>(rp, c0 + kChunk, x);
-      chunk_keep<Plain>(rq, c0, j1, y);
+      if (more) {
+        m.load(rp, c0 + kChunk, j1);
+        chunk_load<Plain>(rp, c0 + kChunk, x);
+      }
+      chunk_keep<Plain>(rq, c0, n, y);
       g(c0, y);
-      if (more) chunk_load<Plain>(rq, c0 + kChunk, y);
+      if (more) {
+        n.load(rq, c0 + kChunk, j1);
+        chunk_load<Plain>(rq, c0 + kChunk, y);
+      }
     }
   }
   if (whole < j1) {
     float t[4][4], u[4][4];
+    m.load(rp, whole, j1);
+    n.load(rq, whole, j1);
     chunk_cut<Plain>(rp.x, rq.x, whole, j1, &t[0][0], &u[0][0]);
-    chunk_keep<Plain>(rp, whole, j1, t);
+    chunk_keep<Plain>(rp, whole, m, t);
     f(whole, t);
-    chunk_keep<Plain>(rq, whole, j1, u);
+    chunk_keep<Plain>(rq, whole, n, u);
     g(whole, u);
   }
 }
@@ -494,15 +533,20 @@ __device__ __forceinline__ void pass_two(const Row<TP>& rp, const Row<TQ>& rq, i
 template <bool Plain, typename TP, typename TQ, typename F>
 __device__ __forceinline__ void pass_both(const Row<TP>& rp, const Row<TQ>& rq, int j0, int j1, F f) {
   const int whole = j1 - (j1 - j0) % kChunk;
+  Bits<Plain> m, n;
   if (j0 < whole) {
     float x[4][4], y[4][4];
+    m.load(rp, j0, j1);
+    n.load(rq, j0, j1);
     chunk_load<Plain>(rp, j0, x);
     chunk_load<Plain>(rq, j0, y);
     for (int c0 = j0; c0 < whole; c0 += kChunk) {
-      chunk_keep<Plain>(rp, c0, j1, x);
-      chunk_keep<Plain>(rq, c0, j1, y);
+      chunk_keep<Plain>(rp, c0, m, x);
+      chunk_keep<Plain>(rq, c0, n, y);
       f(x, y);
       if (c0 + kChunk < whole) {
+        m.load(rp, c0 + kChunk, j1);
+        n.load(rq, c0 + kChunk, j1);
         chunk_load<Plain>(rp, c0 + kChunk, x);
         chunk_load<Plain>(rq, c0 + kChunk, y);
       }
@@ -510,9 +554,11 @@ __device__ __forceinline__ void pass_both(const Row<TP>& rp, const Row<TQ>& rq, 
   }
   if (whole < j1) {
     float t[4][4], u[4][4];
+    m.load(rp, whole, j1);
+    n.load(rq, whole, j1);
     chunk_cut<Plain>(rp.x, rq.x, whole, j1, &t[0][0], &u[0][0]);
-    chunk_keep<Plain>(rp, whole, j1, t);
-    chunk_keep<Plain>(rq, whole, j1, u);
+    chunk_keep<Plain>(rp, whole, m, t);
+    chunk_keep<Plain>(rq, whole, n, u);
     f(t, u);
   }
 }
@@ -800,8 +846,12 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
     if (!started) {  // meanwhile: the nodes' logits
       if (tid < n) {
         Node& me = nodes[tid];
-        read_token<TP>(a.p, p0, V, my_parent, my_tok, me.lp, me.bit[0]);
-        if (drawn) read_token<TQ>(a.q, q0, V, my_parent, my_tok, me.lq, me.bit[1]);
+        float lp, lq = RL_NEG_INF;  // both loads in flight
+        uint8_t bp, bq = 1;
+        read_token<TP>(a.p, p0, V, my_parent, my_tok, lp, bp);
+        if (drawn) read_token<TQ>(a.q, q0, V, my_parent, my_tok, lq, bq);
+        me.lp = lp, me.lq = lq;
+        me.bit[0] = bp, me.bit[1] = bq;
       }
       __syncthreads();
       started = true;
