@@ -1032,17 +1032,31 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
     };
     if (!resid && nrem > 0) {
       // the parts that hold refused given tokens sum again (taking a weight
-      // off a sum would leave its rounding)
+      // off a sum would leave its rounding), each by all warps of its CTA
       const Part me = sh.part[par ^ 1][0][mypart];
       double f = me.m > RL_NEG_INF ? me.s * static_cast<double>(rebase(me.m, frame(me.m, cp), Pm, Fp, cp)) : 0.0;
-      bool again = false;
-      for (int k = 0; k < nrem; ++k) {
-        const int t = nodes[sh.removed[k]].tok;
-        again |= t >= j0 && t < j1;
+      unsigned again = 0;  // this CTA's parts that do
+      const int64_t cta0 = static_cast<int64_t>(rank) * kVW * a.part;
+      for (int k = lane; k < nrem; k += 32) {
+        const int64_t t = nodes[sh.removed[k]].tok - cta0;
+        if (t >= 0 && t < static_cast<int64_t>(kVW) * a.part) again |= 1u << (static_cast<int>(t) / a.part);
       }
-      if (again) {
-        const double s = sum_kept<Plain>(rp, j0, j1, cp, Pm, Fp, &sh, nodes, nrem);
-        f = warp_sum_d(s);
+      again = __reduce_or_sync(0xffffffffu, again);
+      for (; again; again &= again - 1) {
+        const int w = __ffs(again) - 1;
+        const int w0 = static_cast<int>(min(cta0 + static_cast<int64_t>(w) * a.part, static_cast<int64_t>(V)));
+        const int w1 = static_cast<int>(min(static_cast<int64_t>(w0) + a.part, static_cast<int64_t>(V)));
+        const int chunks = (w1 - w0 + kChunk - 1) / kChunk;
+        const int s0 = w0 + chunks * warp / kVW * kChunk, s1 = min(w0 + chunks * (warp + 1) / kVW * kChunk, w1);
+        double s = 0.0;
+        if (s0 < s1) s = warp_sum_d(sum_kept<Plain>(rp, s0, s1, cp, Pm, Fp, &sh, nodes, nrem));
+        if (lane == 0) sh.scan[warp] = s;
+        __syncthreads();
+        if (warp == w) {
+          f = 0.0;
+          for (int i = 0; i < kVW; ++i) f += sh.scan[i];
+        }
+        __syncthreads();
       }
       if (lane < C) (C > 1 ? cl.map_shared_rank(&sh.w[par][0], lane) : &sh.w[par][0])[mypart] = f;
       if (C > 1) cl.sync();
@@ -1062,22 +1076,46 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
     __syncthreads();
     const int owner = sh.owner;
     if (owner >= 0 && owner / kVW == rank) {
-      // ---- the drawn token inside that part, by the whole CTA ----
-      const int w0 = static_cast<int>(min(static_cast<int64_t>(owner) * a.part, static_cast<int64_t>(V)));
-      const int w1 = static_cast<int>(min(static_cast<int64_t>(w0) + a.part, static_cast<int64_t>(V)));
-      const int per = ((w1 - w0 + kVT - 1) / kVT + 3) & ~3;
-      const int a0 = static_cast<int>(min(static_cast<int64_t>(w0) + static_cast<int64_t>(tid) * per, static_cast<int64_t>(w1)));
-      const int a1 = min(a0 + per, w1);
+      // ---- the drawn token inside that part, by the whole CTA: down to 4 ids a
+      // thread by the sums of the warps' shares ----
+      int w0 = static_cast<int>(min(static_cast<int64_t>(owner) * a.part, static_cast<int64_t>(V)));
+      int w1 = static_cast<int>(min(static_cast<int64_t>(w0) + a.part, static_cast<int64_t>(V)));
+      double rest = sh.rest;
+      while (w1 - w0 > 4 * kVT) {
+        const int chunks = (w1 - w0 + kChunk - 1) / kChunk;
+        const auto share = [&](int w) { return min(w0 + chunks * w / kVW * kChunk, w1); };
+        const int s0 = share(warp), s1 = share(warp + 1);
+        double s = 0.0;
+        if (s0 < s1)
+          s = warp_sum_d(resid ? sum_resid<Plain>(rp, rq, s0, s1, Resid{cp, cq, Pm, Qm, Fp, Fq, rhi, rlo})
+                               : sum_kept<Plain>(rp, s0, s1, cp, Pm, Fp, &sh, nodes, nrem));
+        if (lane == 0) sh.scan[warp] = s;
+        __syncthreads();
+        int pick = 0;
+        double run = 0.0, before = 0.0;
+        for (int w = 0; w < kVW; ++w) {
+          const double v = sh.scan[w];
+          if (v > 0.0 && !(run > rest)) {
+            pick = w;
+            before = run;
+          }
+          run += v;
+        }
+        rest -= before;
+        const int to = share(pick + 1);
+        w0 = share(pick);
+        w1 = to;
+        __syncthreads();
+      }
+      const int a0 = w0 + 4 * tid;
+      float w[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (a0 < w1) w4(a0, w1, w);
       double s = 0.0;
       int last = -1;
-      for (int j = a0; j < a1; j += 4) {
-        float w[4];
-        w4(j, a1, w);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          s += static_cast<double>(w[k]);
-          if (w[k] > 0.0f) last = j + k;
-        }
+      for (int k = 0; k < 4; ++k) {
+        s += static_cast<double>(w[k]);
+        if (w[k] > 0.0f) last = a0 + k;
       }
       double incl = s;
 #pragma unroll
@@ -1088,20 +1126,15 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
       if (lane == 31) sh.scan[warp] = incl;
       __syncthreads();
       double run = incl - s;
-      for (int w = 0; w < warp; ++w) run += sh.scan[w];
-      const double rest = sh.rest;
+      for (int i = 0; i < warp; ++i) run += sh.scan[i];
       if (run + s > rest && s > 0.0) {
         bool hit = false;
-        for (int j = a0; j < a1 && !hit; j += 4) {
-          float w[4];
-          w4(j, a1, w);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            run += static_cast<double>(w[k]);
-            if (!hit && w[k] > 0.0f && run > rest) {
-              atomicMin(&sh.at, j + k);
-              hit = true;
-            }
+        for (int k = 0; k < 4; ++k) {
+          run += static_cast<double>(w[k]);
+          if (!hit && w[k] > 0.0f && run > rest) {
+            atomicMin(&sh.at, a0 + k);
+            hit = true;
           }
         }
       }
