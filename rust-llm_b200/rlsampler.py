@@ -627,8 +627,7 @@ class Sampler:
             raise ValueError(f"{who}: the draft rows differ from the target rows in V or device")
         t, d = target._of(B, who), draft._of(B, who) if draft is not None else None
         acc, st = torch.empty_like(n_draft), torch.empty_like(n_draft)
-        tok = torch.empty((B, K + 1), dtype=i32, device=dev)
-        prob = torch.empty((B, K + 1), dtype=f32, device=dev)
+        tok, prob = drafts.new_empty((B, K + 1)), accept_u.new_empty((B, K + 1))
         check(lib().rl_specdec_verify_draft(self.h, B, V, K, t, d, drafts.data_ptr(), n_draft.data_ptr(),
                                             accept_u.data_ptr(), draw_u.data_ptr(), acc.data_ptr(), tok.data_ptr(),
                                             prob.data_ptr(), st.data_ptr(), _raw_stream(stream, dev)),
