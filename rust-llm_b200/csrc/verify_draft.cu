@@ -249,6 +249,7 @@ struct Node {
 struct Ctl {
   Part part[2][2][kParts];  // [parity][side]: every CTA's warps write into every CTA
   double w[2][kParts];      // [parity] the parts' sums of w
+  uint64_t bar[2][2];       // [parity][0 parts, 1 sums of w]: what is to come has come
   double scan[kVW];
   double rest;              // draw target inside the draw's part
   double Ps, Qs;            // sums of weights of both rows, relative to Pm, Qm
@@ -722,6 +723,46 @@ __device__ __forceinline__ void read_cut(const VdSide& a, int64_t row, int V, in
   }
 }
 
+// ---- exchanges: every warp of the cluster writes what it has into every CTA, each
+// write counted by that CTA's barrier as it lands. (Plain remote stores behind a
+// barrier of the cluster wait for each store's way back first, about 1200 cycles
+// of the 1700 that such an exchange took.) ----
+__device__ __forceinline__ uint32_t in_cta(const void* p, int rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void send(const Part* to, const Part& v, const uint64_t* bar, int rank) {
+  const long long d = __double_as_longlong(v.s);
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(in_cta(to, rank)),
+               "r"(static_cast<uint32_t>(d)), "r"(static_cast<uint32_t>(d >> 32)), "r"(__float_as_uint(v.m)), "r"(v.id), "r"(in_cta(bar, rank))
+               : "memory");
+}
+__device__ __forceinline__ void send(const double* to, double v, const uint64_t* bar, int rank) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(in_cta(to, rank)),
+               "l"(__double_as_longlong(v)), "r"(in_cta(bar, rank))
+               : "memory");
+}
+// Warp 0 waits for `bytes` of them; bounded, and alike for its lanes.
+__device__ __forceinline__ bool receive(uint64_t* bar, uint32_t parity, uint32_t bytes) {
+  if ((threadIdx.x & 31) == 0) mbar_expect_tx(bar, bytes);
+  const long long t0 = clock64();
+  bool in = false;
+  while (!in) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    in = done != 0;
+    if (!in && clock64() - t0 > kWaitBudget) break;
+  }
+  return __all_sync(0xffffffffu, in) != 0;
+}
+
 // Whether a mask row has a bit (one without allows every id); block-wide.
 __device__ __forceinline__ bool any_bit(const uint32_t* mask, int V) {
   const int words = (V + 31) >> 5;
@@ -786,7 +827,11 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
     fetch(px0, j0, j1);
     if (drawn && n > 1) fetch(qx0, j0, j1);
   }
-  if (C > 1) cgx::this_cluster().barrier_arrive();
+  if (tid == 0) {
+    for (int i = 0; i < 4; ++i) mbar_init(&sh.bar[i >> 1][i & 1], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  cgx::this_cluster().barrier_arrive();
   if (tid < N) {
     Node& nd = nodes[tid];
     nd.tok = my_tok;
@@ -809,6 +854,7 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
   int token = -1;  // drawn token, in the CTA that finds it (thread 0)
   float tprob = 0.0f;
   bool found = false, started = false;
+  uint32_t phase = 0;  // the barriers' parities, bit 2 par + kind
   while (status == RL_OK) {
     // ---- the node's rows and its children ----
     const Node& nd = nodes[node];
@@ -835,14 +881,12 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
       Part pp, pq;
       warp_parts(zp, cp, zq, cq, greedy, pp, pq);
       // every CTA of the cluster has started: its shared memory may be written
-      if (C > 1 && !started) cgx::this_cluster().barrier_wait();
+      if (!started) cgx::this_cluster().barrier_wait();
       if (lane < C) {
-        Part* to = C > 1 ? cl.map_shared_rank(&sh.part[par][0][0], lane) : &sh.part[par][0][0];
-        to[mypart] = pp;
-        if (with_q) to[kParts + mypart] = pq;
+        send(&sh.part[par][0][mypart], pp, &sh.bar[par][0], lane);
+        if (with_q) send(&sh.part[par][1][mypart], pq, &sh.bar[par][0], lane);
       }
     }
-    if (C > 1) cgx::this_cluster().barrier_arrive();
     if (!started) {  // meanwhile: the nodes' logits
       if (tid < n) {
         Node& me = nodes[tid];
@@ -856,16 +900,15 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
       __syncthreads();
       started = true;
     }
-    if (C > 1) cgx::this_cluster().barrier_wait();
-    else __syncthreads();
     // ---- joined by warp 0 of every CTA ----
     double wp[kPerLane];
     if (warp == 0) {
       Part P, Q;
+      const bool in = receive(&sh.bar[par][0], phase >> (2 * par) & 1u, static_cast<uint32_t>(np * sizeof(Part)) << (with_q ? 1 : 0));
       join_parts(sh.part[par][0], np, greedy, with_q, cp, cq, P, Q, wp);
       if (!with_q) Q.s = 1.0, Q.m = 0.0f;
       const float Fp = frame(P.m, cp), Fq = frame(Q.m, cq);
-      const bool good = P.s == P.s && fabsf(P.m) < RL_POS_INF && Q.s == Q.s && fabsf(Q.m) < RL_POS_INF;
+      const bool good = in && P.s == P.s && fabsf(P.m) < RL_POS_INF && Q.s == Q.s && fabsf(Q.m) < RL_POS_INF;
       // the children: their weights
       int nchild = 0;
       for (int i0 = good ? firstc : INT_MAX; i0 < n; i0 += 32) {
@@ -886,7 +929,7 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
         if (!tree) break;
       }
       if (lane == 0) {
-        sh.status = good ? RL_OK : RL_ERR_NONFINITE;
+        sh.status = good ? RL_OK : in ? RL_ERR_NONFINITE : RL_ERR_TIMEOUT;
         sh.Ps = P.s;
         sh.Qs = Q.s;
         sh.Pm = P.m;
@@ -900,6 +943,7 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
       }
       __syncwarp();
     }
+    phase ^= 1u << (2 * par);
     par ^= 1;
     bool sums = false;  // sh.w holds the parts' sums of w = max(p - C q, 0)
     float rhi = 0.0f, rlo = 0.0f;
@@ -960,23 +1004,26 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
       const float Pm = sh.Pm, Qm = sh.Qm, Fp = frame(Pm, cp), Fq = frame(Qm, cq);
       double s = sum_resid<Plain>(rp, rq, j0, j1, Resid{cp, cq, Pm, Qm, Fp, Fq, rhi, rlo});
       s = warp_sum_d(s);
-      if (lane < C) (C > 1 ? cl.map_shared_rank(&sh.w[par][0], lane) : &sh.w[par][0])[mypart] = s;
-      if (C > 1) cl.sync();
-      else __syncthreads();
+      if (lane < C) send(&sh.w[par][mypart], s, &sh.bar[par][1], lane);
       if (warp == 0) {
+        const bool in = receive(&sh.bar[par][1], phase >> (2 * par + 1) & 1u, static_cast<uint32_t>(np * sizeof(double)));
         double t = 0.0;
         for (int i = lane; i < np; i += 32) t += sh.w[par][i];
         t = warp_sum_d(t);
-        if (lane == 0) sh.S = t * sh.C / sh.Qs;  // as a probability
+        if (lane == 0) {
+          sh.S = t * sh.C / sh.Qs;  // as a probability
+          if (!in) sh.status = RL_ERR_TIMEOUT;
+        }
         __syncwarp();
       }
+      phase ^= 2u << (2 * par);
       par ^= 1;
       sums = true;
     }
     if (status != RL_OK) {
       // an empty row: once more without its mask, if that has no bit
-      const bool ep = rp.mask && sh.Pm == RL_NEG_INF && !any_bit(rp.mask, V);
-      const bool eq = with_q && rq.mask && sh.Qm == RL_NEG_INF && !any_bit(rq.mask, V);
+      const bool ep = status == RL_ERR_NONFINITE && rp.mask && sh.Pm == RL_NEG_INF && !any_bit(rp.mask, V);
+      const bool eq = status == RL_ERR_NONFINITE && with_q && rq.mask && sh.Qm == RL_NEG_INF && !any_bit(rq.mask, V);
       no_mask |= (ep ? 1 : 0) | (eq ? 2 : 0);
       if (!ep && !eq) break;
       status = RL_OK;
@@ -1058,9 +1105,10 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
         }
         __syncthreads();
       }
-      if (lane < C) (C > 1 ? cl.map_shared_rank(&sh.w[par][0], lane) : &sh.w[par][0])[mypart] = f;
-      if (C > 1) cl.sync();
-      else __syncthreads();
+      if (lane < C) send(&sh.w[par][mypart], f, &sh.bar[par][1], lane);
+      if (warp == 0 && !receive(&sh.bar[par][1], phase >> (2 * par + 1) & 1u, static_cast<uint32_t>(np * sizeof(double))) && lane == 0)
+        sh.status = RL_ERR_TIMEOUT;
+      phase ^= 2u << (2 * par);
       par ^= 1;
     }
     // ---- which part holds the drawn token ----
@@ -1074,6 +1122,8 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
       find_owner(sh, wp, np, du);
     }
     __syncthreads();
+    status = sh.status;
+    if (status != RL_OK) break;
     const int owner = sh.owner;
     if (owner >= 0 && owner / kVW == rank) {
       // ---- the drawn token inside that part, by the whole CTA: down to 4 ids a
@@ -1157,7 +1207,12 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
     }
     break;
   }
-  if (C > 1 && !started) cgx::this_cluster().barrier_wait();
+  if (!started) cgx::this_cluster().barrier_wait();
+  // behind a wait that ran out no CTA leaves while others may still write to it
+  if (status == RL_ERR_TIMEOUT) {
+    cgx::this_cluster().barrier_arrive();
+    cgx::this_cluster().barrier_wait();
+  }
   // ---- outputs ----
   if (found) {
     out_tok[acc] = token;
