@@ -19,10 +19,13 @@
 // again. A refusal with a draft row costs a second pass over the two rows
 // (from L2) for the sums of w.
 //
-// What bounds it is HBM for many rows and, for few, the dependent steps of the
-// walk. While the cluster joins its sums and decides, the rows of the node's
-// first child are fetched into L2; a pass then runs on L2, a warp's next chunk
-// loaded as soon as the registers of the last are free.
+// What bounds it is the dependent steps of the walk: loads of a pass, exchange,
+// join and accept test follow one another (for 512 ids a warp about 2400, 1000,
+// 2300 and 650 cycles), and the longest walk of a batch ends the call. While the
+// cluster joins its sums and decides, the rows of the node's first child are
+// fetched into L2; a pass then runs on L2, a warp's next chunk loaded as soon as
+// the registers of the last are free. 64 chains of 4 x 128256 f32 take 67 us, of
+// which HBM needs 27 for the rows that are looked at; one chain of 3 x 32000 10.
 //
 // Precision. A weight is 2^(x c - F): one FMA and ex2.approx, relative error
 // about 2^-22 with no bias that two ids would not share; c = log2(e) / T in
@@ -1300,9 +1303,9 @@ rl_status side_of(const rl_dist_rows* d, int V, int per_seq, VdSide* s) {
 // rows can be split: eight where they find room on the GPU at once (two CTAs an
 // SM), four where there are sequences enough, and at least 2048 ids a CTA,
 // below which the join costs more than it saves. us a call at 2 / 4 / 8 CTAs:
-// 64 x 4 x 128256 f32 100 / 72 / 80, 128 x 7 x 151936 bf16 180 / 116 / 123, 16
-// trees of 29 nodes x 128256 70 / 43 / 32, one chain of 3 x 32000 15.9 / 12.3 /
-// 12.3 (an earlier form at 16 CTAs: 142 where 4 took 81).
+// 64 x 4 x 128256 f32 88 / 67 / 73, 128 x 7 x 151936 bf16 178 / 111 / 111, 16
+// trees of 29 nodes x 128256 64 / 41 / 30, 24 masked chains of 5 x 32000 61 / 40 /
+// 34, one chain of 3 x 32000 13.9 / 10.9 / 10.2.
 int cluster_size(int B, int V) {
   int C = 1;
   while (C < kMaxCluster && (C < 4 || static_cast<int64_t>(B) * C * 2 <= 256) && V / (2 * C) >= 2048) C *= 2;
