@@ -572,6 +572,11 @@ class Sampler:
               "rl_grammar_greedy_host")
         return tok
 
+    def _on_device(self, who, dev):
+        """Refuses tensors that are not on the handle's device."""
+        if dev.type != "cuda" or dev.index != self.device:
+            raise ValueError(f"{who}: the tensors are on {dev}, the sampler on another device")
+
     # -- speculative decoding ---------------------------------------------------
     def specdec_sample(self, logits, temperature, offset, uniforms, stream=None):
         """rl_specdec_sample: SpeculativeDecoder::sample per row of device
@@ -625,6 +630,7 @@ class Sampler:
             raise _wrong(who, "draw_u", draw_u, f32, one, dev)
         if draft is not None and (draft.V != V or draft.device != dev):
             raise ValueError(f"{who}: the draft rows differ from the target rows in V or device")
+        self._on_device(who, dev)
         t, d = target._of(B, who), draft._of(B, who) if draft is not None else None
         acc, st = torch.empty_like(n_draft), torch.empty_like(n_draft)
         tok, prob = drafts.new_empty((B, K + 1)), accept_u.new_empty((B, K + 1))
@@ -659,6 +665,7 @@ class Sampler:
             raise _wrong(who, "draw_u", draw_u, f32, one, dev)
         if draft is not None and (draft.V != V or draft.device != dev):
             raise ValueError(f"{who}: the draft rows differ from the target rows in V or device")
+        self._on_device(who, dev)
         t, d = target._of(B, who), draft._of(B, who) if draft is not None else None
         acc, st = torch.empty_like(n_node), torch.empty_like(n_node)
         path, tok, prob = torch.empty_like(tokens), torch.empty_like(tokens), torch.empty_like(accept_u)
@@ -741,6 +748,7 @@ class Sampler:
         if group not in (32, 64, 128) or H % 64 or H % group:
             raise ValueError("lmhead_q4_quantize: group must be 32, 64 or 128, H a multiple of it and of 64")
         dev = weight.device
+        self._on_device("lmhead_q4_quantize", dev)
         q = torch.empty(V, H // 2, dtype=torch.uint8, device=dev)
         scale = torch.empty(V, H // group, dtype=torch.bfloat16, device=dev)
         w = Q4Weight(q, scale, group)
@@ -749,8 +757,7 @@ class Sampler:
               "rl_lmhead_q4_quantize")
         return w
 
-    @staticmethod
-    def _q4_operands(hidden, weight):
+    def _q4_operands(self, hidden, weight):
         import torch
 
         if hidden.dtype is not torch.bfloat16 or hidden.dim() != 2 or hidden.stride(1) != 1:
@@ -758,6 +765,7 @@ class Sampler:
         B, H = hidden.shape
         if H != weight.H or hidden.device != weight.device:
             raise ValueError(f"lmhead_q4: hidden has {H} columns on {hidden.device}, weight {weight.H} on {weight.device}")
+        self._on_device("lmhead_q4", hidden.device)
         return B, H, hidden.stride(0) if B > 1 else max(hidden.stride(0), H)
 
     @staticmethod

@@ -32,6 +32,24 @@ def test_refusals_before_any_device_work():
         engine.SpeculativeStep(100, 4, rlsampler.VERIFY_MAX_NODES)
 
 
+def test_tensors_on_another_device_are_refused():
+    s = rlsampler.Sampler.__new__(rlsampler.Sampler)
+    s.h, s.device = None, 0
+    i32, f32, bf16 = torch.int32, torch.float32, torch.bfloat16
+    n, du = torch.zeros(2, dtype=i32), torch.zeros(2)
+    with pytest.raises(ValueError, match="on cpu"):
+        s.specdec_verify_draft(rlsampler.DistRows(torch.zeros(8, 40)), torch.zeros(2, 3, dtype=i32), n, torch.zeros(2, 3), du)
+    with pytest.raises(ValueError, match="on cpu"):
+        s.specdec_verify_tree(rlsampler.DistRows(torch.zeros(6, 40)), torch.zeros(2, 3, dtype=i32), torch.zeros(2, 3, dtype=i32), n,
+                              torch.zeros(2, 3, dtype=f32), du)
+    w = rlsampler.Q4Weight(torch.zeros(6, 64, dtype=torch.uint8), torch.zeros(6, 2, dtype=bf16), 64)
+    x = torch.zeros(2, 128, dtype=bf16)
+    for call in (lambda: s.lmhead_q4_logits(x, w), lambda: s.lmhead_q4_greedy(x, w), lambda: s.lmhead_q4_sample(x, w, n, du),
+                 lambda: s.lmhead_q4_quantize(torch.zeros(6, 128, dtype=bf16), 64)):
+        with pytest.raises(ValueError, match="on cpu"):
+            call()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("given", [False, True])
 def test_draft_head_target_head_verify(given):
