@@ -103,12 +103,18 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
       : "memory");
 }
 
+// a & b | c in one instruction (two immediates would make it two).
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
 // Eight codes of a word as bf16 code - 8, in element order.
 __device__ __forceinline__ void expand(uint32_t w, uint32_t* out) {
   const __nv_bfloat162 c136 = __halves2bfloat162(__ushort_as_bfloat16(0x4308), __ushort_as_bfloat16(0x4308));
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const uint32_t x = ((w >> (4 * j)) & 0x000f000fu) | 0x43004300u;  // 128 + code
+    const uint32_t x = and_or(w >> (4 * j), 0x000f000fu, 0x43004300u);  // 128 + code
     __nv_bfloat162 v;
     *reinterpret_cast<uint32_t*>(&v) = x;
     v = __hsub2(v, c136);
@@ -567,8 +573,8 @@ __device__ __forceinline__ __half2 bits_h2(uint32_t v) { return *reinterpret_cas
 // f16 code - 8: 0x6400 | code is 1024 + code, with the code four bits up
 // 1024 + 16 code.
 __device__ __forceinline__ void expand_h(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  lo = h2_bits(__hsub2(bits_h2((w & 0x000f000fu) | 0x64006400u), bits_h2(0x64086408u)));
-  hi = h2_bits(__hfma2(bits_h2((w & 0x00f000f0u) | 0x64006400u), bits_h2(0x2c002c00u), bits_h2(0xd480d480u)));
+  lo = h2_bits(__hsub2(bits_h2(and_or(w, 0x000f000fu, 0x64006400u)), bits_h2(0x64086408u)));
+  hi = h2_bits(__hfma2(bits_h2(and_or(w, 0x00f000f0u, 0x64006400u)), bits_h2(0x2c002c00u), bits_h2(0xd480d480u)));
 }
 
 // D = A B + C: 16 x 8 f32, A 16 x 16 and B 16 x 8 f16.
