@@ -39,8 +39,8 @@
 //
 // Bound: HBM, half a byte a weight, up to about 100 batch rows; beside it the
 // expansion, 9 (f16) or 11 (bf16) instructions for 8 weights, and for more rows
-// the hand-overs and N / group FMAs a weight. H 4096, V 128256: 63 us for one row
-// (HBM needs 42), 101 for 12 (43), 150 for 128 (the MMAs need 81). Every wait is
+// the hand-overs and N / group FMAs a weight. H 4096, V 128256: 52 us for one row
+// (HBM needs 42), 94 for 12 (43), 147 for 128 (the MMAs need 81). Every wait is
 // bounded; where one runs out the error flag is set, copies in flight land and
 // TMEM is freed.
 #include <cuda_bf16.h>
@@ -1030,8 +1030,8 @@ cudaError_t few_run(const CUtensorMap& mq, const FewArgs& a, int group, size_t s
 
 // Up to 16 batch rows, where the hidden states fit shared memory beside the rings
 // (H <= 8192 at 8 batch rows, 4096 at 16). us a call, few rows' kernel / the
-// tensor cores' roles: 1 x 4096 x 128256 64 / 103, 12 rows of it 102 / 113, 1 x
-// 2048 x 32000 15 / 19; behind 16 rows it would load each code again for every 16.
+// tensor cores' roles: 1 x 4096 x 128256 52 / 94, 12 rows of it 94 / 104, 1 x
+// 2048 x 32000 14 / 18; behind 16 rows it would load each code again for every 16.
 size_t few_hidden(int B, int H) { return static_cast<size_t>(B <= 8 ? 8 : 16) * ((H + 255) / 256) * 512; }
 bool is_few(int B, int H) { return B <= 16 && few_hidden(B, H) <= kFewHidden; }
 
