@@ -30,9 +30,9 @@
 // Precision. A weight is 2^(x c - F): one FMA and ex2.approx, relative error
 // about 2^-22 with no bias that two ids would not share; c = log2(e) / T in
 // single precision tilts a row by at most 2^-25 |t|. A lane's F is the product
-// x c of the first logit it sees, moved only where a later logit lies 64
-// binades above: any F does, as long as the sums are joined with it, and no
-// maximum has to be found. Sums are doubles, and draws are compared in
+// max c of the first logits it sees, so that what weighs most has a short
+// exponent, and is moved only where a later logit lies 64 binades above: any F
+// does, as long as the sums are joined with it. Sums are doubles, and draws are compared in
 // doubles: a token can differ from the exact one only where the draw lies
 // within about 1e-8 of a border.
 #include <cooperative_groups.h>
@@ -300,8 +300,8 @@ __device__ __forceinline__ void see_max(Seen& z, const float (&x)[4][4], int j0)
 }
 
 __device__ __forceinline__ void see(Seen& z, const float (&x)[4][4], float c) {
-  if (!(z.m > RL_NEG_INF)) {  // nothing seen yet: the first logit's frame
-    z.m = x[0][0];
+  if (!(z.m > RL_NEG_INF)) {  // nothing seen yet
+    z.m = max16(x);
     z.F = frame(z.m, c);
   }
   float e[4];
