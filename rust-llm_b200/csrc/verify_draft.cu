@@ -355,17 +355,15 @@ __device__ __forceinline__ void warp_parts(const Seen& a, float ca, const Seen& 
   pb.s = sb;
 }
 
-// Warp 0 joins the parts of both sides: their sums relative to the largest m;
-// the lane's own parts' sums of the target relative to it in w.
+// Warp 0 joins the parts of both sides: their sums relative to the largest m.
 __device__ __forceinline__ void join_parts(const Part* parts, int np, bool greedy, bool with_q, float cp, float cq, Part& P,
-                                           Part& Q, double (&w)[kPerLane]) {
+                                           Part& Q) {
   const int lane = threadIdx.x & 31;
   const int per = (np + 31) >> 5;
   Part a[kPerLane], b[kPerLane];
   float ma = RL_NEG_INF, mb = RL_NEG_INF;
 #pragma unroll
   for (int k = 0; k < kPerLane; ++k) {
-    w[k] = 0.0;
     if (k >= per) continue;
     const int i = lane * per + k;
     a[k].s = b[k].s = 0.0;
@@ -389,8 +387,7 @@ __device__ __forceinline__ void join_parts(const Part* parts, int np, bool greed
     if (a[k].m == P.m) id = min(id, static_cast<unsigned>(a[k].id));
     const float fa = greedy ? 1.0f : a[k].m > RL_NEG_INF ? rebase(a[k].m, frame(a[k].m, cp), P.m, Ga, cp) : 0.0f;
     const float fb = b[k].m > RL_NEG_INF ? rebase(b[k].m, frame(b[k].m, cq), Q.m, Gb, cq) : 0.0f;
-    w[k] = a[k].s == a[k].s ? a[k].s * static_cast<double>(fa) : a[k].s;
-    sa += w[k];
+    sa += a[k].s == a[k].s ? a[k].s * static_cast<double>(fa) : a[k].s;
     sb += b[k].s == b[k].s ? b[k].s * static_cast<double>(fb) : b[k].s;
   }
   P.id = static_cast<int>(__reduce_min_sync(0xffffffffu, id));
@@ -635,42 +632,87 @@ __device__ __noinline__ Seen2 see_rows(Row<TP> rp, Row<TQ> rq, int j0, int j1, f
                   [&](int, const float (&y)[4][4]) { see(zq, y, cq); });
   return {zp, zq};
 }
-// The frames and factors of w = max(p rho - q, 0).
-struct Resid {
-  float cp, cq, Pm, Qm, Fp, Fq, rhi, rlo;
+// What a draw is decided on: the frames and factors of w = max(p rho - q, 0), or
+// of p alone. Ids within 6 binades of the frames' logits, which are few, are
+// weighed in doubles: nearly all of the error of a running sum comes from them
+// (150 thousand normal logits of deviation 3: 3 to 6e-9 of the whole without,
+// 0.3 to 1e-9 with).
+struct Side {
+  float c, m, F, heavy;  // heavy: logits from here on
+  double cd, r;          // log2(e) / T, and how far m's exponent is from its frame
 };
-// A lane's sum of w over its part.
+struct Resid {
+  Side p, q;
+  double rho;
+  float rhi, rlo;
+};
+__device__ __forceinline__ Side side(float c, float m, float T, bool plain_T) {
+  Side f;
+  f.c = c;
+  f.m = m;
+  f.F = frame(m, c);
+  f.heavy = m - 3.0f / c;
+  f.cd = fmin(fmax(1.4426950408889634074 / static_cast<double>(plain_T ? 1.0f : T), 1e-30), 3e38);
+  f.r = is_near(f.F) ? static_cast<double>(__fmaf_rn(m, c, -f.F)) : 0.0;
+  return f;
+}
+__device__ __noinline__ double weight_d(float x, float m, double c, double r) {
+  return exp2((static_cast<double>(x) - static_cast<double>(m)) * c + r);
+}
+__device__ __forceinline__ double weight_d(float x, const Side& f) { return weight_d(x, f.m, f.cd, f.r); }
+__device__ __forceinline__ float resid_w(float ep, float eq, const Resid& f) {
+  return fmaxf(__fmaf_rn(ep, f.rhi, __fmaf_rn(ep, f.rlo, -eq)), 0.0f);
+}
+__device__ __forceinline__ float weight(float x, const Side& f) { return weight(x, f.m, f.c, f.F); }
+// The weight of one id.
+__device__ __forceinline__ double one_weight(float x, const Side& f) {
+  return x >= f.heavy ? weight_d(x, f) : static_cast<double>(weight(x, f));
+}
+__device__ __forceinline__ double one_weight(float x, float y, const Resid& f) {
+  if (x >= f.p.heavy || y >= f.q.heavy) return fmax(weight_d(x, f.p) * f.rho - weight_d(y, f.q), 0.0);
+  return static_cast<double>(resid_w(weight(x, f.p), weight(y, f.q), f));
+}
+__device__ __forceinline__ float pick16(const float (&x)[4][4], int i) {
+  float v = x[0][0];
+#pragma unroll
+  for (int k = 1; k < 16; ++k) v = i == k ? x[k >> 2][k & 3] : v;
+  return v;
+}
+// A lane's sum of w over ids [j0, j1).
 template <bool Plain, typename TP, typename TQ>
 __device__ __noinline__ double sum_resid(Row<TP> rp, Row<TQ> rq, int j0, int j1, Resid f) {
   double s = 0.0;
   pass_both<Plain>(rp, rq, j0, j1, [&](const float (&x)[4][4], const float (&y)[4][4]) {
     float w = 0.0f;
-    if (is_near(f.Fp) && is_near(f.Fq)) {
+    if (is_near(f.p.F) && is_near(f.q.F)) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         float v[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float ep = weight(x[i][k], f.cp, f.Fp), eq = weight(y[i][k], f.cq, f.Fq);
-          v[k] = fmaxf(__fmaf_rn(ep, f.rhi, __fmaf_rn(ep, f.rlo, -eq)), 0.0f);
-        }
+        for (int k = 0; k < 4; ++k) v[k] = resid_w(weight(x[i][k], f.p.c, f.p.F), weight(y[i][k], f.q.c, f.q.F), f);
         w += (v[0] + v[1]) + (v[2] + v[3]);
       }
     } else {
 #pragma unroll
-      for (int k = 0; k < 16; ++k) {
-        const float ep = weight(x[k >> 2][k & 3], f.Pm, f.cp, f.Fp), eq = weight(y[k >> 2][k & 3], f.Qm, f.cq, f.Fq);
-        w += fmaxf(__fmaf_rn(ep, f.rhi, __fmaf_rn(ep, f.rlo, -eq)), 0.0f);
-      }
+      for (int k = 0; k < 16; ++k) w += resid_w(weight(x[k >> 2][k & 3], f.p), weight(y[k >> 2][k & 3], f.q), f);
     }
     s += static_cast<double>(w);
+    if (max16(x) >= f.p.heavy || max16(y) >= f.q.heavy) {
+      unsigned hv = 0;
+#pragma unroll
+      for (int k = 0; k < 16; ++k)
+        if (x[k >> 2][k & 3] >= f.p.heavy || y[k >> 2][k & 3] >= f.q.heavy) hv |= 1u << k;
+      for (; hv; hv &= hv - 1) {
+        const float a = pick16(x, __ffs(hv) - 1), b = pick16(y, __ffs(hv) - 1);
+        s += one_weight(a, b, f) - static_cast<double>(resid_w(weight(a, f.p), weight(b, f.q), f));
+      }
+    }
   });
   return s;
 }
-// A lane's sum of p over its part without the refused given tokens.
+// A lane's sum of p over ids [j0, j1) without the refused given tokens.
 template <bool Plain, typename T>
-__device__ __noinline__ double sum_kept(Row<T> r, int j0, int j1, float c, float m, float F, const Ctl* sh, const Node* nodes,
-                                        int nrem) {
+__device__ __noinline__ double sum_kept(Row<T> r, int j0, int j1, Side f, const Ctl* sh, const Node* nodes, int nrem) {
   double s = 0.0;
   const int lane = threadIdx.x & 31;
   pass<Plain>(r, j0, j1, [&](int c0, float (&x)[4][4]) {
@@ -684,8 +726,18 @@ __device__ __noinline__ double sum_kept(Row<T> r, int j0, int j1, float c, float
     }
     float w = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) w += weight(x[i >> 2][i & 3], m, c, F);
+    for (int i = 0; i < 16; ++i) w += weight(x[i >> 2][i & 3], f);
     s += static_cast<double>(w);
+    if (max16(x) >= f.heavy) {
+      unsigned hv = 0;
+#pragma unroll
+      for (int k = 0; k < 16; ++k)
+        if (x[k >> 2][k & 3] >= f.heavy) hv |= 1u << k;
+      for (; hv; hv &= hv - 1) {
+        const float a = pick16(x, __ffs(hv) - 1);
+        s += weight_d(a, f) - static_cast<double>(weight(a, f));
+      }
+    }
   });
   return s;
 }
@@ -904,11 +956,10 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
       started = true;
     }
     // ---- joined by warp 0 of every CTA ----
-    double wp[kPerLane];
     if (warp == 0) {
       Part P, Q;
       const bool in = receive(&sh.bar[par][0], phase >> (2 * par) & 1u, static_cast<uint32_t>(np * sizeof(Part)) << (with_q ? 1 : 0));
-      join_parts(sh.part[par][0], np, greedy, with_q, cp, cq, P, Q, wp);
+      join_parts(sh.part[par][0], np, greedy, with_q, cp, cq, P, Q);
       if (!with_q) Q.s = 1.0, Q.m = 0.0f;
       const float Fp = frame(P.m, cp), Fq = frame(Q.m, cq);
       const bool good = in && P.s == P.s && fabsf(P.m) < RL_POS_INF && Q.s == Q.s && fabsf(Q.m) < RL_POS_INF;
@@ -949,7 +1000,7 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
     phase ^= 1u << (2 * par);
     par ^= 1;
     bool sums = false;  // sh.w holds the parts' sums of w = max(p - C q, 0)
-    float rhi = 0.0f, rlo = 0.0f;
+    Resid rs = {};
     int next = kNone;
     while (true) {
       // ---- accept tests: thread 0 of every CTA, all alike; both sides of a
@@ -1001,11 +1052,12 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
       next = sh.next;
       if (status != RL_OK || next != kSums) break;
       // ---- sums of w = max(p - C q, 0) over the parts ----
-      const double rho = sh.Qs / (sh.C * sh.Ps);
-      rhi = static_cast<float>(rho);
-      rlo = static_cast<float>(rho - static_cast<double>(rhi));
-      const float Pm = sh.Pm, Qm = sh.Qm, Fp = frame(Pm, cp), Fq = frame(Qm, cq);
-      double s = sum_resid<Plain>(rp, rq, j0, j1, Resid{cp, cq, Pm, Qm, Fp, Fq, rhi, rlo});
+      rs.rho = sh.Qs / (sh.C * sh.Ps);
+      rs.rhi = static_cast<float>(rs.rho);
+      rs.rlo = static_cast<float>(rs.rho - static_cast<double>(rs.rhi));
+      rs.p = side(cp, sh.Pm, Tp, greedy);
+      rs.q = side(cq, sh.Qm, Tq, !drawn);
+      double s = sum_resid<Plain>(rp, rq, j0, j1, rs);
       s = warp_sum_d(s);
       if (lane < C) send(&sh.w[par][mypart], s, &sh.bar[par][1], lane);
       if (warp == 0) {
@@ -1056,58 +1108,32 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
     }
     const bool resid = sums && sh.S > 0.0;  // else all of w rounded away: from p
     const int nrem = sh.nremoved;
-    const float Pm = sh.Pm, Qm = sh.Qm, Fp = frame(Pm, cp), Fq = frame(Qm, cq);
-    // The weights w of ids j .. j + 3: max(p rho - q, 0) in units of q's
-    // largest, or p without the refused given tokens in units of p's largest.
-    const auto w4 = [&](int j, int end, float (&w)[4]) {
-      float x[4];
+    if (!resid) rs.p = side(cp, sh.Pm, Tp, greedy);
+    // The weights w of ids j .. j + 3: max(p rho - q, 0) in units of q's frame,
+    // or p without the refused given tokens in units of p's.
+    const auto w4 = [&](int j, int end, double (&w)[4]) {
+      float x[4], y[4];
       unit_guarded(rp.x, j, end, x);
+      if (resid) unit_guarded(rq.x, j, end, y);
       keep4(rp, j, rp.mask ? bits4(rp.mask, j, end) : 0u, x);
-      if (resid) {
-        float y[4];
-        unit_guarded(rq.x, j, end, y);
-        keep4(rq, j, rq.mask ? bits4(rq.mask, j, end) : 0u, y);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float ep = weight(x[k], Pm, cp, Fp), eq = weight(y[k], Qm, cq, Fq);
-          w[k] = fmaxf(__fmaf_rn(ep, rhi, __fmaf_rn(ep, rlo, -eq)), 0.0f);
-        }
-      } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          w[k] = weight(x[k], Pm, cp, Fp);
-          if (nrem > 0 && is_removed(sh, nodes, nrem, j + k)) w[k] = 0.0f;
-        }
+      if (resid) keep4(rq, j, rq.mask ? bits4(rq.mask, j, end) : 0u, y);
+#pragma unroll 1
+      for (int k = 0; k < 4; ++k) {
+        const float a = k == 0 ? x[0] : k == 1 ? x[1] : k == 2 ? x[2] : x[3];
+        double v;
+        if (resid) v = one_weight(a, k == 0 ? y[0] : k == 1 ? y[1] : k == 2 ? y[2] : y[3], rs);
+        else v = nrem > 0 && is_removed(sh, nodes, nrem, j + k) ? 0.0 : one_weight(a, rs.p);
+        if (k == 0) w[0] = v;
+        else if (k == 1) w[1] = v;
+        else if (k == 2) w[2] = v;
+        else w[3] = v;
       }
     };
-    if (!resid && nrem > 0) {
-      // the parts that hold refused given tokens sum again (taking a weight
-      // off a sum would leave its rounding), each by all warps of its CTA
-      const Part me = sh.part[par ^ 1][0][mypart];
-      double f = me.m > RL_NEG_INF ? me.s * static_cast<double>(rebase(me.m, frame(me.m, cp), Pm, Fp, cp)) : 0.0;
-      unsigned again = 0;  // this CTA's parts that do
-      const int64_t cta0 = static_cast<int64_t>(rank) * kVW * a.part;
-      for (int k = lane; k < nrem; k += 32) {
-        const int64_t t = nodes[sh.removed[k]].tok - cta0;
-        if (t >= 0 && t < static_cast<int64_t>(kVW) * a.part) again |= 1u << (static_cast<int>(t) / a.part);
-      }
-      again = __reduce_or_sync(0xffffffffu, again);
-      for (; again; again &= again - 1) {
-        const int w = __ffs(again) - 1;
-        const int w0 = static_cast<int>(min(cta0 + static_cast<int64_t>(w) * a.part, static_cast<int64_t>(V)));
-        const int w1 = static_cast<int>(min(static_cast<int64_t>(w0) + a.part, static_cast<int64_t>(V)));
-        const int chunks = (w1 - w0 + kChunk - 1) / kChunk;
-        const int s0 = w0 + chunks * warp / kVW * kChunk, s1 = min(w0 + chunks * (warp + 1) / kVW * kChunk, w1);
-        double s = 0.0;
-        if (s0 < s1) s = warp_sum_d(sum_kept<Plain>(rp, s0, s1, cp, Pm, Fp, &sh, nodes, nrem));
-        if (lane == 0) sh.scan[warp] = s;
-        __syncthreads();
-        if (warp == w) {
-          f = 0.0;
-          for (int i = 0; i < kVW; ++i) f += sh.scan[i];
-        }
-        __syncthreads();
-      }
+    if (!resid) {
+      // the parts' sums once more, without refused given tokens (taking a weight
+      // off a sum would leave its rounding) and with the heavy ids' exact weights
+      double f = 0.0;
+      if (j0 < j1) f = warp_sum_d(sum_kept<Plain>(rp, j0, j1, rs.p, &sh, nodes, nrem));
       if (lane < C) send(&sh.w[par][mypart], f, &sh.bar[par][1], lane);
       if (warp == 0 && !receive(&sh.bar[par][1], phase >> (2 * par + 1) & 1u, static_cast<uint32_t>(np * sizeof(double))) && lane == 0)
         sh.status = RL_ERR_TIMEOUT;
@@ -1116,12 +1142,10 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
     }
     // ---- which part holds the drawn token ----
     if (warp == 0) {
-      if (resid || nrem > 0) {
-        const int per = (np + 31) >> 5;
+      const int per = (np + 31) >> 5;
+      double wp[kPerLane];
 #pragma unroll
-        for (int k = 0; k < kPerLane; ++k)
-          wp[k] = k < per && lane * per + k < np ? sh.w[par ^ 1][lane * per + k] : 0.0;
-      }
+      for (int k = 0; k < kPerLane; ++k) wp[k] = k < per && lane * per + k < np ? sh.w[par ^ 1][lane * per + k] : 0.0;
       find_owner(sh, wp, np, du);
     }
     __syncthreads();
@@ -1140,8 +1164,7 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
         const int s0 = share(warp), s1 = share(warp + 1);
         double s = 0.0;
         if (s0 < s1)
-          s = warp_sum_d(resid ? sum_resid<Plain>(rp, rq, s0, s1, Resid{cp, cq, Pm, Qm, Fp, Fq, rhi, rlo})
-                               : sum_kept<Plain>(rp, s0, s1, cp, Pm, Fp, &sh, nodes, nrem));
+          s = warp_sum_d(resid ? sum_resid<Plain>(rp, rq, s0, s1, rs) : sum_kept<Plain>(rp, s0, s1, rs.p, &sh, nodes, nrem));
         if (lane == 0) sh.scan[warp] = s;
         __syncthreads();
         int pick = 0;
@@ -1161,14 +1184,14 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
         __syncthreads();
       }
       const int a0 = w0 + 4 * tid;
-      float w[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      double w[4] = {0.0, 0.0, 0.0, 0.0};
       if (a0 < w1) w4(a0, w1, w);
       double s = 0.0;
       int last = -1;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        s += static_cast<double>(w[k]);
-        if (w[k] > 0.0f) last = a0 + k;
+        s += w[k];
+        if (w[k] > 0.0) last = a0 + k;
       }
       double incl = s;
 #pragma unroll
@@ -1184,8 +1207,8 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
         bool hit = false;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          run += static_cast<double>(w[k]);
-          if (!hit && w[k] > 0.0f && run > rest) {
+          run += w[k];
+          if (!hit && w[k] > 0.0 && run > rest) {
             atomicMin(&sh.at, a0 + k);
             hit = true;
           }
@@ -1202,7 +1225,7 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
       }
       if (tid == 0) {
         token = sh.at;
-        if (token >= 0) tprob = static_cast<float>(weight_2(to_f(rp.x[token]), Pm, cp, Fp) / sh.Ps);
+        if (token >= 0) tprob = static_cast<float>(weight_2(to_f(rp.x[token]), sh.Pm, cp, frame(sh.Pm, cp)) / sh.Ps);
         found = true;
       }
     } else if (owner < 0 && rank == 0 && tid == 0) {
