@@ -249,9 +249,25 @@ struct Node {
   uint8_t bit[2];      // the token's mask bits in its parent's rows
 };
 
+// What a draw is decided on: the frames and factors of w = max(p rho - q, 0), or
+// of p alone. Ids within 6 binades of the frames' logits, which are few, are
+// weighed in doubles: nearly all of the error of a running sum comes from them
+// (150 thousand normal logits of deviation 3: 3 to 6e-9 of the whole without,
+// 0.3 to 1e-9 with).
+struct Side {
+  float c, m, F, heavy;  // heavy: logits from here on
+  double cd, r;          // log2(e) / T, and how far m's exponent is from its frame
+};
+struct Resid {
+  Side p, q;
+  double rho;
+  float rhi, rlo;
+};
 struct Ctl {
   Part part[2][2][kParts];  // [parity][side]: every CTA's warps write into every CTA
   double w[2][kParts];      // [parity] the parts' sums of w
+  Resid rs;
+  double cd[2];             // log2(e) / T of both sides
   uint64_t bar[2][2];       // [parity][0 parts, 1 sums of w]: what is to come has come
   double scan[kVW];
   double rest;              // draw target inside the draw's part
@@ -632,27 +648,17 @@ __device__ __noinline__ Seen2 see_rows(Row<TP> rp, Row<TQ> rq, int j0, int j1, f
                   [&](int, const float (&y)[4][4]) { see(zq, y, cq); });
   return {zp, zq};
 }
-// What a draw is decided on: the frames and factors of w = max(p rho - q, 0), or
-// of p alone. Ids within 6 binades of the frames' logits, which are few, are
-// weighed in doubles: nearly all of the error of a running sum comes from them
-// (150 thousand normal logits of deviation 3: 3 to 6e-9 of the whole without,
-// 0.3 to 1e-9 with).
-struct Side {
-  float c, m, F, heavy;  // heavy: logits from here on
-  double cd, r;          // log2(e) / T, and how far m's exponent is from its frame
-};
-struct Resid {
-  Side p, q;
-  double rho;
-  float rhi, rlo;
-};
-__device__ __forceinline__ Side side(float c, float m, float T, bool plain_T) {
+// log2(e) / T in doubles.
+__device__ __forceinline__ double scale_d(float T) {
+  return fmin(fmax(1.4426950408889634074 / static_cast<double>(T), 1e-30), 3e38);
+}
+__device__ __forceinline__ Side side(float c, double cd, float m) {
   Side f;
   f.c = c;
   f.m = m;
   f.F = frame(m, c);
-  f.heavy = m - 3.0f / c;
-  f.cd = fmin(fmax(1.4426950408889634074 / static_cast<double>(plain_T ? 1.0f : T), 1e-30), 3e38);
+  f.heavy = m - __fdividef(3.0f, c);
+  f.cd = cd;
   f.r = is_near(f.F) ? static_cast<double>(__fmaf_rn(m, c, -f.F)) : 0.0;
   return f;
 }
@@ -680,7 +686,8 @@ __device__ __forceinline__ float pick16(const float (&x)[4][4], int i) {
 }
 // A lane's sum of w over ids [j0, j1).
 template <bool Plain, typename TP, typename TQ>
-__device__ __noinline__ double sum_resid(Row<TP> rp, Row<TQ> rq, int j0, int j1, Resid f) {
+__device__ __noinline__ double sum_resid(Row<TP> rp, Row<TQ> rq, int j0, int j1, const Resid* of) {
+  const Resid f = *of;
   double s = 0.0;
   pass_both<Plain>(rp, rq, j0, j1, [&](const float (&x)[4][4], const float (&y)[4][4]) {
     float w = 0.0f;
@@ -712,7 +719,8 @@ __device__ __noinline__ double sum_resid(Row<TP> rp, Row<TQ> rq, int j0, int j1,
 }
 // A lane's sum of p over ids [j0, j1) without the refused given tokens.
 template <bool Plain, typename T>
-__device__ __noinline__ double sum_kept(Row<T> r, int j0, int j1, Side f, const Ctl* sh, const Node* nodes, int nrem) {
+__device__ __noinline__ double sum_kept(Row<T> r, int j0, int j1, const Ctl* sh, const Node* nodes, int nrem) {
+  const Side f = sh->rs.p;
   double s = 0.0;
   const int lane = threadIdx.x & 31;
   pass<Plain>(r, j0, j1, [&](int c0, float (&x)[4][4]) {
@@ -886,6 +894,8 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
     for (int i = 0; i < 4; ++i) mbar_init(&sh.bar[i >> 1][i & 1], 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if (tid == kVT - 1) sh.cd[0] = scale_d(greedy ? 1.0f : Tp);
+  if (tid == kVT - 33) sh.cd[1] = scale_d(drawn ? Tq : 1.0f);
   cgx::this_cluster().barrier_arrive();
   if (tid < N) {
     Node& nd = nodes[tid];
@@ -1000,7 +1010,6 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
     phase ^= 1u << (2 * par);
     par ^= 1;
     bool sums = false;  // sh.w holds the parts' sums of w = max(p - C q, 0)
-    Resid rs = {};
     int next = kNone;
     while (true) {
       // ---- accept tests: thread 0 of every CTA, all alike; both sides of a
@@ -1043,6 +1052,14 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
           }
         }
         if (nx == kNone && sh.nremoved > 0) nx = kRefresh;
+        if (nx == kSums) {
+          const double rho = sh.Qs / (sh.C * sh.Ps);
+          sh.rs.rho = rho;
+          sh.rs.rhi = static_cast<float>(rho);
+          sh.rs.rlo = static_cast<float>(rho - static_cast<double>(sh.rs.rhi));
+          sh.rs.q = side(cq, sh.cd[1], sh.Qm);
+        }
+        if (nx < 0 && !greedy) sh.rs.p = side(cp, sh.cd[0], sh.Pm);
         sh.S = S;
         sh.k = k;
         sh.next = nx;
@@ -1052,12 +1069,7 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
       next = sh.next;
       if (status != RL_OK || next != kSums) break;
       // ---- sums of w = max(p - C q, 0) over the parts ----
-      rs.rho = sh.Qs / (sh.C * sh.Ps);
-      rs.rhi = static_cast<float>(rs.rho);
-      rs.rlo = static_cast<float>(rs.rho - static_cast<double>(rs.rhi));
-      rs.p = side(cp, sh.Pm, Tp, greedy);
-      rs.q = side(cq, sh.Qm, Tq, !drawn);
-      double s = sum_resid<Plain>(rp, rq, j0, j1, rs);
+      double s = sum_resid<Plain>(rp, rq, j0, j1, &sh.rs);
       s = warp_sum_d(s);
       if (lane < C) send(&sh.w[par][mypart], s, &sh.bar[par][1], lane);
       if (warp == 0) {
@@ -1108,7 +1120,6 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
     }
     const bool resid = sums && sh.S > 0.0;  // else all of w rounded away: from p
     const int nrem = sh.nremoved;
-    if (!resid) rs.p = side(cp, sh.Pm, Tp, greedy);
     // The weights w of ids j .. j + 3: max(p rho - q, 0) in units of q's frame,
     // or p without the refused given tokens in units of p's.
     const auto w4 = [&](int j, int end, double (&w)[4]) {
@@ -1121,8 +1132,8 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
       for (int k = 0; k < 4; ++k) {
         const float a = k == 0 ? x[0] : k == 1 ? x[1] : k == 2 ? x[2] : x[3];
         double v;
-        if (resid) v = one_weight(a, k == 0 ? y[0] : k == 1 ? y[1] : k == 2 ? y[2] : y[3], rs);
-        else v = nrem > 0 && is_removed(sh, nodes, nrem, j + k) ? 0.0 : one_weight(a, rs.p);
+        if (resid) v = one_weight(a, k == 0 ? y[0] : k == 1 ? y[1] : k == 2 ? y[2] : y[3], sh.rs);
+        else v = nrem > 0 && is_removed(sh, nodes, nrem, j + k) ? 0.0 : one_weight(a, sh.rs.p);
         if (k == 0) w[0] = v;
         else if (k == 1) w[1] = v;
         else if (k == 2) w[2] = v;
@@ -1133,7 +1144,7 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
       // the parts' sums once more, without refused given tokens (taking a weight
       // off a sum would leave its rounding) and with the heavy ids' exact weights
       double f = 0.0;
-      if (j0 < j1) f = warp_sum_d(sum_kept<Plain>(rp, j0, j1, rs.p, &sh, nodes, nrem));
+      if (j0 < j1) f = warp_sum_d(sum_kept<Plain>(rp, j0, j1, &sh, nodes, nrem));
       if (lane < C) send(&sh.w[par][mypart], f, &sh.bar[par][1], lane);
       if (warp == 0 && !receive(&sh.bar[par][1], phase >> (2 * par + 1) & 1u, static_cast<uint32_t>(np * sizeof(double))) && lane == 0)
         sh.status = RL_ERR_TIMEOUT;
@@ -1164,7 +1175,7 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
         const int s0 = share(warp), s1 = share(warp + 1);
         double s = 0.0;
         if (s0 < s1)
-          s = warp_sum_d(resid ? sum_resid<Plain>(rp, rq, s0, s1, rs) : sum_kept<Plain>(rp, s0, s1, rs.p, &sh, nodes, nrem));
+          s = warp_sum_d(resid ? sum_resid<Plain>(rp, rq, s0, s1, &sh.rs) : sum_kept<Plain>(rp, s0, s1, &sh, nodes, nrem));
         if (lane == 0) sh.scan[warp] = s;
         __syncthreads();
         int pick = 0;
