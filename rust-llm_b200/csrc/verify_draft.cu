@@ -250,10 +250,10 @@ struct Node {
 };
 
 // What a draw is decided on: the frames and factors of w = max(p rho - q, 0), or
-// of p alone. Ids within 6 binades of the frames' logits, which are few, are
-// weighed in doubles: nearly all of the error of a running sum comes from them
-// (150 thousand normal logits of deviation 3: 3 to 6e-9 of the whole without,
-// 0.3 to 1e-9 with).
+// of p alone. Ids within 3 binades of the frames' logits, which are few, are
+// weighed in doubles: most of the error of a running sum comes from them (150
+// thousand normal logits of deviation 3: 3 to 6e-9 of the whole without, 0.8 to
+// 1.5e-9 with; 6 binades halve that again and cost 15% of a call).
 struct Side {
   float c, m, F, heavy;  // heavy: logits from here on
   double cd, r;          // log2(e) / T, and how far m's exponent is from its frame
@@ -736,7 +736,7 @@ __device__ __noinline__ double sum_kept(Row<T> r, int j0, int j1, const Ctl* sh,
 #pragma unroll
     for (int i = 0; i < 16; ++i) w += weight(x[i >> 2][i & 3], f);
     s += static_cast<double>(w);
-    if (max16(x) >= f.heavy) {
+    if (w > 0.12f) {  // a heavy id weighs 1 / 8 at least
       unsigned hv = 0;
 #pragma unroll
       for (int k = 0; k < 16; ++k)
