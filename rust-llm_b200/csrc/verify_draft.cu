@@ -24,17 +24,17 @@
 // 2300 and 650 cycles), and the longest walk of a batch ends the call. While the
 // cluster joins its sums and decides, the rows of the node's first child are
 // fetched into L2; a pass then runs on L2, a warp's next chunk loaded as soon as
-// the registers of the last are free. 64 chains of 4 x 128256 f32 take 67 us, of
-// which HBM needs 27 for the rows that are looked at; one chain of 3 x 32000 10.
+// the registers of the last are free. 64 chains of 4 x 128256 f32 take 74 us, of
+// which HBM needs 27 for the rows that are looked at; one chain of 3 x 32000 12.
 //
 // Precision. A weight is 2^(x c - F): one FMA and ex2.approx, relative error
 // about 2^-22 with no bias that two ids would not share; c = log2(e) / T in
 // single precision tilts a row by at most 2^-25 |t|. A lane's F is the product
 // max c of the first logits it sees, so that what weighs most has a short
 // exponent, and is moved only where a later logit lies 64 binades above: any F
-// does, as long as the sums are joined with it. Sums are doubles, and draws are compared in
-// doubles: a token can differ from the exact one only where the draw lies
-// within about 1e-8 of a border.
+// does, as long as the sums are joined with it. Sums are doubles, and a draw is
+// decided on sums in which the heaviest ids are weighed in doubles: a token can
+// differ from the exact one only where the draw lies within some 1e-9 of a border.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -1337,9 +1337,9 @@ rl_status side_of(const rl_dist_rows* d, int V, int per_seq, VdSide* s) {
 // rows can be split: eight where they find room on the GPU at once (two CTAs an
 // SM), four where there are sequences enough, and at least 2048 ids a CTA,
 // below which the join costs more than it saves. us a call at 2 / 4 / 8 CTAs:
-// 64 x 4 x 128256 f32 88 / 67 / 73, 128 x 7 x 151936 bf16 178 / 111 / 111, 16
-// trees of 29 nodes x 128256 64 / 41 / 30, 24 masked chains of 5 x 32000 61 / 40 /
-// 34, one chain of 3 x 32000 13.9 / 10.9 / 10.2.
+// 64 x 4 x 128256 f32 102 / 74 / 81, 128 x 7 x 151936 bf16 197 / 126 / 128, 16
+// trees of 29 nodes x 128256 80 / 49 / 35, 24 masked chains of 5 x 32000 69 / 47 /
+// 39, one chain of 3 x 32000 18.1 / 13.5 / 11.9.
 int cluster_size(int B, int V) {
   int C = 1;
   while (C < kMaxCluster && (C < 4 || static_cast<int64_t>(B) * C * 2 <= 256) && V / (2 * C) >= 2048) C *= 2;
