@@ -236,8 +236,6 @@ def _prepare_head(case, seed):
 def prepare(case, seed):
     s = {"verify": _prepare_verify, "tree": _prepare_tree, "head": _prepare_head}[case["op"]](case, seed)
     s["case"] = case
-    if own:  # the handle that a program keeps
-        s["sampler"] = _package().Sampler(torch.cuda.current_device(), max_batch=256, max_vocab=64, max_history=1)
     return s
 
 
@@ -370,8 +368,20 @@ def _plain_head(s):
 # ---------------------------------------------------------------------------------------------------------------------
 # one pass
 # ---------------------------------------------------------------------------------------------------------------------
+#: The handles that a program keeps for all of its calls, one a device: made at a device's first call, whatever its inputs.
+_handles = {}
+
+
+def _handle(rl):
+    device = torch.cuda.current_device()
+    if device not in _handles:
+        _handles[device] = rl.Sampler(device, max_batch=256, max_vocab=64, max_history=1)
+    return _handles[device]
+
+
 def _own(s):
-    rl, h, op = _package(), s["sampler"], s["case"]["op"]
+    rl, op = _package(), s["case"]["op"]
+    h = _handle(rl)
     if op == "head":
         w = rl.Q4Weight(s["q"], s["scale"], s["case"]["group"])
         if s["case"]["out"] == "greedy":
