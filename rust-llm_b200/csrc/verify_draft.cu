@@ -905,7 +905,8 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
     nd.first = !tree && tid + 1 < n ? tid + 1 : INT_MAX;
     if (!Plain && status == RL_OK && tid < n) {
       read_cut<TP>(a.p, p0 + tid, V, nd.cut[0], nd.xcut[0]);
-      if (drawn && (tree || tid + 1 < n)) read_cut<TQ>(a.q, q0 + tid, V, nd.cut[1], nd.xcut[1]);
+      // (a root alone has no use for a draft row, and its place was not checked)
+      if (drawn && n > 1 && (tree || tid + 1 < n)) read_cut<TQ>(a.q, q0 + tid, V, nd.cut[1], nd.xcut[1]);
     }
   }
   __syncthreads();
