@@ -329,7 +329,9 @@ rl_status rl_specdec_verify(rl_sampler* h, const float* logits, int B, int V, in
  * (prompt lookup, a draft model's best tokens): q is 1 at the draft, so a
  * refused draft x is taken out of w. With a target temperature <= 0 drafts
  * equal to the row's largest are accepted, and q is not looked at.
- * Drafts outside [0, V) have probability 0.
+ * Drafts outside [0, V) have probability 0. Where the refused drafts hold all of
+ * the row (uniforms of 1, or a last one that rounding leaves at its border) the
+ * token is drawn from p: a sequence that is RL_OK always gets one.
  *
  *  out_accepted[B]  drafts accepted
  *  out_path[B, max_node]  (tree, nullable) the accepted nodes, then -1

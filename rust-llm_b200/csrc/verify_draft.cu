@@ -273,6 +273,7 @@ struct Ctl {
   double rest;              // draw target inside the draw's part
   double Ps, Qs;            // sums of weights of both rows, relative to Pm, Qm
   double C, S, px;
+  double summed;            // S as it was last summed (given drafts: less is taken off it since)
   float Pm, Qm;
   int Pid;
   int status;
@@ -1001,7 +1002,7 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
         sh.Qm = Q.m;
         sh.Pid = P.id;
         sh.C = 0.0;
-        sh.S = 1.0;
+        sh.S = sh.summed = 1.0;
         sh.k = 0;
         sh.nchild = nchild;
         sh.nremoved = 0;
@@ -1050,10 +1051,18 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
           if (!gone && ep > 0.0) {
             sh.removed[sh.nremoved++] = static_cast<int16_t>(c);
             S = fmax(S - ep / sh.Ps, 0.0);
+            // with most of a sum taken off, what is left is its rounding: where
+            // another child asks for it, it is summed again (1 / 4: an error of
+            // 1e-6 becomes 4e-6 at most)
+            if (S < 0.25 * sh.summed && k + 1 < sh.nchild) {
+              nx = kSums;
+              ++k;
+              break;
+            }
           }
         }
         if (nx == kNone && sh.nremoved > 0) nx = kRefresh;
-        if (nx == kSums) {
+        if (nx == kSums && with_q) {
           const double rho = sh.Qs / (sh.C * sh.Ps);
           sh.rs.rho = rho;
           sh.rs.rhi = static_cast<float>(rho);
@@ -1069,8 +1078,9 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
       status = sh.status;
       next = sh.next;
       if (status != RL_OK || next != kSums) break;
-      // ---- sums of w = max(p - C q, 0) over the parts ----
-      double s = sum_resid<Plain>(rp, rq, j0, j1, &sh.rs);
+      // ---- sums of w over the parts: max(p - C q, 0), or p without the refused
+      // given tokens ----
+      double s = with_q ? sum_resid<Plain>(rp, rq, j0, j1, &sh.rs) : sum_kept<Plain>(rp, j0, j1, &sh, nodes, sh.nremoved);
       s = warp_sum_d(s);
       if (lane < C) send(&sh.w[par][mypart], s, &sh.bar[par][1], lane);
       if (warp == 0) {
@@ -1079,14 +1089,14 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
         for (int i = lane; i < np; i += 32) t += sh.w[par][i];
         t = warp_sum_d(t);
         if (lane == 0) {
-          sh.S = t * sh.C / sh.Qs;  // as a probability
+          sh.S = sh.summed = with_q ? t * sh.C / sh.Qs : t / sh.Ps;  // as a probability
           if (!in) sh.status = RL_ERR_TIMEOUT;
         }
         __syncwarp();
       }
       phase ^= 2u << (2 * par);
       par ^= 1;
-      sums = true;
+      sums = with_q;
     }
     if (status != RL_OK) {
       // an empty row: once more without its mask, if that has no bit
@@ -1120,7 +1130,7 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
       break;
     }
     const bool resid = sums && sh.S > 0.0;  // else all of w rounded away: from p
-    const int nrem = sh.nremoved;
+    int nrem = sh.nremoved;
     // The weights w of ids j .. j + 3: max(p rho - q, 0) in units of q's frame,
     // or p without the refused given tokens in units of p's.
     const auto w4 = [&](int j, int end, double (&w)[4]) {
@@ -1141,30 +1151,35 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
         else w[3] = v;
       }
     };
-    if (!resid) {
-      // the parts' sums once more, without refused given tokens (taking a weight
-      // off a sum would leave its rounding) and with the heavy ids' exact weights
-      double f = 0.0;
-      if (j0 < j1) f = warp_sum_d(sum_kept<Plain>(rp, j0, j1, &sh, nodes, nrem));
-      if (lane < C) send(&sh.w[par][mypart], f, &sh.bar[par][1], lane);
-      if (warp == 0 && !receive(&sh.bar[par][1], phase >> (2 * par + 1) & 1u, static_cast<uint32_t>(np * sizeof(double))) && lane == 0)
-        sh.status = RL_ERR_TIMEOUT;
-      phase ^= 2u << (2 * par);
-      par ^= 1;
-    }
-    // ---- which part holds the drawn token ----
-    if (warp == 0) {
-      const int per = (np + 31) >> 5;
-      double wp[kPerLane];
+    while (true) {
+      if (!resid) {
+        // the parts' sums once more, without refused given tokens (taking a weight
+        // off a sum would leave its rounding) and with the heavy ids' exact weights
+        double f = 0.0;
+        if (j0 < j1) f = warp_sum_d(sum_kept<Plain>(rp, j0, j1, &sh, nodes, nrem));
+        if (lane < C) send(&sh.w[par][mypart], f, &sh.bar[par][1], lane);
+        if (warp == 0 && !receive(&sh.bar[par][1], phase >> (2 * par + 1) & 1u, static_cast<uint32_t>(np * sizeof(double))) && lane == 0)
+          sh.status = RL_ERR_TIMEOUT;
+        phase ^= 2u << (2 * par);
+        par ^= 1;
+      }
+      // ---- which part holds the drawn token ----
+      if (warp == 0) {
+        const int per = (np + 31) >> 5;
+        double wp[kPerLane];
 #pragma unroll
-      for (int k = 0; k < kPerLane; ++k) wp[k] = k < per && lane * per + k < np ? sh.w[par ^ 1][lane * per + k] : 0.0;
-      find_owner(sh, wp, np, du);
+        for (int k = 0; k < kPerLane; ++k) wp[k] = k < per && lane * per + k < np ? sh.w[par ^ 1][lane * per + k] : 0.0;
+        find_owner(sh, wp, np, du);
+      }
+      __syncthreads();
+      status = sh.status;
+      if (status != RL_OK || sh.owner >= 0 || nrem == 0) break;
+      nrem = 0;  // the refused tokens hold all of the row (uniforms of 1): from p
+      __syncthreads();
     }
-    __syncthreads();
-    status = sh.status;
     if (status != RL_OK) break;
     const int owner = sh.owner;
-    if (owner >= 0 && owner / kVW == rank) {
+    if (owner >= 0 && owner / kVW == rank) {  // (a row that passed the join has weight somewhere)
       // ---- the drawn token inside that part, by the whole CTA: down to 4 ids a
       // thread by the sums of the warps' shares ----
       int w0 = static_cast<int>(min(static_cast<int64_t>(owner) * a.part, static_cast<int64_t>(V)));
@@ -1240,8 +1255,6 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
         if (token >= 0) tprob = static_cast<float>(weight_2(to_f(rp.x[token]), sh.Pm, cp, frame(sh.Pm, cp)) / sh.Ps);
         found = true;
       }
-    } else if (owner < 0 && rank == 0 && tid == 0) {
-      found = true;  // every id with weight was refused (uniforms of 1): no token
     }
     break;
   }
