@@ -25,16 +25,20 @@
 // cluster joins its sums and decides, the rows of the node's first child are
 // fetched into L2; a pass then runs on L2, a warp's next chunk loaded as soon as
 // the registers of the last are free. 64 chains of 4 x 128256 f32 take 74 us, of
-// which HBM needs 27 for the rows that are looked at; one chain of 3 x 32000 12.
+// which HBM needs 27 for the rows that are looked at; one chain of 3 x 32000 12.6.
 //
-// Precision. A weight is 2^(x c - F): one FMA and ex2.approx, relative error
-// about 2^-22 with no bias that two ids would not share; c = log2(e) / T in
-// single precision tilts a row by at most 2^-25 |t|. A lane's F is the product
-// max c of the first logits it sees, so that what weighs most has a short
+// Precision. A weight is 2^(x c - F): one FMA and ex2.approx, a relative error of
+// 2^-22 and the exponent's rounding (2^-24 of it); c = log2(e) / T in single
+// precision tilts a row by at most 2^-24 |t| at the exponent t. A lane's F is the
+// product max c of the first logits it sees, so that what weighs most has a short
 // exponent, and is moved only where a later logit lies 64 binades above: any F
-// does, as long as the sums are joined with it. Sums are doubles, and a draw is
-// decided on sums in which the heaviest ids are weighed in doubles: a token can
-// differ from the exact one only where the draw lies within some 1e-9 of a border.
+// does, as long as the sums are joined with it. Sums are doubles. The rows' sums,
+// and with them the accept tests, the factor of a residual and the probabilities
+// that are put out, are within about 1e-6 of 64 bits (1.4e-6 the worst of 20,000
+// sequences). A draw is decided on sums of its own: log2(e) / T there is two floats,
+// and ids with a 256th of the row or more are weighed in doubles and kept out of
+// the sums in floats. What is left is the light ids' ex2, at most 2^-24 of the
+// whole, 2e-9 (alike ids) to 5e-9 (one with half of the row) on the average.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -118,12 +122,13 @@ __device__ __forceinline__ float ex2(float t) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
   return r;
 }
-// Where a logit m lies in the exponent's domain: F = m c. From 2^24 on the
-// product's rounding would be binades (and it can leave the range of floats): such
-// frames are marked by NaN, and weights are taken from the difference x - m.
+// Where a logit m lies in the exponent's domain: F = m c. Far from 0 the product's
+// rounding counts in binades (and it can leave the range of floats): such frames
+// are marked by NaN, and weights are taken from the difference x - m. From 2^16 on,
+// where a row's tilt (Side) is still a small part of a binade.
 __device__ __forceinline__ float frame(float m, float c) {
   const float F = m * c;
-  return fabsf(F) < 16777216.0f ? F : __int_as_float(0x7fc00000);
+  return fabsf(F) < 65536.0f ? F : __int_as_float(0x7fc00000);
 }
 __device__ __forceinline__ bool is_near(float F) { return F == F; }
 // The exponent of x relative to the frame of logit m.
@@ -250,13 +255,26 @@ struct Node {
 };
 
 // What a draw is decided on: the frames and factors of w = max(p rho - q, 0), or
-// of p alone. Ids within 3 binades of the frames' logits, which are few, are
-// weighed in doubles: most of the error of a running sum comes from them (150
-// thousand normal logits of deviation 3: 3 to 6e-9 of the whole without, 0.8 to
-// 1.5e-9 with; 6 binades halve that again and cost 15% of a call).
+// of p alone. Ids of a 2^-kHeavy of their row and more, 256 at most, are weighed in
+// doubles and left out of the sums in floats: most of the error of a running sum
+// comes from them, and a flat row has none. Mean error of a running sum next to
+// its borders, as a share of the whole, at 32,000 / 128,256 normal logits of
+// deviation 3, and where one id has 0.3 to 0.6 of the row beside them:
+//   kHeavy 7   2.4e-9 / 2.6e-9, 4.7e-9 / 5.0e-9
+//          8   2.2e-9 / 2.4e-9, 4.4e-9 / 5.0e-9
+//         10   2.1e-9 / 1.6e-9, 3.6e-9 / 4.4e-9   64 chains of 4 x 128256 2% slower
+// (by a share of the row: ids within 3 binades of the frame took 131 us of 64
+// chains at T = 5 where this takes 78).
+constexpr int kHeavy = 8;
+struct Scale {
+  double cd, dc;
+  float c, crz, lo;
+};
 struct Side {
-  float c, m, F, heavy;  // heavy: logits from here on
-  double cd, r;          // log2(e) / T, and how far m's exponent is from its frame
+  float c, lo, m, F;  // log2(e) / T = c + lo, lo > 0
+  float heavy;        // logits from here on
+  double cd, r;       // log2(e) / T, and how far m's exponent is from its frame
+  double unit;        // what a weight is multiplied by to be as those of the row's sum
 };
 struct Resid {
   Side p, q;
@@ -267,7 +285,7 @@ struct Ctl {
   Part part[2][2][kParts];  // [parity][side]: every CTA's warps write into every CTA
   double w[2][kParts];      // [parity] the parts' sums of w
   Resid rs;
-  double cd[2];             // log2(e) / T of both sides
+  Scale scale[2];
   uint64_t bar[2][2];       // [parity][0 parts, 1 sums of w]: what is to come has come
   double scan[kVW];
   double rest;              // draw target inside the draw's part
@@ -278,14 +296,14 @@ struct Ctl {
   int Pid;
   int status;
   int k;                    // next child to try
-  int next;                 // accepted child, or kNone, kSums, kRefresh
+  int next;                 // accepted child, or kNone, kSums, kRefresh, kRest
   int owner;                // part that holds the drawn token
   int at;                   // first id found by the draw
   int nchild, nremoved;
   int16_t child[RL_VERIFY_MAX_NODES];    // of the present node
   int16_t removed[RL_VERIFY_MAX_NODES];  // its refused given children
 };
-constexpr int kNone = -1, kSums = -2, kRefresh = -3;
+constexpr int kNone = -1, kSums = -2, kRefresh = -3, kRest = -4;
 
 // Whether id j is one of the refused given tokens.
 __device__ __forceinline__ bool is_removed(const Ctl& sh, const Node* nodes, int n, int j) {
@@ -649,28 +667,44 @@ __device__ __noinline__ Seen2 see_rows(Row<TP> rp, Row<TQ> rq, int j0, int j1, f
                   [&](int, const float (&y)[4][4]) { see(zq, y, cq); });
   return {zp, zq};
 }
-// log2(e) / T in doubles.
-__device__ __forceinline__ double scale_d(float T) {
-  return fmin(fmax(1.4426950408889634074 / static_cast<double>(T), 1e-30), 3e38);
-}
-__device__ __forceinline__ Side side(float c, double cd, float m) {
-  Side f;
-  f.c = c;
-  f.m = m;
-  f.F = frame(m, c);
-  f.heavy = m - __fdividef(3.0f, c);
-  f.cd = cd;
-  f.r = is_near(f.F) ? static_cast<double>(__fmaf_rn(m, c, -f.F)) : 0.0;
-  return f;
+// A side's log2(e) / T: in doubles, the float c that sums are made with, and as
+// crz + lo, rounded towards 0 so that both products of a logit of -inf are -inf.
+__device__ __forceinline__ void set_scale(Scale& k, float T, float c) {
+  k.cd = fmin(fmax(1.4426950408889634074 / static_cast<double>(T), 1e-30), 3e38);
+  k.dc = 0.69314718055994530942 * (static_cast<double>(c) - k.cd);
+  k.c = c;
+  k.crz = __double2float_rz(k.cd);
+  k.lo = fmaxf(static_cast<float>(k.cd - static_cast<double>(k.crz)), 1.17549435e-38f);
 }
 __device__ __noinline__ double weight_d(float x, float m, double c, double r) {
   return exp2((static_cast<double>(x) - static_cast<double>(m)) * c + r);
 }
 __device__ __forceinline__ double weight_d(float x, const Side& f) { return weight_d(x, f.m, f.cd, f.r); }
+// The weight of x, 2^(x c + x lo - F): c alone would tilt the row by 2^-24 of an exponent.
+__device__ __forceinline__ float near_weight(float x, const Side& f) { return ex2(__fmaf_rn(x, f.lo, __fmaf_rn(x, f.c, -f.F))); }
+__device__ __forceinline__ float weight(float x, const Side& f) {
+  if (is_near(f.F)) return near_weight(x, f);
+  const float t = x - f.m;
+  return ex2(__fmaf_rn(t, f.lo, t * f.c));
+}
+// Of a row whose sum is relative to logit m's frame.
+__device__ __forceinline__ Side side(const Scale& k, float m, double sum) {
+  Side f;
+  f.c = k.crz;
+  f.lo = k.lo;
+  f.m = m;
+  f.F = frame(m, k.c);
+  f.heavy = m + __fdividef(__log2f(static_cast<float>(sum)) - static_cast<float>(kHeavy), k.c);
+  f.cd = k.cd;
+  const double md = static_cast<double>(m);
+  f.r = is_near(f.F) ? fma(md, k.cd, -static_cast<double>(f.F)) : 0.0;
+  const double y = is_near(f.F) ? md * k.dc : 0.0;  // |y| < 2^-8
+  f.unit = fma(fma(fma(y, 1.0 / 6.0, 0.5), y, 1.0), y, 1.0);
+  return f;
+}
 __device__ __forceinline__ float resid_w(float ep, float eq, const Resid& f) {
   return fmaxf(__fmaf_rn(ep, f.rhi, __fmaf_rn(ep, f.rlo, -eq)), 0.0f);
 }
-__device__ __forceinline__ float weight(float x, const Side& f) { return weight(x, f.m, f.c, f.F); }
 // The weight of one id.
 __device__ __forceinline__ double one_weight(float x, const Side& f) {
   return x >= f.heavy ? weight_d(x, f) : static_cast<double>(weight(x, f));
@@ -685,19 +719,30 @@ __device__ __forceinline__ float pick16(const float (&x)[4][4], int i) {
   for (int k = 1; k < 16; ++k) v = i == k ? x[k >> 2][k & 3] : v;
   return v;
 }
-// A lane's sum of w over ids [j0, j1).
+// A lane's sum of w over ids [j0, j1). Heavy ids are left out of the sums in
+// floats: added there, what each addition rounds off would stay.
 template <bool Plain, typename TP, typename TQ>
 __device__ __noinline__ double sum_resid(Row<TP> rp, Row<TQ> rq, int j0, int j1, const Resid* of) {
   const Resid f = *of;
   double s = 0.0;
-  pass_both<Plain>(rp, rq, j0, j1, [&](const float (&x)[4][4], const float (&y)[4][4]) {
+  pass_both<Plain>(rp, rq, j0, j1, [&](float (&x)[4][4], const float (&y)[4][4]) {
+    if (max16(x) >= f.p.heavy || max16(y) >= f.q.heavy) {
+      unsigned hv = 0;
+#pragma unroll
+      for (int k = 0; k < 16; ++k)
+        if (x[k >> 2][k & 3] >= f.p.heavy || y[k >> 2][k & 3] >= f.q.heavy) hv |= 1u << k;
+      for (unsigned h = hv; h; h &= h - 1) s += one_weight(pick16(x, __ffs(h) - 1), pick16(y, __ffs(h) - 1), f);
+#pragma unroll
+      for (int k = 0; k < 16; ++k)
+        if (hv >> k & 1u) x[k >> 2][k & 3] = RL_NEG_INF;
+    }
     float w = 0.0f;
     if (is_near(f.p.F) && is_near(f.q.F)) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         float v[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = resid_w(weight(x[i][k], f.p.c, f.p.F), weight(y[i][k], f.q.c, f.q.F), f);
+        for (int k = 0; k < 4; ++k) v[k] = resid_w(near_weight(x[i][k], f.p), near_weight(y[i][k], f.q), f);
         w += (v[0] + v[1]) + (v[2] + v[3]);
       }
     } else {
@@ -705,16 +750,6 @@ __device__ __noinline__ double sum_resid(Row<TP> rp, Row<TQ> rq, int j0, int j1,
       for (int k = 0; k < 16; ++k) w += resid_w(weight(x[k >> 2][k & 3], f.p), weight(y[k >> 2][k & 3], f.q), f);
     }
     s += static_cast<double>(w);
-    if (max16(x) >= f.p.heavy || max16(y) >= f.q.heavy) {
-      unsigned hv = 0;
-#pragma unroll
-      for (int k = 0; k < 16; ++k)
-        if (x[k >> 2][k & 3] >= f.p.heavy || y[k >> 2][k & 3] >= f.q.heavy) hv |= 1u << k;
-      for (; hv; hv &= hv - 1) {
-        const float a = pick16(x, __ffs(hv) - 1), b = pick16(y, __ffs(hv) - 1);
-        s += one_weight(a, b, f) - static_cast<double>(resid_w(weight(a, f.p), weight(b, f.q), f));
-      }
-    }
   });
   return s;
 }
@@ -733,20 +768,29 @@ __device__ __noinline__ double sum_kept(Row<T> r, int j0, int j1, const Ctl* sh,
           if (i == ((t >> 7) << 2 | (t & 3))) x[i >> 2][i & 3] = RL_NEG_INF;
       }
     }
-    float w = 0.0f;
+    const auto sum = [&] {
+      float w = 0.0f;
+      if (is_near(f.F)) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) w += weight(x[i >> 2][i & 3], f);
-    s += static_cast<double>(w);
-    if (w > 0.12f) {  // a heavy id weighs 1 / 8 at least
+        for (int i = 0; i < 4; ++i)
+          w += (near_weight(x[i][0], f) + near_weight(x[i][1], f)) + (near_weight(x[i][2], f) + near_weight(x[i][3], f));
+      } else {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) w += weight(x[k >> 2][k & 3], f);
+      }
+      return w;
+    };
+    if (max16(x) >= f.heavy) {
       unsigned hv = 0;
 #pragma unroll
       for (int k = 0; k < 16; ++k)
         if (x[k >> 2][k & 3] >= f.heavy) hv |= 1u << k;
-      for (; hv; hv &= hv - 1) {
-        const float a = pick16(x, __ffs(hv) - 1);
-        s += weight_d(a, f) - static_cast<double>(weight(a, f));
-      }
+      for (unsigned h = hv; h; h &= h - 1) s += weight_d(pick16(x, __ffs(h) - 1), f);
+#pragma unroll
+      for (int k = 0; k < 16; ++k)
+        if (hv >> k & 1u) x[k >> 2][k & 3] = RL_NEG_INF;
     }
+    s += static_cast<double>(sum());
   });
   return s;
 }
@@ -895,8 +939,9 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
     for (int i = 0; i < 4; ++i) mbar_init(&sh.bar[i >> 1][i & 1], 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (tid == kVT - 1) sh.cd[0] = scale_d(greedy ? 1.0f : Tp);
-  if (tid == kVT - 33) sh.cd[1] = scale_d(drawn ? Tq : 1.0f);
+  if (tid == kVT - 1) set_scale(sh.scale[0], greedy ? 1.0f : Tp, cp);
+  if (tid == kVT - 33) set_scale(sh.scale[1], drawn ? Tq : 1.0f, cq);
+  __syncwarp();
   cgx::this_cluster().barrier_arrive();
   if (tid < N) {
     Node& nd = nodes[tid];
@@ -1055,21 +1100,21 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
             // another child asks for it, it is summed again (1 / 4: an error of
             // 1e-6 becomes 4e-6 at most)
             if (S < 0.25 * sh.summed && k + 1 < sh.nchild) {
-              nx = kSums;
+              nx = kRest;
               ++k;
               break;
             }
           }
         }
         if (nx == kNone && sh.nremoved > 0) nx = kRefresh;
-        if (nx == kSums && with_q) {
-          const double rho = sh.Qs / (sh.C * sh.Ps);
+        if (nx < 0 && !greedy) sh.rs.p = side(sh.scale[0], sh.Pm, sh.Ps);
+        if (nx == kSums) {
+          sh.rs.q = side(sh.scale[1], sh.Qm, sh.Qs);
+          const double rho = sh.Qs * sh.rs.p.unit / (sh.C * sh.Ps * sh.rs.q.unit);
           sh.rs.rho = rho;
           sh.rs.rhi = static_cast<float>(rho);
           sh.rs.rlo = static_cast<float>(rho - static_cast<double>(sh.rs.rhi));
-          sh.rs.q = side(cq, sh.cd[1], sh.Qm);
         }
-        if (nx < 0 && !greedy) sh.rs.p = side(cp, sh.cd[0], sh.Pm);
         sh.S = S;
         sh.k = k;
         sh.next = nx;
@@ -1077,10 +1122,10 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
       __syncthreads();
       status = sh.status;
       next = sh.next;
-      if (status != RL_OK || next != kSums) break;
+      if (status != RL_OK || (next != kSums && next != kRest)) break;
       // ---- sums of w over the parts: max(p - C q, 0), or p without the refused
       // given tokens ----
-      double s = with_q ? sum_resid<Plain>(rp, rq, j0, j1, &sh.rs) : sum_kept<Plain>(rp, j0, j1, &sh, nodes, sh.nremoved);
+      double s = next == kSums ? sum_resid<Plain>(rp, rq, j0, j1, &sh.rs) : sum_kept<Plain>(rp, j0, j1, &sh, nodes, sh.nremoved);
       s = warp_sum_d(s);
       if (lane < C) send(&sh.w[par][mypart], s, &sh.bar[par][1], lane);
       if (warp == 0) {
@@ -1089,14 +1134,14 @@ __global__ void __launch_bounds__(kVT, 2) verify_kernel(const __grid_constant__ 
         for (int i = lane; i < np; i += 32) t += sh.w[par][i];
         t = warp_sum_d(t);
         if (lane == 0) {
-          sh.S = sh.summed = with_q ? t * sh.C / sh.Qs : t / sh.Ps;  // as a probability
+          sh.S = sh.summed = next == kSums ? t * sh.rs.q.unit * sh.C / sh.Qs : t * sh.rs.p.unit / sh.Ps;  // as a probability
           if (!in) sh.status = RL_ERR_TIMEOUT;
         }
         __syncwarp();
       }
       phase ^= 2u << (2 * par);
       par ^= 1;
-      sums = with_q;
+      sums = next == kSums;
     }
     if (status != RL_OK) {
       // an empty row: once more without its mask, if that has no bit
