@@ -159,38 +159,68 @@ def apply_tokens(states, tokens) -> dict:
     return out
 
 
+def speculative_params(states, cutoffs: bool) -> np.ndarray:
+    """The sampling parameters of a speculative step's sequences: their
+    temperatures, with `cutoffs` their top_p and top_k too. What the step would
+    drop is refused: penalties, which change a row's logits with every accepted
+    token, and a top_k without `cutoffs`."""
+    p = params_of(states)
+    for s in states:
+        if (s.repeat_penalty, s.presence_penalty, s.frequency_penalty) != (1.0, 0.0, 0.0):
+            raise ValueError(f"sequence {s.seq_id}: a speculative step applies no penalties")
+        if s.top_k > 0 and not cutoffs:
+            raise ValueError(f"sequence {s.seq_id}: top_k {s.top_k} needs SpeculativeStep(cutoffs=True)")
+    if not cutoffs:
+        p["top_p"], p["top_k"] = 1.0, 0
+    return p
+
+
 class SpeculativeStep:
     """Draft and verify for the live sequences of a batch: `draft` draws one
     token a sequence from the draft model's logits (called once for each
     position of the drafts), `verify` checks the drafts against the target's
     logits and gives each sequence its accepted drafts and one more token,
     distributed as the target's own samples are. Both models sample at the
-    sequences' temperatures (top-p and penalties are not applied here: verify
-    takes whole distributions)."""
+    sequences' temperatures, over whole distributions (a sequence's top_p is not
+    applied), or with `cutoffs` over what its top_k and top_p keep of each row.
+    Sequences with penalties are refused."""
 
-    def __init__(self, vocab: int, max_batch: int, max_draft: int, device: int = 0, uniform=None):
+    def __init__(self, vocab: int, max_batch: int, max_draft: int, device: int = 0, uniform=None, cutoffs: bool = False):
         if max_draft < 1 or max_draft + 1 > rlsampler.VERIFY_MAX_NODES:
             raise ValueError(f"max_draft {max_draft}")
-        self.V, self.K, self.device = vocab, max_draft, device
+        self.V, self.K, self.device, self.max_batch, self.cutoffs = vocab, max_draft, device, max_batch, cutoffs
         self.sampler = rlsampler.Sampler(device, max_batch=max_batch, max_vocab=vocab, max_history=1)
         rng = np.random.Generator(np.random.PCG64())
         self.uniform = uniform or (lambda n: (rng.random(n) * (1.0 - 2.0 ** -24)).astype(np.float32))
-
-    def _params(self, states, dev):
-        p = np.zeros(len(states), rlsampler.ROW_PARAMS_DTYPE)
-        p["temperature"], p["top_p"], p["repeat_penalty"] = [s.temperature for s in states], 1.0, 1.0
-        return rlsampler.params_tensor(p, dev)
 
     def _uniforms(self, shape, dev):
         import torch
 
         return torch.from_numpy(np.ascontiguousarray(self.uniform(int(np.prod(shape))), np.float32).reshape(shape)).to(dev)
 
+    def _rows(self, states, params, logits, each):
+        """The distributions of `each` rows a sequence."""
+        import torch
+
+        dev = logits.device
+        T = torch.tensor([s.temperature for s in states], dtype=torch.float32, device=dev)
+        if not self.cutoffs:
+            return rlsampler.DistRows(logits, T)
+        p = rlsampler.params_tensor(np.repeat(params, each), dev)
+        size, u = params.dtype.itemsize, torch.zeros(self.max_batch, device=dev)
+        cut = torch.empty(len(logits), dtype=torch.int32, device=dev)
+        for r in range(0, len(logits), self.max_batch):
+            n = min(self.max_batch, len(logits) - r)
+            # rows that are not finite have no cutoff; verify reports those it looks at
+            cut[r : r + n] = self.sampler.sample_debug(logits[r : r + n], p[r * size : (r + n) * size], u[:n], list_cap=1)[6][:, 2]
+        return rlsampler.DistRows(logits, T, cut=cut)
+
     def draft(self, states, logits):
         """One drafted token [B] (device) a sequence from draft logits [B, V]."""
         if tuple(logits.shape) != (len(states), self.V):
             raise ValueError(f"draft logits {tuple(logits.shape)} for {len(states)} sequences of vocabulary {self.V}")
-        tok, _, _ = self.sampler.sample(logits, self._params(states, logits.device), self._uniforms((len(states),), logits.device))
+        p = rlsampler.params_tensor(speculative_params(states, self.cutoffs), logits.device)
+        tok, _, _ = self.sampler.sample(logits, p, self._uniforms((len(states),), logits.device))
         return tok
 
     def verify(self, states, target_logits, drafts, draft_logits=None, n_draft=None):
@@ -204,11 +234,13 @@ class SpeculativeStep:
         B, dev = len(states), target_logits.device
         if tuple(drafts.shape) != (B, self.K) or tuple(target_logits.shape) != (B * (self.K + 1), self.V):
             raise ValueError(f"drafts {tuple(drafts.shape)} and target logits {tuple(target_logits.shape)} for {B} sequences")
-        T = torch.tensor([s.temperature for s in states], dtype=torch.float32, device=dev)
+        if draft_logits is not None and tuple(draft_logits.shape) != (B * self.K, self.V):
+            raise ValueError(f"draft logits {tuple(draft_logits.shape)} for {B} sequences of {self.K} drafts")
+        params = speculative_params(states, self.cutoffs)
         n = torch.full((B,), self.K, dtype=torch.int32, device=dev) if n_draft is None else n_draft
         acc, tok, _, st = self.sampler.specdec_verify_draft(
-            rlsampler.DistRows(target_logits, T), drafts, n, self._uniforms((B, self.K), dev), self._uniforms((B,), dev),
-            draft=None if draft_logits is None else rlsampler.DistRows(draft_logits, T))
+            self._rows(states, params, target_logits, self.K + 1), drafts, n, self._uniforms((B, self.K), dev),
+            self._uniforms((B,), dev), draft=None if draft_logits is None else self._rows(states, params, draft_logits, self.K))
         bad = st.cpu().numpy()
         if (bad != 0).any():
             i = int(np.flatnonzero(bad)[0])
