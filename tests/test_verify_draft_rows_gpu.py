@@ -51,3 +51,17 @@ def test_no_draft_rows_at_all(smp):
                                   cuda(c.u), cuda(c.du), draft=d)
     for g, w in zip(got, want):
         assert np.array_equal(g.cpu().numpy(), w)
+
+
+@pytest.mark.parametrize("which", ["draft", "target", "both"])
+@pytest.mark.parametrize("parents", [None, [-1, 0, 0, 1, 1, 2]])
+def test_masks_without_a_bit(smp, which, parents):
+    """A mask row without a bit allows every id, on either side, at any node."""
+    rng = np.random.default_rng(52)
+    B, V = 24, 700
+    c = Case(rng, B, V, parents=parents, K=None if parents else 4, mask=True, noise=1.5)
+    if which != "target":
+        c.qmask[rng.random(len(c.qmask)) < 0.6] = 0
+    if which != "draft":
+        c.mask[rng.random(len(c.mask)) < 0.6] = 0
+    c.check(c.call(smp))
