@@ -289,7 +289,10 @@ rl_status rl_specdec_verify(rl_sampler* h, const float* logits, int B, int V, in
  * softmax(x / T) over its kept ids, x at element r * ld:
  *   temperature[B]  one per sequence (NULL: 1). T <= 0: all of the row's
  *                   probability is on its largest kept logit, the lowest id on
- *                   ties. A non-finite T is an error of the sequence.
+ *                   ties (as rl_sample_batch; rl_greedy, rl_lmhead_greedy and
+ *                   rl_lmhead_q4_greedy take the last of equal maxima, so a draft
+ *                   of theirs is refused where bf16 logits tie).
+ *                   A non-finite T is an error of the sequence.
  *   mask            bit-packed allowed ids, a row per logits row (nullable);
  *                   a row with no bit set allows every id. Masked ids are not
  *                   looked at: NaN and infinities are allowed there.
@@ -303,7 +306,10 @@ rl_status rl_specdec_verify(rl_sampler* h, const float* logits, int B, int V, in
  *                   another at the widest number of rows); `rows` is the
  *                   number of rows that may be read.
  * -inf logits have probability 0. Weights below 2^-60 of the row's largest may
- * count as 0. 1e-30 and 3e38 bound log2(e) / T.
+ * count as 0. 1e-30 and 3e38 bound log2(e) / T. Accept tests and out_prob are
+ * computed from f32 weights, within about 1e-6 of 64 bits (2e-6 for tokens 50
+ * binades below their row's largest); a draw's running sums are within 1e-7 of the
+ * whole, 5e-9 on the average.
  *
  * rl_specdec_verify_draft -- a chain. Sequence b has n_draft[b] in [0,
  * max_draft] drafts drafts[b, i], target rows first_row + 0 .. n_draft and
@@ -466,7 +472,9 @@ rl_status rl_lmhead_sample(rl_sampler* h, const uint16_t* hidden, int64_t ldh, c
  *   group  32, 64 or 128; H a multiple of group and of 64
  * Products are exact in f32 and sums are f32; a group's sum is multiplied by
  * its scale in f32 (scales of magnitudes up to 2^90). Up to 16 batch rows, hidden
- * elements below 2^-27 of their row's largest are rounded to 2^-35 of it.
+ * elements below 2^-27 of their row's largest are rounded to 2^-35 of it, and sums
+ * are added in another order: a row's logits may differ in their last bits from
+ * those that a larger batch gives it.
  *
  * rl_lmhead_q4_quantize: such a weight from the bf16 one that rl_lmhead_*
  *   takes (read once, laid out once): per group scale = -m / 8 for the element

@@ -21,7 +21,8 @@ __device__ __forceinline__ uint64_t lm_policy_last() {
 }
 
 // 2-D tiled TMA load into this CTA's shared memory (no multicast); x is the
-// K coordinate, always a multiple of 64 elements (128 bytes).
+// K coordinate in the map's elements: a multiple of 64 bf16 values (128 bytes), or
+// of 64 or 128 one-byte pairs of codes, whatever a box is wide.
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar,
                                             uint64_t policy) {
   asm volatile(

@@ -32,7 +32,8 @@
 // Up to 16 batch rows (q4_few_kernel) the hand-overs between those roles cost
 // more than the work: there each warp multiplies what it loads, on its own. It
 // streams the codes of 32 vocabulary rows through a ring of its own and takes
-// them, as f16, straight into mma.sync fragments; the hidden states lie in
+// them, as f16 (the published way of setting codes under the exponent of 1024 and
+// subtracting), straight into mma.sync fragments; the hidden states lie in
 // shared memory in the order of the fragments. A CTA's warps share its rows'
 // codes evenly, cut where they fall, so that none waits for another; the sums of
 // rows that two warps share are added at the end.
@@ -488,8 +489,8 @@ __global__ void __launch_bounds__((4 + NDQ + NEP) * 32, 1)
           for (int i = 0; i < kNg; ++i) {
             if (i > 0 && g0 + h0 + i >= ngroups) break;  // half a block, the tile's last
             const float s = bf16_at(sw[(h0 + i) >> 1], (h0 + i) & 1);
-            // sixteen columns at a time: wider loads keep the MMAs from TMEM (128
-            // batch rows, H 4096, V 128256: 157 us, with 32 columns 200)
+            // sixteen columns at a time: wider loads keep the MMAs from TMEM (32
+            // columns took 27% longer at 128 batch rows, H 4096, V 128256)
 #pragma unroll
             for (int c = 0; c < NC; c += 16) {
               uint32_t r[16];
@@ -601,7 +602,8 @@ __device__ __forceinline__ float finite_abs(float x) { return fabsf(x) < RL_POS_
 // step j multiplies 4 j .. 4 j + 3 of those. A group's sum is scaled in f32.
 //
 // Hidden states are bf16 brought near 2^10 by the power of two of the batch
-// row's largest, and so exact in f16 but for what is below 2^-24 of the largest.
+// row's largest, and so exact in f16 (steps of 2^-24, eight bits a value) but for
+// what is below 2^-27 of the largest.
 template <int GS>
 __device__ __forceinline__ void row_words(const uint8_t* row, int swz, int half, int t, uint32_t (&w)[4]) {
   // the four words of this lane in K = 128 of a row (64 bytes of a box, whose
@@ -896,7 +898,9 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1)
 
 // ---------------------------------------------------------------------------
 // Quantisation: a thread takes eight elements (a word of codes), the lanes of a
-// group find its largest magnitude. Bound by HBM (2.5 bytes an element).
+// group find its largest magnitude. 128256 x 4096: 763 us, bound by instructions
+// (integer pipe 63% active); HBM needs 203 for the 2.5 bytes an element. It runs
+// once for a weight.
 // ---------------------------------------------------------------------------
 __global__ void __launch_bounds__(256) q4_quantize_kernel(const uint16_t* __restrict__ w, int64_t ldw, int H, int V,
                                                           int group, uint8_t* __restrict__ q, int64_t ldq,

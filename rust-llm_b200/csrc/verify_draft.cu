@@ -1395,10 +1395,10 @@ rl_status side_of(const rl_dist_rows* d, int V, int per_seq, VdSide* s) {
 // CTAs of a sequence's cluster. A walk's steps follow one another and only its
 // rows can be split: eight where they find room on the GPU at once (two CTAs an
 // SM), four where there are sequences enough, and at least 2048 ids a CTA,
-// below which the join costs more than it saves. us a call at 2 / 4 / 8 CTAs:
-// 64 x 4 x 128256 f32 102 / 74 / 81, 128 x 7 x 151936 bf16 197 / 126 / 128, 16
-// trees of 29 nodes x 128256 80 / 49 / 35, 24 masked chains of 5 x 32000 69 / 47 /
-// 39, one chain of 3 x 32000 18.1 / 13.5 / 11.9.
+// below which the join costs more than it saves. us by graph replay at 2 /
+// 4 / 8 CTAs: 64 x 4 x 128256 f32 99 / 74 / 82, 128 x 7 x 151936 bf16 193 / 121 /
+// 126, 16 trees of 29 nodes x 128256 74 / 48 / 35, 24 masked chains of 5 x 32000
+// 71 / 48 / 41, one chain of 3 x 32000 19.2 / 14.2 / 12.8.
 int cluster_size(int B, int V) {
   int C = 1;
   while (C < kMaxCluster && (C < 4 || static_cast<int64_t>(B) * C * 2 <= 256) && V / (2 * C) >= 2048) C *= 2;
