@@ -234,8 +234,10 @@ class SpeculativeStep:
         B, dev = len(states), target_logits.device
         if tuple(drafts.shape) != (B, self.K) or tuple(target_logits.shape) != (B * (self.K + 1), self.V):
             raise ValueError(f"drafts {tuple(drafts.shape)} and target logits {tuple(target_logits.shape)} for {B} sequences")
-        if draft_logits is not None and tuple(draft_logits.shape) != (B * self.K, self.V):
-            raise ValueError(f"draft logits {tuple(draft_logits.shape)} for {B} sequences of {self.K} drafts")
+        if draft_logits is not None:
+            if len(draft_logits) < B * self.K or draft_logits.shape[-1] != self.V:
+                raise ValueError(f"draft logits {tuple(draft_logits.shape)} for {B} sequences of {self.K} drafts")
+            draft_logits = draft_logits[: B * self.K]
         params = speculative_params(states, self.cutoffs)
         n = torch.full((B,), self.K, dtype=torch.int32, device=dev) if n_draft is None else n_draft
         acc, tok, _, st = self.sampler.specdec_verify_draft(

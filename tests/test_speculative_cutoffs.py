@@ -83,4 +83,7 @@ def test_cutoffs(given):
         step.draft([engine.SequenceState(seq_id=1, max_tokens=2, repeat_penalty=1.2)], rows[1][:1])
     with pytest.raises(ValueError, match="draft logits"):
         step.verify(states, rows[0], drafts, rows[1][:-1])
+    if not given:  # rows behind the last sequence's are not looked at
+        acc, tok = step.verify(states, rows[0], drafts, torch.cat([rows[1], torch.full((2, V), float("nan"), device=dev)]))
+        assert tuple(tok.shape) == (B, K + 1) and (acc >= 0).all()
     step.close()
